@@ -405,6 +405,115 @@ int sl_debug_set_spin_limit(sl_engine* e, unsigned rounds);
 int sl_debug_set_flow_counter(sl_engine* e, uint32_t value);
 int sl_debug_flow_tags(uint32_t base, int layer, int stage, int steps, int n_layers, uint32_t* tag16, uint32_t* tag32);
 
+/* ---- paged key/value cache held in 4 bits (no counterpart in the reference, whose caches are fp16 arenas) --------------
+ * Operators on device memory for caches of any number of sequences: page tables and slots from request lengths
+ * (sl_kv4_plan), norm and rotation of queries and keys together with the quantised store of keys and values
+ * (sl_kv4_append), attention over the pages (sl_kv4_attention), rows back as values (sl_kv4_read).  sl_set_kv4 puts an
+ * engine's attention layers on them.
+ *
+ * They only enqueue on `stream` (a hipStream_t of the current device, NULL = the default stream): no allocation, no
+ * copy, no synchronisation, so they can be captured into a graph; like sl_head_argmax_noalloc they stand outside the
+ * process-wide lock.  Every pointer inside the argument structs is device memory, of which a call reads nothing but
+ * what it names and writes nothing but its outputs; outputs must not overlap inputs or each other.  Lengths, tables and slots
+ * are read on the device and checked there: what they say can make a call leave rows out, never reach out of bounds.
+ * Returns SL_OK, SL_ERR_ARG, SL_ERR_TOO_LARGE (a size beyond the stated limits), SL_ERR_UNSUPPORTED (head_dim,
+ * page_size) or SL_ERR_DEVICE (the launch failed).
+ *
+ * A page holds page_size tokens of every key/value head; per head, one part behind the other:
+ *   key codes    [page_size][4][head_dim/64][8 bytes]     token, quarter of a group of 64 dims, group: 16 dims
+ *   key s|b      [page_size][head_dim/64] words           scale (low half) and bias (high half), fp16
+ *   value codes  [page_size/8][16][8][head_dim/32 bytes]  block of 8 tokens, sixteenth of the dims, token: head_dim/16 dims
+ *   value s|b    [page_size][head_dim/64] words
+ * low nibble first: the orders in which the matrix instructions take them.  A value is scale * code + bias with the
+ * scales of the checkpoint's rule (group 64: the edge of larger magnitude is represented exactly, the scale is negative
+ * where that is the largest value); the codes are chosen for the stored fp16 scale and bias, in double precision.
+ * Values beyond +-65504 are stored as that; a group with a value that is not finite reads back as NaN. */
+typedef struct {
+  void* pages;              /* [n_pages][sl_kv4_page_bytes()], 16-byte aligned */
+  int32_t n_pages;          /* n_pages * page_size < 2^31 */
+  int32_t page_size;        /* 16, 32, 64, 128 or 256 tokens */
+  int32_t n_kv;             /* key/value heads, 1..1024 */
+  int32_t head_dim;         /* 64, 128 or 256 */
+} sl_kv4_pool;
+/* Element types of rows that go in and come out. */
+#define SL_F16  0
+#define SL_BF16 1
+#define SL_F32  2
+/* page_size * n_kv * 9/8 * head_dim; 0 for a layout that is not supported. */
+int64_t sl_kv4_page_bytes(int page_size, int n_kv, int head_dim);
+
+/* Page tables, slots and row offsets for one step, from the requests' lengths.  Request r keeps ctx_len[r] tokens and
+ * gets new_len[r] more, for which it needs ceil((ctx_len + new_len) / page_size) pages.  Pages it holds beyond that
+ * (a request that ended or was cut back) go onto the free list, in the requests' order; missing pages come off the
+ * end of that list, in the requests' order.  The free list is free_in[0 .. free_count); its length n_free is the most it can hold.
+ * A request that does not get its pages, whose rows do not fit max_tokens, or whose numbers make no sense (negative,
+ * more pages than table_width, fewer held than ctx_len needs) is not served: it keeps what it holds, kv_len 0, slots -1
+ * (its rows then read no key and write none), counted in `unserved`; after the first request that finds too few pages no
+ * later one gets new pages.  Outputs are written whole: -1 behind the used entries of table_out and free_out, slot -1 and
+ * pos 0 behind the last row.  n_req <= 4096, n_req * table_width < 2^31. */
+typedef struct {
+  int32_t n_req, table_width, n_free, page_size, max_tokens;
+  const int32_t* ctx_len;        /* [n_req] */
+  const int32_t* new_len;        /* [n_req] */
+  const int32_t* table_in;       /* [n_req, table_width] page ids, held_in[r] of them used */
+  const int32_t* held_in;        /* [n_req] */
+  const int32_t* free_in;        /* [n_free] */
+  const int32_t* free_count_in;  /* [1] */
+  int32_t* table_out;            /* [n_req, table_width] */
+  int32_t* held_out;             /* [n_req] */
+  int32_t* free_out;             /* [n_free] */
+  int32_t* free_count_out;       /* [1] */
+  int32_t* q_start;              /* [n_req + 1] first row of each request, then the number of rows */
+  int32_t* kv_len;               /* [n_req] tokens in the cache once the new ones are stored */
+  int32_t* slot;                 /* [max_tokens] page * page_size + offset of each row's token, or -1 */
+  int32_t* pos;                  /* [max_tokens] its position in its sequence */
+  int32_t* unserved;             /* [1] */
+} sl_kv4_plan_args;
+int sl_kv4_plan(const sl_kv4_plan_args* a, void* stream);
+
+/* Norm of queries and keys per head (x / sqrt(mean(x^2) + eps) * weight; a NULL weight leaves that norm out), rotation of
+ * the pairs (i, i + rot_dim/2) of the first rot_dim dims by the angle tables' row of the token's position, queries to
+ * q_out, keys and the values as they are into the cache at `slot`.  Queries are computed in fp32 and rounded once, keys
+ * in double precision up to their codes.  A token whose slot is outside the pool stores nothing (its query row is
+ * written); one whose position is outside the tables stores nothing and its query row is zeros.  The slots of
+ * one call must differ: of two tokens with one slot each head's row may mix both.  q == NULL: keys and values only. */
+typedef struct {
+  int32_t n_tokens, n_heads, rot_dim, max_pos, dtype, reserved;   /* rot_dim: 0 or a multiple of 8 up to head_dim; dtype SL_F16 or SL_BF16 */
+  double eps;
+  const void *q, *k, *v, *q_weight, *k_weight;
+  const float *cos, *sin;                     /* [max_pos, rot_dim/2], 16-byte aligned */
+  const int32_t *slot, *pos;                  /* [n_tokens] */
+  void* q_out;
+  /* strides in elements, from token to token and head to head; multiples of 4 as the addresses are of 8 bytes; dims side by side */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+} sl_kv4_append_args;
+int sl_kv4_append(const sl_kv4_pool* pool, const sl_kv4_append_args* a, void* stream);
+
+/* out = softmax(scale * q k^T) v [* sigmoid(gate)] per row and head, query head h with key/value head h / (n_heads / n_kv).
+ * Rows q_start[r] .. q_start[r+1] - 1 are request r's last tokens: row i of n sees keys 0 .. kv_len[r] - n + i.  A row
+ * that sees no key is zeros; rows behind q_start[n_req], and rows of a request from max_rows on, are left as they
+ * were.  Keys whose page id lies outside the pool are not there (as if masked); what masked places hold never matters.
+ * Scores, softmax statistics and sums are fp32, the result is rounded once.  max_rows: the most rows of one request;
+ * max_keys: about how many keys the longest request has, by which long axes are split (any value >= 1 gives right
+ * results).  The same inputs give the same bits; how long axes are cut depends on all lengths of the call, so a request's
+ * last bits may differ between batches. */
+typedef struct {
+  int32_t n_req, n_tokens, n_heads, dtype, table_width, max_rows, max_keys;
+  float scale;
+  const void *q, *gate;                       /* gate may be NULL */
+  void* out;
+  int64_t q_token, q_head, gate_token, gate_head, out_token, out_head;   /* in elements, multiples of 8; addresses 16-byte aligned */
+  const int32_t *table, *q_start, *kv_len;    /* [n_req, table_width], [n_req + 1], [n_req] */
+  void* workspace;                            /* 16-byte aligned; its contents mean nothing between calls */
+  int64_t workspace_bytes;                    /* at least sl_kv4_attention_workspace() */
+} sl_kv4_attn_args;
+int64_t sl_kv4_attention_workspace(const sl_kv4_pool* pool, const sl_kv4_attn_args* a);
+int sl_kv4_attention(const sl_kv4_pool* pool, const sl_kv4_attn_args* a, void* stream);
+
+/* Rows of the cache as values scale * code + bias (fp32, rounded to dtype SL_F32 or SL_F16): k_out, v_out [n, n_kv, head_dim],
+ * 16-byte aligned; a slot outside the pool gives zeros.  Either output may be NULL. */
+int sl_kv4_read(const sl_kv4_pool* pool, const int32_t* slots, int n, int dtype, void* k_out, void* v_out, void* stream);
+
 /* Micro-benchmarks of the machine limits that bound the kernels (measurement hooks; no counterpart in the reference).
  * Each runs on the current device's default stream, allocates and frees its own buffers and returns one figure.
  *  sl_ubench_exchange: a chain of `rounds` dependent hand-overs between the 256 resident workgroups of a persistent

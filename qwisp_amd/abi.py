@@ -91,6 +91,34 @@ class BatchSlots(C.Structure):
                 ("release", RELEASE_FN), ("can_admit", CAN_ADMIT_FN)]
 
 
+SL_F16, SL_BF16, SL_F32 = 0, 1, 2
+
+
+def _fields(text):
+    """[("name", type)] of "type name name; type name": i4, i8, f4, f8, p (pointer)"""
+    kinds = {"i4": C.c_int32, "i8": C.c_int64, "f4": C.c_float, "f8": C.c_double, "p": C.c_void_p}
+    return [(name, kinds[part.split()[0]]) for part in text.split(";") for name in part.split()[1:]]
+
+
+class Kv4Pool(C.Structure):
+    _fields_ = _fields("p pages; i4 n_pages page_size n_kv head_dim")
+
+
+class Kv4PlanArgs(C.Structure):
+    _fields_ = _fields("i4 n_req table_width n_free page_size max_tokens; p ctx_len new_len table_in held_in free_in free_count_in "
+                       "table_out held_out free_out free_count_out q_start kv_len slot pos unserved")
+
+
+class Kv4AppendArgs(C.Structure):
+    _fields_ = _fields("i4 n_tokens n_heads rot_dim max_pos dtype reserved; f8 eps; p q k v q_weight k_weight cos sin slot pos q_out; "
+                       "i8 q_token q_head k_token k_head v_token v_head out_token out_head")
+
+
+class Kv4AttnArgs(C.Structure):
+    _fields_ = _fields("i4 n_req n_tokens n_heads dtype table_width max_rows max_keys; f4 scale; p q gate out; "
+                       "i8 q_token q_head gate_token gate_head out_token out_head; p table q_start kv_len workspace; i8 workspace_bytes")
+
+
 def _ptr(t):
     """Address of a numpy array or a torch tensor."""
     if t is None:

@@ -1,0 +1,182 @@
+"""A paged key/value cache held in 4 bits, on torch tensors: the sl_kv4_* operators of include/seedless_hip.h, which says
+what each computes, refuses and leaves alone.
+
+    pool = kv4.new_pool(n_pages, page_size, n_kv, head_dim)
+    step = kv4.plan(ctx_len, new_len, table, held, free, free_count, page_size, max_tokens)     # once per step
+    q = kv4.append(pool, q, k, v, step.slot, step.pos, cos, sin, q_weight, k_weight)            # per attention layer
+    out = kv4.attention(pool, q, step.table, step.q_start, step.kv_len, max_rows=..., max_keys=...)
+
+torch only owns the memory.  Calls enqueue on torch's current stream of the tensors' device and return without waiting;
+they can be captured into a graph.  A call that the library refuses raises SeedlessError, a tensor of the wrong kind
+ValueError; nothing is copied or converted on the way.
+"""
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from . import abi, lib as _lib
+
+_DTYPES = {torch.float16: abi.SL_F16, torch.bfloat16: abi.SL_BF16}
+
+
+class Pool(NamedTuple):
+    """Pages of one layer's cache: `pages` uint8 [n_pages, page_size * n_kv * 9/8 * head_dim]."""
+    pages: torch.Tensor
+    page_size: int
+    n_kv: int
+    head_dim: int
+
+
+class Plan(NamedTuple):
+    table: torch.Tensor        # [n_req, width] page ids, -1 behind the used ones
+    held: torch.Tensor         # [n_req] pages that each request holds
+    free: torch.Tensor         # [n_free] free pages, -1 behind them
+    free_count: torch.Tensor   # [1]
+    q_start: torch.Tensor      # [n_req + 1] first row of each request
+    kv_len: torch.Tensor       # [n_req] tokens in the cache once the new ones are stored; 0: not served
+    slot: torch.Tensor         # [max_tokens] where each row's token goes, or -1
+    pos: torch.Tensor          # [max_tokens] its position
+    unserved: torch.Tensor     # [1] requests that did not get their pages
+
+
+def page_bytes(page_size, n_kv, head_dim):
+    n = _lib.get().dll.sl_kv4_page_bytes(page_size, n_kv, head_dim)
+    if not n:
+        raise ValueError(f"no such layout: pages of {page_size} tokens, {n_kv} heads of {head_dim} dims")
+    return n
+
+
+def new_pool(n_pages, page_size, n_kv, head_dim, device="cuda"):
+    return Pool(torch.empty(n_pages, page_bytes(page_size, n_kv, head_dim), dtype=torch.uint8, device=device), page_size, n_kv, head_dim)
+
+
+def rope_tables(max_pos, rot_dim, theta=1e7, device="cuda"):
+    """cos and sin [max_pos, rot_dim/2] of pos * theta^(-2i/rot_dim); angles in double precision, so that far positions
+    keep theirs."""
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    angle = torch.arange(max_pos, dtype=torch.float64)[:, None] * torch.exp(i * (-2.0 / rot_dim) * torch.log(torch.tensor(theta, dtype=torch.float64)))
+    return angle.cos().float().to(device), angle.sin().float().to(device)
+
+
+def _flat(t, shape, dtype, device, what):
+    if t.dtype is not dtype or t.device != device or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: {dtype} {list(shape)} side by side on {device} is wanted, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(t, shape, dtype, device, what):
+    """Address and strides of [tokens, heads, dims] with the dims side by side."""
+    if t.dtype is not dtype or t.device != device or t.shape != shape or t.stride(2) != 1:
+        raise ValueError(f"{what}: {dtype} {list(shape)} with dims side by side on {device} is wanted, got {t.dtype} {list(t.shape)} "
+                         f"with strides {t.stride()} on {t.device}")
+    return t.data_ptr(), t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
+
+
+def _pool(pool):
+    p = pool.pages
+    if p.dtype is not torch.uint8 or not p.is_cuda or p.dim() != 2 or not p.is_contiguous() or p.shape[1] != page_bytes(*pool[1:]):
+        raise ValueError(f"pages: uint8 [n_pages, {page_bytes(*pool[1:])}] side by side on a GPU is wanted, got {p.dtype} {list(p.shape)} on {p.device}")
+    return abi.Kv4Pool(p.data_ptr(), p.shape[0], *pool[1:])
+
+
+def _call(name, device, *args):
+    """The library's call on torch's current stream of `device`, with that device current."""
+    fn = getattr(_lib.get().dll, name)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.Library.check(status, name)
+
+
+def plan(ctx_len, new_len, table, held, free, free_count, page_size, max_tokens, out=None):
+    """sl_kv4_plan: page tables, slots and row offsets of one step from the requests' lengths (int32 tensors).  `out`: a
+    Plan whose tensors are written, none of which may be an input."""
+    dev, i32 = ctx_len.device, torch.int32
+    if not ctx_len.is_cuda or ctx_len.dim() != 1 or table.dim() != 2 or free.dim() != 1:
+        raise ValueError("lengths [n_req], table [n_req, width] and free [n_free] on a GPU are wanted")
+    n, width, n_free = ctx_len.shape[0], table.shape[1], free.shape[0]
+    shapes = ((n, width), (n,), (n_free,), (1,), (n + 1,), (n,), (max_tokens,), (max_tokens,), (1,))
+    if out is None:
+        out = Plan(*(torch.empty(s, dtype=i32, device=dev) for s in shapes))
+    ins = [_flat(t, s, i32, dev, w) for t, s, w in ((ctx_len, (n,), "ctx_len"), (new_len, (n,), "new_len"), (table, (n, width), "table"),
+                                                    (held, (n,), "held"), (free, (n_free,), "free"), (free_count, (1,), "free_count"))]
+    outs = [_flat(t, s, i32, dev, "out." + w) for t, s, w in zip(out, shapes, Plan._fields)]
+    _call("sl_kv4_plan", dev, abi.Kv4PlanArgs(n, width, n_free, page_size, max_tokens, *ins, *outs))
+    return out
+
+
+def append(pool, q, k, v, slot, pos, cos, sin, q_weight, k_weight, eps=1e-6, out=None):
+    """sl_kv4_append: queries normed and rotated are returned, keys normed and rotated and values go into the pool.  q None:
+    keys and values only; cos and sin None: no rotation; a weight None: no norm."""
+    p, dev = _pool(pool), pool.pages.device
+    if k.dtype not in _DTYPES or k.dim() != 3:
+        raise ValueError(f"keys [tokens, heads, dims] in float16 or bfloat16 are wanted, got {k.dtype} {list(k.shape)}")
+    dt, n, dim = k.dtype, k.shape[0], pool.head_dim
+    a = abi.Kv4AppendArgs(n_tokens=n, dtype=_DTYPES[dt], eps=eps, slot=_flat(slot, (n,), torch.int32, dev, "slot"))
+    a.k, a.k_token, a.k_head = _rows(k, (n, pool.n_kv, dim), dt, dev, "k")
+    a.v, a.v_token, a.v_head = _rows(v, (n, pool.n_kv, dim), dt, dev, "v")
+    if q is not None:
+        shape = (n, q.shape[1], dim)
+        if out is None:
+            out = torch.empty(shape, dtype=dt, device=dev)
+        a.n_heads = q.shape[1]
+        a.q, a.q_token, a.q_head = _rows(q, shape, dt, dev, "q")
+        a.q_out, a.out_token, a.out_head = _rows(out, shape, dt, dev, "out")
+        if q_weight is not None:
+            a.q_weight = _flat(q_weight, (dim,), dt, dev, "q_weight")
+    if k_weight is not None:
+        a.k_weight = _flat(k_weight, (dim,), dt, dev, "k_weight")
+    if cos is not None:
+        a.max_pos, a.rot_dim = cos.shape[0], 2 * cos.shape[1]
+        a.cos, a.sin = _flat(cos, cos.shape, torch.float32, dev, "cos"), _flat(sin, cos.shape, torch.float32, dev, "sin")
+        a.pos = _flat(pos, (n,), torch.int32, dev, "pos")
+    _call("sl_kv4_append", dev, p, a)
+    return out
+
+
+def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, gate=None, out=None, workspace=None):
+    """sl_kv4_attention: q [tokens, heads, dims] against the pages of each request; `workspace` (uint8, of at least
+    attention_workspace() bytes) is taken from torch if it is not given."""
+    p, dev = _pool(pool), pool.pages.device
+    if q.dtype not in _DTYPES or q.dim() != 3 or table.dim() != 2:
+        raise ValueError(f"queries [tokens, heads, dims] in float16 or bfloat16 and a table [n_req, width] are wanted, got {q.dtype} {list(q.shape)}, {list(table.shape)}")
+    n, heads, n_req, dim = q.shape[0], q.shape[1], table.shape[0], pool.head_dim
+    shape, dt = (n, heads, dim), q.dtype
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=dev)
+    a = abi.Kv4AttnArgs(n_req, n, heads, _DTYPES[dt], table.shape[1], max_rows, max_keys, dim ** -0.5 if scale is None else scale)
+    a.q, a.q_token, a.q_head = _rows(q, shape, dt, dev, "q")
+    a.out, a.out_token, a.out_head = _rows(out, shape, dt, dev, "out")
+    if gate is not None:
+        a.gate, a.gate_token, a.gate_head = _rows(gate, shape, dt, dev, "gate")
+    a.table = _flat(table, table.shape, torch.int32, dev, "table")
+    a.q_start = _flat(q_start, (n_req + 1,), torch.int32, dev, "q_start")
+    a.kv_len = _flat(kv_len, (n_req,), torch.int32, dev, "kv_len")
+    need = _lib.get().dll.sl_kv4_attention_workspace(p, a)
+    if need > 0:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.dtype is not torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("workspace: uint8 side by side on the pool's device is wanted")
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _call("sl_kv4_attention", dev, p, a)
+    return out
+
+
+def attention_workspace(pool, n_tokens, n_heads, n_req, max_rows, max_keys):
+    """Bytes of workspace that attention() takes for such a call."""
+    return _lib.get().dll.sl_kv4_attention_workspace(_pool(pool), abi.Kv4AttnArgs(n_req=n_req, n_tokens=n_tokens, n_heads=n_heads, max_rows=max_rows, max_keys=max_keys))
+
+
+def read(pool, slots, dtype=torch.float32):
+    """sl_kv4_read: keys and values [n, n_kv, head_dim] (float32 or float16) of the given slots."""
+    p, dev = _pool(pool), pool.pages.device
+    if slots.dim() != 1 or dtype not in (torch.float32, torch.float16):
+        raise ValueError("slots [n] and float32 or float16 values are wanted")
+    n = slots.shape[0]
+    k, v = (torch.empty(n, pool.n_kv, pool.head_dim, dtype=dtype, device=dev) for _ in range(2))
+    _call("sl_kv4_read", dev, p, _flat(slots, (n,), torch.int32, dev, "slots"), n, abi.SL_F32 if dtype is torch.float32 else abi.SL_F16, k.data_ptr(), v.data_ptr())
+    return k, v

@@ -71,6 +71,12 @@ SIGNATURES = {
     "sl_debug_set_spin_limit": (_i32, [_vp, C.c_uint32]),
     "sl_debug_set_flow_counter": (_i32, [_vp, C.c_uint32]),
     "sl_debug_flow_tags": (_i32, [C.c_uint32, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "sl_kv4_page_bytes": (_i64, [_i32, _i32, _i32]),
+    "sl_kv4_plan": (_i32, [C.POINTER(abi.Kv4PlanArgs), _vp]),
+    "sl_kv4_append": (_i32, [C.POINTER(abi.Kv4Pool), C.POINTER(abi.Kv4AppendArgs), _vp]),
+    "sl_kv4_attention_workspace": (_i64, [C.POINTER(abi.Kv4Pool), C.POINTER(abi.Kv4AttnArgs)]),
+    "sl_kv4_attention": (_i32, [C.POINTER(abi.Kv4Pool), C.POINTER(abi.Kv4AttnArgs), _vp]),
+    "sl_kv4_read": (_i32, [C.POINTER(abi.Kv4Pool), _vp, _i32, _i32, _vp, _vp, _vp]),
     "sl_ubench_exchange": (_i32, [_i32, _i32, C.POINTER(_f32)]),
     "sl_ubench_gemv_stream": (_i32, [_i32, _i32, C.POINTER(_f32)]),
     "sl_ubench_mfma_issue": (_i32, [_i32, _i32, _i32, C.POINTER(_f32), C.POINTER(_f32)]),
