@@ -426,7 +426,8 @@ int sl_debug_flow_tags(uint32_t base, int layer, int stage, int steps, int n_lay
  *   value s|b    [page_size][head_dim/64] words
  * low nibble first: the orders in which the matrix instructions take them.  A value is scale * code + bias with the
  * scales of the checkpoint's rule (group 64: the edge of larger magnitude is represented exactly, the scale is negative
- * where that is the largest value); the codes are chosen for the stored fp16 scale and bias, in double precision.
+ * where that is the largest value), the step first taken as the range times the double next to 1/15, all in double
+ * precision; the codes are the nearest ones (halfway: the even one) for the stored fp16 scale and bias.
  * Values beyond +-65504 are stored as that; a group with a value that is not finite reads back as NaN. */
 typedef struct {
   void* pages;              /* [n_pages][sl_kv4_page_bytes()], 16-byte aligned */

@@ -6,6 +6,7 @@
 #include "sl_device.cuh"
 #include "../../include/seedless_hip.h"
 #include <algorithm>
+#include <atomic>
 
 using namespace sl;
 
@@ -257,7 +258,7 @@ SL_DEV uint32_t quantise4(const double* v, uint32_t& sb) {
   const unsigned long long bads = __ballot(bad);
   if ((bads >> (threadIdx.x & 48)) & 0xffffull) { sb = 0x7e007e00u; return 0; }
   const bool low = fabs(mn) > fabs(mx);
-  double scale = fmax((mx - mn) / 15.0, 1e-7);
+  double scale = fmax((mx - mn) * (1.0 / 15.0), 1e-7);
   scale = low ? scale : -scale;
   const double edge = low ? mn : mx, steps = rint(edge / scale);
   double bias = 0.0;
@@ -345,55 +346,534 @@ __global__ __launch_bounds__(256) void k_kv4_read(Pool pool, const int32_t* slot
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------------
-// One wave per (row, query head), a key after the other: running maximum m and sum l of the softmax, o rescaled when m
-// moves.
+// Flash attention on the matrix cores (v_mfma_f32_16x16x32_f16), straight from the codes.  A wave takes 32 keys a step and
+// 16 * NT query rows (row = token * group + head within the group):
+//   S[key, row] = sum over groups of 64 dims of  s_g * (sum q c) + b_g * (sum q)      c = code
+//   O[dim, row] += sum over keys of  (p s_g) * (c - 8)  +  p * (b_g + 8 s_g)
+// Codes become fp16 operands without rounding: for the keys a masked nibble IS the fp16 number c * 2^-24 (or c * 2^-20 four
+// bits up, which the query's operand makes good), for the values c - 8 is formed through 1024 + c.  So the scales meet
+// fp32 scores, and the weights p s_g are the only operands that are rounded (11 bits); centred codes keep
+// that rounding at the size of a value's own spread.  Queries become fp16 after a power of two per row that puts the largest
+// near 2^10: exact for both element types but for dims 2^-20 below the row's largest.
+// Layouts: S comes out with a lane holding 8 consecutive keys of one row, which is how the second product wants p, because
+// row m of the two key operands is key 8 (m / 4) + m % 4 (+ 4).  Values are stored as a lane loads them (8 keys x D/16
+// dims) and change lanes through LDS on their way, so that the 16 rows of an operand lie in one group and share p s_g.
+// Each of the four waves of a workgroup takes every fourth step; their sums are joined in LDS at the end.
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int AT_WAVES = 4, AT_STEP = 32, AT_UNIT = AT_WAVES * AT_STEP;   // keys of a workgroup's round
+constexpr int AT_MAX_REQ = 4096;
+
+// How the work of a call is cut.  Few rows (one row tile per request and head): the rounds of all requests and heads, in order,
+// are dealt to the workgroups in equal runs of `share`... of the total over the grid; a run that covers a head's rounds
+// only in part leaves a partial sum (a workgroup has at most two: its first item and its last).  Many rows: a workgroup
+// per (row tile, head, request, split).
+struct AttnCut {
+  int tiles;          // 0: runs of rounds; else row tiles per request
+  int splits;         // parts of the key axis per row tile
+  int rows;           // rows of a partial sum
+  int32_t* first;     // [n_req + 1] rounds before each request (written by the first workgroup, for the merge)
+  float* part;        // partial sums: [slot][rows][D], then [slot][rows] maximum, [slot][rows] sum
+  long slots;
+};
+SL_DEV long seen_keys(const sl_kv4_attn_args& a, const Pool& pool, int r) {
+  const long cap = (long)a.table_width << pool.page_shift;
+  return max(0l, min((long)a.kv_len[r], cap));
+}
+// rows of request r that this call computes
+SL_DEV int rows_of(const sl_kv4_attn_args& a, int r, int& start, int& n) {
+  start = a.q_start[r];
+  n = a.q_start[r + 1] - start;
+  if (start < 0 || n <= 0 || start >= a.n_tokens) return 0;
+  return min(min(n, a.max_rows), a.n_tokens - start);
+}
+SL_DEV int rounds_of(const sl_kv4_attn_args& a, const Pool& pool, int r) {
+  int start, n;
+  if (rows_of(a, r, start, n) <= 0) return 0;
+  return max(1, (int)((seen_keys(a, pool, r) + AT_UNIT - 1) / AT_UNIT));
+}
+
+template <int D, int NT>
+struct AttnLds {
+  static constexpr int G = D / 64;                                    // groups of a row
+  static constexpr int V_STRIDE = 64 * 16 + 16;                       // a group's value pieces
+  static constexpr int SB = 4 * AT_STEP * G * 2;                      // key s, key b, value s [32][G] and value b' [G][32], fp16
+  static constexpr int WAVE = G * V_STRIDE + SB;
+  static constexpr int Q = NT > 1 ? NT * (D / 32) * 64 * 16 : 0;      // query operands in the order of the lanes
+  static constexpr int JOIN = AT_WAVES * 16 * (D + 4) * 4;            // one row tile of every wave
+  static constexpr int MAIN = AT_WAVES * WAVE + Q > JOIN ? AT_WAVES * WAVE + Q : JOIN;
+  static constexpr int STAT = 2 * AT_WAVES * 16 * NT * 4;             // maximum and sum per wave and row
+  static constexpr int BYTES = MAIN + STAT;
+};
+
+SL_DEV float swap16_max(float v) {
+  const unsigned u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+SL_DEV float swap32_max(float v) {
+  const unsigned u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+SL_DEV float rows4_max(float v) { return swap32_max(swap16_max(v)); }     // over the four rows of 16 lanes
+SL_DEV float rows4_sum(float v) { return swap32_sum(swap16_sum(v)); }
+SL_DEV float nth_half(const uint32_t* w, int i) { return i & 1 ? hi_h(w[i / 2]) : lo_h(w[i / 2]); }
+SL_DEV uint32_t half_pair(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
+// Sends what the wave has written to LDS ahead of what it reads there next (its LDS operations stay in order by themselves).
+SL_DEV void wave_lds_order() { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); }
+
+// Raw bytes of a step as the lanes load them.
+template <int D>
+struct KvStep {
+  uint32_t k[2][D / 32];      // two key operands' quarter rows: words [group][2]
+  uint32_t v[D / 16];         // 8 keys x D/32 bytes
+  uint32_t sb[D / 64];        // lanes 0..31: key s|b of key `lane`, lanes 32..63: value s|b of key lane - 32
+  bool there;                 // this lane's s|b key exists
+};
+template <int N>
+SL_DEV void load_words(uint32_t* to, const unsigned char* p) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) { const uint4 x = ld16(p + 4 * i); to[i] = x.x; to[i + 1] = x.y; to[i + 2] = x.z; to[i + 3] = x.w; }
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p); to[0] = x.x; to[1] = x.y;
+  } else to[0] = *reinterpret_cast<const uint32_t*>(p);
+}
+// Page ids for a step's three uses by this lane.
+struct KvPages { int k, v, sb; };
+
+// Normalised, gated, rounded: the last step of a row (sum 0: the row saw no key).
+template <bool BF>
+SL_DEV float finish_value(const sl_kv4_attn_args& a, float y, float sum, uint16_t gate) {
+  y = sum != 0.0f ? y / sum : 0.0f;
+  return a.gate ? y * (1.0f / (1.0f + __builtin_amdgcn_exp2f(-1.44269504088896f * elem_f<BF>(gate)))) : y;
+}
+template <bool BF>
+SL_DEV void finish_row(const sl_kv4_attn_args& a, int t, int head, int d, float4 y, float sum) {
+  uint2 g = make_uint2(0, 0);
+  if (a.gate) g = *reinterpret_cast<const uint2*>((const uint16_t*)a.gate + t * a.gate_token + head * a.gate_head + d);
+  const float x0 = finish_value<BF>(a, y.x, sum, (uint16_t)g.x), x1 = finish_value<BF>(a, y.y, sum, (uint16_t)(g.x >> 16));
+  const float x2 = finish_value<BF>(a, y.z, sum, (uint16_t)g.y), x3 = finish_value<BF>(a, y.w, sum, (uint16_t)(g.y >> 16));
+  *reinterpret_cast<uint2*>((uint16_t*)a.out + t * a.out_token + head * a.out_head + d) =
+      make_uint2((uint32_t)f_elem<BF>(x0) | ((uint32_t)f_elem<BF>(x1) << 16), (uint32_t)f_elem<BF>(x2) | ((uint32_t)f_elem<BF>(x3) << 16));
+}
+template <bool BF>
+SL_DEV void finish_dim(const sl_kv4_attn_args& a, int t, int head, int d, float y, float sum) {
+  const uint16_t g = a.gate ? ((const uint16_t*)a.gate)[t * a.gate_token + head * a.gate_head + d] : (uint16_t)0;
+  ((uint16_t*)a.out)[t * a.out_token + head * a.out_head + d] = f_elem<BF>(finish_value<BF>(a, y, sum, g));
+}
+
+template <int D, bool BF, int NT>
+__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
+  using L = AttnLds<D, NT>;
+  constexpr int G = L::G;
+  extern __shared__ __align__(16) unsigned char lds[];
+  float* s_m = reinterpret_cast<float*>(lds + L::MAIN);
+  float* s_l = s_m + AT_WAVES * 16 * NT;
+  int* s_first = reinterpret_cast<int*>(lds + L::BYTES);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kg = lane >> 4;
+  unsigned char* s_wave = lds + wave * L::WAVE;
+  uint16_t* s_ks = reinterpret_cast<uint16_t*>(s_wave + G * L::V_STRIDE);
+  uint16_t *s_kb = s_ks + AT_STEP * G, *s_vs = s_kb + AT_STEP * G, *s_vb = s_vs + AT_STEP * G;
+  uint4* s_q = reinterpret_cast<uint4*>(lds + AT_WAVES * L::WAVE);
+  const int group = a.n_heads / pool.n_kv, shift = pool.page_shift, page_mask = (1 << shift) - 1;
+  const size_t hb = head_bytes<D>(pool);
+  const int part_c = (D / 2) << shift, part_sb = (D / 16) << shift;
+
+  // ---- this workgroup's run of rounds ----
+  long run0 = 0, run1 = 1;
+  if (cut.tiles == 0) {
+    // rounds before each request, in chunks of a workgroup's threads
+    int carry = 0;
+    for (int base = 0; base < a.n_req; base += 256) {
+      const int r = base + tid;
+      int x = r < a.n_req ? rounds_of(a, pool, r) : 0;
+      const int own = x;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(x, d); if (lane >= d) x += y; }
+      if (lane == 63) reinterpret_cast<int*>(s_m)[wave] = x;
+      __syncthreads();
+      int before = carry, all = 0;
+#pragma unroll
+      for (int w = 0; w < AT_WAVES; ++w) { const int v = reinterpret_cast<int*>(s_m)[w]; if (w < wave) before += v; all += v; }
+      if (r < a.n_req) s_first[r] = before + x - own;
+      carry += all;
+      __syncthreads();
+    }
+    if (tid == 0) s_first[a.n_req] = carry;
+    __syncthreads();
+    if (blockIdx.x == 0) for (int r = tid; r <= a.n_req; r += 256) cut.first[r] = s_first[r];
+    const long total = (long)carry * pool.n_kv, share = (total + gridDim.x - 1) / gridDim.x;
+    run0 = blockIdx.x * share;
+    run1 = min(total, run0 + share);
+  }
+
+  for (long at = run0; at < run1;) {
+    int r, h, tile, round0, round1, start, n;
+    long slot = -1;
+    if (cut.tiles == 0) {
+      r = owner_of(s_first, a.n_req, (int)(at / pool.n_kv));
+      const int rounds = s_first[r + 1] - s_first[r];
+      const long in = at - (long)s_first[r] * pool.n_kv;
+      h = (int)(in / rounds); round0 = (int)(in - (long)h * rounds); round1 = (int)min((long)rounds, round0 + (run1 - at));
+      tile = 0;
+      if (round0 > 0 || round1 < rounds) slot = 2l * blockIdx.x + (at == run0 ? 0 : 1);
+      at += round1 - round0;
+    } else {
+      tile = cut.tiles - 1 - (int)blockIdx.x; h = blockIdx.y; r = blockIdx.z / cut.splits;
+      at = run1;
+    }
+    const int rows = rows_of(a, r, start, n);
+    const int row0 = tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);
+    if (rows_here <= 0) continue;
+    const long keys = seen_keys(a, pool, r);
+    // keys that the tile's last row sees
+    const long last = min(keys, keys - n + (row0 + rows_here - 1) / group + 1);
+    int key0, key1;
+    if (cut.tiles == 0) { key0 = round0 * AT_UNIT; key1 = (int)min((long)round1 * AT_UNIT, max(last, 0l)); }
+    else {
+      const int rounds = (int)((max(last, 0l) + AT_UNIT - 1) / AT_UNIT), split = blockIdx.z % cut.splits;
+      const int per = (rounds + cut.splits - 1) / cut.splits;
+      key0 = split * per * AT_UNIT; key1 = (int)min((long)(split + 1) * per * AT_UNIT, max(last, 0l));
+      if (cut.splits > 1) slot = (((long)r * pool.n_kv + h) * cut.tiles + tile) * cut.splits + split;
+    }
+
+    // ---- queries: operands in fp16, their sums per group, the factor back to scores in units of log2 ----
+    __syncthreads();                                     // (LDS of the item before)
+    h8 q[NT > 1 ? 1 : D / 32];
+    float qsum[NT][G], mul[NT];
+    int limit[NT];                                       // keys that row n16 of tile nt sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + nt * 16 + n16, tok = row / group, head = h * group + (row - tok * group);
+      const bool valid = nt * 16 + n16 < rows_here;
+      limit[nt] = valid ? (int)max(0l, keys - n + tok + 1) : 0x7fffffff;      // (the columns behind the last row are never written)
+      float x[D / 4], top = 0.0f;
+      const uint16_t* src = (const uint16_t*)a.q + (long)(start + (valid ? tok : 0)) * a.q_token + (long)(valid ? head : h * group) * a.q_head + 16 * kg;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint4 w = ld16(src + 64 * g + 8 * c);
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float* y = x + 16 * g + 8 * c + 2 * j;
+            y[0] = valid ? elem_f<BF>((uint16_t)ws[j]) : 0.0f; y[1] = valid ? elem_f<BF>((uint16_t)(ws[j] >> 16)) : 0.0f;
+            top = fmaxf(top, fmaxf(fabsf(y[0]), fabsf(y[1])));
+          }
+        }
+      top = rows4_max(top);
+      const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 100);
+      const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+      mul[nt] = a.scale * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23));
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { x[16 * g + i] = x[16 * g + i] * f; sum = sum + x[16 * g + i]; }
+        qsum[nt][g] = rows4_sum(sum) * 5.9604644775390625e-8f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float* y = x + 16 * g + 8 * c;
+          const uint4 w = make_uint4(half_pair(y[0], y[4]), half_pair(y[1] * 0.0625f, y[5] * 0.0625f), half_pair(y[2], y[6]), half_pair(y[3] * 0.0625f, y[7] * 0.0625f));
+          if constexpr (NT == 1) q[2 * g + c] = __builtin_bit_cast(h8, w);
+          else if (wave == nt % AT_WAVES) s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane] = w;
+        }
+      }
+    }
+    if (NT > 1) __syncthreads();
+
+    f4 o[NT][G][4], ob[NT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = -__builtin_inff(); l[nt] = 0.0f; ob[nt] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][g][i] = f4{0, 0, 0, 0};
+    }
+
+    // ---- keys ----
+    const int32_t* table = a.table + (size_t)r * a.table_width;
+    const int end_page = key1 > 0 ? (key1 - 1) >> shift : 0;
+    auto pages = [&](int k0) {
+      KvPages p;
+      if (shift >= 5) p.k = p.v = p.sb = table[min(k0 >> shift, end_page)];
+      else {
+        p.k = table[min((k0 + 8 * (n16 >> 2)) >> shift, end_page)];
+        p.v = table[min((k0 + 8 * kg) >> shift, end_page)];
+        p.sb = table[min((k0 + (lane & 31)) >> shift, end_page)];
+      }
+      return p;
+    };
+    auto base = [&](int page) { return pool.pages + ((size_t)((unsigned)page < (unsigned)pool.n_pages ? page : 0) * pool.n_kv + h) * hb; };
+    auto load_keys = [&](int k0, const KvPages& p, KvStep<D>& s) {
+      const int ok = (k0 + 8 * (n16 >> 2) + (n16 & 3)) & page_mask;
+      const unsigned char* bk = base(p.k) + ok * (D / 2) + kg * (D / 8);
+      load_words<D / 32>(s.k[0], bk);
+      load_words<D / 32>(s.k[1], bk + 4 * (D / 2));
+    };
+    auto load_rest = [&](int k0, const KvPages& p, KvStep<D>& s) {
+      const int ov = (k0 + 8 * kg) & page_mask, os = (k0 + (lane & 31)) & page_mask;
+      load_words<G>(s.sb, base(p.sb) + (lane < 32 ? part_c : 2 * part_c + part_sb) + os * (D / 16));
+      load_words<D / 16>(s.v, base(p.v) + part_c + part_sb + ((ov >> 3) * 16 + n16) * (D / 4));
+      s.there = (unsigned)p.sb < (unsigned)pool.n_pages && k0 + (lane & 31) < key1;
+    };
+    // A step's registers are loaded again as soon as they have been used: the next values while this step's keys are
+    // multiplied, the next keys while its softmax and its values are.
+    int k0 = key0 + wave * AT_STEP;
+    KvStep<D> cur;
+    KvPages ahead{};
+    if (k0 < key1) { const KvPages p = pages(k0); load_rest(k0, p, cur); load_keys(k0, p, cur); ahead = pages(k0 + AT_UNIT); }
+    for (; k0 < key1; k0 += AT_UNIT) {
+      const bool more = k0 + AT_UNIT < key1;
+      // scales and biases; a key that is not there gets zeros, a value bias that is not finite leaves its NaN to the scale
+      const unsigned there = (unsigned)__ballot(cur.there);
+      {
+        uint16_t sc[G], bi[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t w = cur.there ? cur.sb[g] : 0u;
+          sc[g] = (uint16_t)w; bi[g] = (uint16_t)(w >> 16);
+          if (lane >= 32) {
+            const float b = fmaf(8.0f, h2f(sc[g]), h2f(bi[g]));
+            bi[g] = f2h(b);
+            if ((bi[g] & 0x7c00u) == 0x7c00u) { bi[g] = 0; sc[g] = 0x7e00; }
+          }
+        }
+        wave_lds_order();
+        const int key = lane & 31;
+        uint16_t* to = (lane < 32 ? s_ks : s_vs) + key * G;
+        if constexpr (G == 4) *reinterpret_cast<uint2*>(to) = make_uint2((uint32_t)sc[0] | ((uint32_t)sc[1] << 16), (uint32_t)sc[2] | ((uint32_t)sc[3] << 16));
+        else if constexpr (G == 2) *reinterpret_cast<uint32_t*>(to) = (uint32_t)sc[0] | ((uint32_t)sc[1] << 16);
+        else to[0] = sc[0];
+        if (lane < 32) {
+#pragma unroll
+          for (int g = 0; g < G; ++g) s_kb[key * G + g] = bi[g];
+        } else {
+#pragma unroll
+          for (int g = 0; g < G; ++g) s_vb[g * AT_STEP + key] = bi[g];
+        }
+        // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
+#pragma unroll
+        for (int c = 0; c < G; ++c) {
+          uint32_t x[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if constexpr (G == 4) x[t] = __builtin_amdgcn_perm(cur.v[4 * t + 2 + c / 2], cur.v[4 * t + c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+            else if constexpr (G == 2) x[t] = __builtin_amdgcn_perm(cur.v[2 * t + 1], cur.v[2 * t], c & 1 ? 0x07060302u : 0x05040100u);
+            else x[t] = cur.v[t];
+          }
+          const int to_m = G * (n16 % (16 / G)) + c, to_g = n16 / (16 / G);
+          st16(s_wave + to_g * L::V_STRIDE + (kg * 16 + to_m) * 16, make_uint4(x[0], x[1], x[2], x[3]));
+        }
+        wave_lds_order();
+      }
+      if (more) load_rest(k0 + AT_UNIT, ahead, cur);
+      // scores
+      float s[NT][8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t ks[2 * G], kb[2 * G];
+        load_words<2 * G>(ks, (const unsigned char*)(s_ks + (8 * kg + 4 * i) * G));
+        load_words<2 * G>(kb, (const unsigned char*)(s_kb + (8 * kg + 4 * i) * G));
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            f4 acc[NT];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t w = cur.k[i][2 * g + c], w8 = w >> 8;
+              const h8 kf = __builtin_bit_cast(h8, make_uint4(w & 0x000F000Fu, w & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                h8 qf;
+                if constexpr (NT == 1) qf = q[2 * g + c];
+                else qf = __builtin_bit_cast(h8, s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane]);
+                acc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf, c ? acc[nt] : f4{0, 0, 0, 0}, 0, 0, 0);
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int t = 4 * i + j;
+                const float before = g ? s[nt][t] : 0.0f;
+                s[nt][t] = fmaf(nth_half(kb, j * G + g), qsum[nt][g], fmaf(nth_half(ks, j * G + g), acc[nt][j], before));
+              }
+          }
+      }
+      if (more) { load_keys(k0 + AT_UNIT, ahead, cur); ahead = pages(k0 + 2 * AT_UNIT); }
+      // softmax: in units of log2, the running maximum per row, p relative to it
+      uint32_t pw[NT][G + 1][4];       // operands p s_g, and p itself
+      {
+        uint32_t vs[4 * G];
+        load_words<4 * G>(vs, (const unsigned char*)(s_vs + 8 * kg * G));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          unsigned hidden = 0;         // bit t: this lane's key t is not seen by its row
+          const int first = k0 + 8 * kg;
+          if (there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP)) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) if (!((there >> (8 * kg + t)) & 1u) || first + t >= limit[nt]) hidden |= 1u << t;
+          }
+          float top = m[nt];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            s[nt][t] = (hidden >> t) & 1u ? -__builtin_inff() : s[nt][t] * mul[nt];
+            top = fmaxf(top, s[nt][t]);
+          }
+          top = rows4_max(top);
+          const float ref = top == -__builtin_inff() ? 0.0f : top, back = __builtin_amdgcn_exp2f(m[nt] - ref);
+          if (__any(top != m[nt])) {
+            l[nt] = l[nt] * back; ob[nt] = ob[nt] * back;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
+          }
+          m[nt] = top;
+          float p[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) { p[t] = __builtin_amdgcn_exp2f(s[nt][t] - ref); l[nt] = l[nt] + p[t]; }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) pw[nt][G][t] = half_pair(p[2 * t], p[2 * t + 1]);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const float sa = (hidden >> (2 * t)) & 1u ? 0.0f : nth_half(vs, 2 * t * G + g), sb = (hidden >> (2 * t + 1)) & 1u ? 0.0f : nth_half(vs, (2 * t + 1) * G + g);
+              pw[nt][g][t] = half_pair(p[2 * t] * sa, p[2 * t + 1] * sb);
+            }
+        }
+      }
+      // values
+      {
+        uint4 vb = make_uint4(0, 0, 0, 0);
+        if (n16 < G) vb = *reinterpret_cast<const uint4*>(s_vb + n16 * AT_STEP + 8 * kg);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          ob[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vb), __builtin_bit_cast(h8, make_uint4(pw[nt][G][0], pw[nt][G][1], pw[nt][G][2], pw[nt][G][3])), ob[nt], 0, 0, 0);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint4 raw = ld16(s_wave + g * L::V_STRIDE + lane * 16);
+          const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
+            const h2_t off = i & 1 ? h2_t{(_Float16)-1152.0f, (_Float16)-1152.0f} : h2_t{(_Float16)-1032.0f, (_Float16)-1032.0f};
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const uint32_t y = i & 2 ? x[t] >> 8 : x[t];
+              w[t] = __builtin_bit_cast(uint32_t, as_h2((y & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u) + off);
+            }
+            const h8 vf = __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              o[nt][g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(h8, make_uint4(pw[nt][g][0], pw[nt][g][1], pw[nt][g][2], pw[nt][g][3])), o[nt][g][i], 0, 0, 0);
+          }
+        }
+      }
+    }
+
+    // ---- the four waves' sums together; lane (n16, kg) holds dims 64 g + 16 kg + 4 r + i of row n16 ----
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      l[nt] = rows4_sum(l[nt]);
+      if (kg == 0) { s_m[wave * 16 * NT + nt * 16 + n16] = m[nt]; s_l[wave * 16 * NT + nt * 16 + n16] = l[nt]; }
+    }
+    float* s_o = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      __syncthreads();
+      if (nt * 16 >= rows_here) continue;                // (the same for the whole workgroup)
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int w = 0; w < AT_WAVES; ++w) top = fmaxf(top, s_m[w * 16 * NT + nt * 16 + n16]);
+      const float f = m[nt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - top);
+      float bias[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) bias[g] = __shfl(ob[nt][g], n16);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int rr = 0; rr < 4; ++rr) {
+          float4 y;
+          y.x = (o[nt][g][0][rr] + bias[g]) * f; y.y = fmaf(o[nt][g][1][rr], 0.0625f, bias[g]) * f;
+          y.z = (o[nt][g][2][rr] + bias[g]) * f; y.w = fmaf(o[nt][g][3][rr], 0.0625f, bias[g]) * f;
+          *reinterpret_cast<float4*>(s_o + (wave * 16 + n16) * (D + 4) + 64 * g + 16 * kg + 4 * rr) = y;
+        }
+      __syncthreads();
+      // a thread per four dims of a row
+      for (int i = tid; i < 16 * (D / 4); i += 256) {
+        const int row = i / (D / 4), d = 4 * (i % (D / 4)), in = nt * 16 + row;
+        if (in >= rows_here) break;
+        float4 y = make_float4(0, 0, 0, 0);
+        float best = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < AT_WAVES; ++w) best = fmaxf(best, s_m[w * 16 * NT + in]);
+#pragma unroll
+        for (int w = 0; w < AT_WAVES; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(s_o + (w * 16 + row) * (D + 4) + d);
+          y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+          const float mw = s_m[w * 16 * NT + in];
+          sum += s_l[w * 16 * NT + in] * (mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - best));
+        }
+        if (slot >= 0) {
+          *reinterpret_cast<float4*>(cut.part + (slot * cut.rows + in) * D + d) = y;
+          if (d == 0) {
+            float* stat = cut.part + cut.slots * cut.rows * D;
+            stat[slot * cut.rows + in] = best; stat[(cut.slots + slot) * cut.rows + in] = sum;
+          }
+        } else {
+          const int tok = (row0 + in) / group, head = h * group + (row0 + in - tok * group);
+          finish_row<BF>(a, start + tok, head, d, y, sum);
+        }
+      }
+    }
+  }
+}
+
+// Partial sums of a row joined: a workgroup of one wave per (row, head, request).
 template <int D, bool BF>
-__global__ __launch_bounds__(64) void k_kv4_attn_rows(Pool pool, sl_kv4_attn_args a) {
-  constexpr int PER = D / 64;
-  const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y;
-  if (t >= a.q_start[a.n_req]) return;
-  const int r = owner_of(a.q_start, a.n_req, t), i = t - a.q_start[r], n = a.q_start[r + 1] - a.q_start[r];
-  if (i < 0 || i >= n || i >= a.max_rows) return;
-  const int kvh = h / (a.n_heads / pool.n_kv);
-  const long seen = min((long)a.kv_len[r], (long)a.table_width << pool.page_shift) - n + i + 1;
-  float q[PER], o[PER], m = -__builtin_inff(), sum = 0.0f;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    q[j] = a.scale * elem_f<BF>(((const uint16_t*)a.q)[t * a.q_token + h * a.q_head + lane + 64 * j]);
-    o[j] = 0.0f;
+__global__ __launch_bounds__(64) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut, int main_grid, int tile_rows) {
+  const int row = blockIdx.x, h = blockIdx.y, r = blockIdx.z, lane = threadIdx.x, group = a.n_heads / pool.n_kv;
+  int start, n;
+  const int rows = rows_of(a, r, start, n);
+  if (row >= rows * group) return;
+  long slot0, count, step = 1, first_slot = -1;
+  int in = row;
+  if (cut.tiles == 0) {
+    const long rounds = cut.first[r + 1] - cut.first[r], total = (long)cut.first[a.n_req] * pool.n_kv, share = (total + main_grid - 1) / main_grid;
+    const long begin = (long)cut.first[r] * pool.n_kv + h * rounds, end = begin + rounds, w0 = begin / share, w1 = (end - 1) / share;
+    if (w0 == w1) return;                               // one workgroup had it all and wrote the row
+    slot0 = 2 * w0; count = w1 - w0 + 1; step = 2;
+    if (w0 * share < begin) first_slot = 2 * w0 + 1;    // the item was not that workgroup's first
+  } else {
+    const int tile = row / tile_rows;
+    in = row - tile * tile_rows;
+    slot0 = (((long)r * pool.n_kv + h) * cut.tiles + tile) * cut.splits; count = cut.splits;
   }
-  const int part = (D / 2) << pool.page_shift, sbs = (D / 16) << pool.page_shift;
-  for (long key = 0; key < seen; ++key) {
-    const int page = a.table[(size_t)r * a.table_width + (key >> pool.page_shift)], off = (int)key & ((1 << pool.page_shift) - 1);
-    if (page < 0 || page >= pool.n_pages) continue;
-    const unsigned char* at = head_at<D>(pool, page, kvh);
-    float s = 0.0f;
+  const float* stat = cut.part + cut.slots * cut.rows * D;
+  auto slot_of = [&](long i) { return i == 0 && first_slot >= 0 ? first_slot : slot0 + i * step; };
+  float best = -__builtin_inff();
+  for (long i = lane; i < count; i += 64) best = fmaxf(best, stat[slot_of(i) * cut.rows + in]);
+  best = tree_max<64>(best);
+  float y[D / 64] = {}, sum = 0.0f;
+  for (long i = 0; i < count; ++i) {
+    const long slot = slot_of(i);
+    const float ms = stat[slot * cut.rows + in], f = ms == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ms - best);
+    sum += f * stat[(cut.slots + slot) * cut.rows + in];
+    const float* p = cut.part + (slot * cut.rows + in) * D;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int d = lane + 64 * j;
-      const uint32_t sb = reinterpret_cast<const uint32_t*>(at + part)[off * (D / 64) + j];
-      const uint32_t c = (at[key_codes_at<D>(off, d)] >> (4 * (d & 1))) & 15u;
-      s = fmaf(q[j], fmaf(lo_h(sb), (float)c, hi_h(sb)), s);
-    }
-    s = tree_sum<64>(s);
-    const float top = fmaxf(m, s), back = m == top ? 1.0f : expf(m - top), p = s == top ? 1.0f : expf(s - top);
-    m = top;
-    sum = sum * back + p;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int d = lane + 64 * j;
-      const uint32_t sb = reinterpret_cast<const uint32_t*>(at + part + sbs + part)[off * (D / 64) + j];
-      const uint32_t c = (at[part + sbs + value_codes_at<D>(off, d)] >> (4 * (d & 1))) & 15u;
-      o[j] = fmaf(p, fmaf(lo_h(sb), (float)c, hi_h(sb)), o[j] * back);
-    }
+    for (int j = 0; j < D / 64; ++j) y[j] = fmaf(f, p[lane + 64 * j], y[j]);
   }
+  const int tok = row / group, head = h * group + (row - tok * group);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int d = lane + 64 * j;
-    float y = sum != 0.0f ? o[j] / sum : 0.0f;
-    if (a.gate) y = y * (1.0f / (1.0f + expf(-elem_f<BF>(((const uint16_t*)a.gate)[t * a.gate_token + h * a.gate_head + d]))));
-    ((uint16_t*)a.out)[t * a.out_token + h * a.out_head + d] = f_elem<BF>(y);
-  }
+  for (int j = 0; j < D / 64; ++j) finish_dim<BF>(a, start + tok, head, lane + 64 * j, y[j], sum);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -412,6 +892,66 @@ int pool_of(const sl_kv4_pool* p, Pool& out) {
   if ((int64_t)p->n_pages * p->page_size > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
   out = Pool{(unsigned char*)p->pages, p->n_pages, page_shift_of(p->page_size), p->n_kv};
   return SL_OK;
+}
+// How a call is cut, from what the host knows.
+struct AttnShape {
+  AttnCut cut{};
+  int nt = 1;                 // row tiles of 16 in a workgroup
+  int grid = 0;               // workgroups of runs (cut.tiles == 0)
+  int64_t part_bytes = 0, bytes = 0;
+};
+int compute_units() {         // of the current device
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
+  if (!p || !a || a->n_heads < 1 || p->n_kv < 1 || a->n_heads % p->n_kv || a->n_req < 1 || a->max_rows < 1 || !layout_ok(p->page_size, p->n_kv, p->head_dim)) return SL_ERR_ARG;
+  const int64_t group = a->n_heads / p->n_kv, rows = (int64_t)std::min(a->max_rows, std::max(a->n_tokens, 1)) * group;
+  const int64_t widest = (int64_t)a->table_width * p->page_size;
+  if (a->n_req > AT_MAX_REQ || a->n_heads > 65535 || rows > (1ll << 30) || widest > 0x7fffffffLL - 4096 ||
+      a->n_req * (widest / AT_UNIT + 2) * p->n_kv > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
+  const int cus = compute_units();
+  sh.nt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+  const int tile = 16 * sh.nt;
+  if (rows <= tile) {
+    const int64_t rounds = a->n_req * (std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1) * p->n_kv;
+    sh.grid = (int)std::min<int64_t>(rounds, cus * (sh.nt == 1 ? 2 : 1));
+    sh.cut.slots = 2ll * sh.grid; sh.cut.rows = (int)rows; sh.cut.splits = 1;
+  } else {
+    sh.cut.tiles = (int)((rows + tile - 1) / tile);
+    const int64_t items = (int64_t)sh.cut.tiles * p->n_kv * a->n_req;
+    const int64_t rounds = std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1;
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(items, 1), rounds / 4));
+    splits = std::min<int64_t>(splits, std::max<int64_t>(1, 65535 / a->n_req));
+    sh.cut.splits = (int)splits; sh.cut.rows = tile; sh.cut.slots = splits > 1 ? items * splits : 0;
+  }
+  sh.part_bytes = sh.cut.slots * sh.cut.rows * (p->head_dim + 2) * 4;
+  sh.part_bytes = (sh.part_bytes + 15) & ~15ll;
+  sh.bytes = sh.part_bytes + ((a->n_req + 1) * 4 + 15) / 16 * 16;
+  return SL_OK;
+}
+template <int D, bool BF, int NT>
+void launch_attn_nt(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, const AttnShape& sh, hipStream_t st) {
+  const int lds = AttnLds<D, NT>::BYTES + (cut.tiles ? 0 : (a.n_req + 1) * 4);
+  if (lds > 65536) (void)hipFuncSetAttribute((const void*)k_kv4_attn<D, BF, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  const dim3 grid = cut.tiles ? dim3(cut.tiles, pool.n_kv, a.n_req * cut.splits) : dim3(sh.grid);
+  hipLaunchKernelGGL((k_kv4_attn<D, BF, NT>), grid, dim3(256), lds, st, pool, a, cut);
+}
+template <int D, bool BF>
+void launch_attn(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, const AttnShape& sh, hipStream_t st) {
+  if (sh.nt == 1) launch_attn_nt<D, BF, 1>(pool, a, cut, sh, st);
+  else if (sh.nt == 2) launch_attn_nt<D, BF, 2>(pool, a, cut, sh, st);
+  else launch_attn_nt<D, BF, 4>(pool, a, cut, sh, st);
+  if (cut.slots == 0) return;
+  const int rows = cut.tiles ? cut.tiles * cut.rows : cut.rows;
+  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(64), 0, st, pool, a, cut, sh.grid, cut.rows);
 }
 // f<D, BF>() for the pool's head_dim and an element type
 #define KV4_BY_LAYOUT(dim, bf, CALL)                                        \
@@ -472,8 +1012,8 @@ int sl_kv4_append(const sl_kv4_pool* p, const sl_kv4_append_args* a, void* strea
 }
 
 int64_t sl_kv4_attention_workspace(const sl_kv4_pool* p, const sl_kv4_attn_args* a) {
-  (void)p; (void)a;
-  return 0;
+  AttnShape sh;
+  return attn_shape(p, a, sh) == SL_OK ? sh.bytes : 0;
 }
 
 int sl_kv4_attention(const sl_kv4_pool* p, const sl_kv4_attn_args* a, void* stream) {
@@ -482,14 +1022,19 @@ int sl_kv4_attention(const sl_kv4_pool* p, const sl_kv4_attn_args* a, void* stre
   if (!a || a->n_req < 0 || a->n_tokens < 0 || a->table_width < 0 || (a->dtype != SL_F16 && a->dtype != SL_BF16)) return SL_ERR_ARG;
   if (a->n_heads < 1 || a->n_heads % p->n_kv || a->max_rows < 0 || a->max_keys < 1) return SL_ERR_ARG;
   if (a->n_req == 0 || a->n_tokens == 0 || a->max_rows == 0) return SL_OK;
-  if (!a->q || !a->out || !a->table || !a->q_start || !a->kv_len) return SL_ERR_ARG;
+  if (!a->q || !a->out || !a->q_start || !a->kv_len || (!a->table && a->table_width > 0)) return SL_ERR_ARG;
   const void* sixteen[] = {a->q, a->gate, a->out};
   for (const void* x : sixteen) if (!aligned(x, 16)) return SL_ERR_ARG;
   const int64_t strides[] = {a->q_token, a->q_head, a->out_token, a->out_head, a->gate ? a->gate_token : 0, a->gate ? a->gate_head : 0};
   for (int64_t x : strides) if (x % 8) return SL_ERR_ARG;
-  if (a->n_heads > 65535) return SL_ERR_TOO_LARGE;
+  AttnShape sh;
+  r = attn_shape(p, a, sh); if (r) return r;
+  if (!a->workspace || !aligned(a->workspace, 16) || a->workspace_bytes < sh.bytes) return SL_ERR_ARG;
+  AttnCut cut = sh.cut;
+  cut.part = (float*)a->workspace;
+  cut.first = (int32_t*)((unsigned char*)a->workspace + sh.part_bytes);
   (void)hipGetLastError();
-#define KV4_CALL(D, BF) hipLaunchKernelGGL((k_kv4_attn_rows<D, BF>), dim3(a->n_tokens, a->n_heads), dim3(64), 0, (hipStream_t)stream, pool, *a)
+#define KV4_CALL(D, BF) launch_attn<D, BF>(pool, *a, cut, sh, (hipStream_t)stream)
   KV4_BY_LAYOUT(p->head_dim, a->dtype == SL_BF16, KV4_CALL);
 #undef KV4_CALL
   return launch_status();

@@ -58,7 +58,7 @@ def quantise(x):
     g = np.clip(np.where(bad[..., None], 0.0, g), -65504, 65504)
     mn, mx = g.min(-1), g.max(-1)
     low = np.abs(mn) > np.abs(mx)
-    scale = np.maximum((mx - mn) / 15, 1e-7) * np.where(low, 1, -1)
+    scale = np.maximum((mx - mn) * (1 / 15), 1e-7) * np.where(low, 1, -1)      # the range times the double next to 1/15
     edge = np.where(low, mn, mx)
     n = np.rint(edge / scale)
     scale = np.where(n != 0, edge / np.where(n != 0, n, 1), scale).astype(np.float32).astype(np.float16).astype(np.float64)

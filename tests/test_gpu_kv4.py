@@ -132,6 +132,24 @@ def test_append(dim, dtype, heads, kv, page, rot, tokens, norm):
             assert np.array_equal(np.where(ok[:, None, None], val, 0), g.cpu().numpy(), equal_nan=True), (name, dt_out)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_groups_of_equal_edges_and_values_between_two_codes(dtype):
+    """Largest = -smallest leaves the edge 7.5 steps away, and short numbers fall halfway between two codes: the side that the
+    stated arithmetic takes."""
+    m, rng = kv4(), np.random.default_rng(21)
+    edge = rng.integers(1, 256, (600, 1, 1)) / 2.0 ** rng.integers(0, 9, (600, 1, 1))
+    x = np.rint(rng.uniform(-1, 1, (600, 1, 64)) * 16) / 16 * edge
+    x[:, :, 3], x[:, :, 60] = edge[..., 0], -edge[..., 0]
+    x[300:, :, 60] *= rng.choice([0.5, 0.875, 1.0, 0.25], (300, 1))
+    v = gpu(x, DTYPES[dtype])
+    pool = fresh(rng, 10, 64, 1, 64)
+    m.append(pool, None, v, v, gpu(np.arange(600, dtype=np.int32)), None, None, None, None, None)
+    have, want = ref.unpack(pool.pages.cpu().numpy(), 64, 1, 64), ref.quantise(f64(v))
+    for name in "kv":
+        for key in want:
+            assert np.array_equal(have[name][key][:600], want[key]), (name, key)
+
+
 def test_append_of_keys_and_values_alone():
     m, rng = kv4(), np.random.default_rng(3)
     pool, twin = (m.Pool(torch.zeros(4, m.page_bytes(16, 2, 128), dtype=torch.uint8, device="cuda"), 16, 2, 128) for _ in range(2))
