@@ -400,10 +400,10 @@ struct AttnLds {
   static constexpr int V_STRIDE = 64 * 16 + 16;                       // a group's value pieces
   static constexpr int SB = 4 * AT_STEP * G * 2;                      // key s, key b, value s [32][G] and value b' [G][32], fp16
   static constexpr int WAVE = G * V_STRIDE + SB;
-  static constexpr int Q = NT > 1 ? NT * (D / 32) * 64 * 16 : 0;      // query operands in the order of the lanes
+  static constexpr int Q = NT * (D / 32) * 64 * 16;                   // query operands in the order of the lanes
   static constexpr int JOIN = AT_WAVES * 16 * (D + 4) * 4;            // one row tile of every wave
   static constexpr int MAIN = AT_WAVES * WAVE + Q > JOIN ? AT_WAVES * WAVE + Q : JOIN;
-  static constexpr int STAT = 2 * AT_WAVES * 16 * NT * 4;             // maximum and sum per wave and row
+  static constexpr int STAT = (2 * AT_WAVES + G + 2) * 16 * NT * 4;   // maximum and sum per wave and row; per row sums of q, factor, keys seen
   static constexpr int BYTES = MAIN + STAT;
 };
 
@@ -421,6 +421,7 @@ SL_DEV float rows4_max(float v) { return swap32_max(swap16_max(v)); }     // ove
 SL_DEV float rows4_sum(float v) { return swap32_sum(swap16_sum(v)); }
 SL_DEV float nth_half(const uint32_t* w, int i) { return i & 1 ? hi_h(w[i / 2]) : lo_h(w[i / 2]); }
 SL_DEV uint32_t half_pair(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
+SL_DEV uint32_t pair_of(float a, float b) { return __builtin_bit_cast(uint32_t, h2_t{(_Float16)a, (_Float16)b}); }   // (a product and its rounding may become one instruction)
 // Sends what the wave has written to LDS ahead of what it reads there next (its LDS operations stay in order by themselves).
 SL_DEV void wave_lds_order() { asm volatile("" ::: "memory"); __builtin_amdgcn_wave_barrier(); }
 
@@ -459,19 +460,14 @@ SL_DEV void finish_row(const sl_kv4_attn_args& a, int t, int head, int d, float4
   *reinterpret_cast<uint2*>((uint16_t*)a.out + t * a.out_token + head * a.out_head + d) =
       make_uint2((uint32_t)f_elem<BF>(x0) | ((uint32_t)f_elem<BF>(x1) << 16), (uint32_t)f_elem<BF>(x2) | ((uint32_t)f_elem<BF>(x3) << 16));
 }
-template <bool BF>
-SL_DEV void finish_dim(const sl_kv4_attn_args& a, int t, int head, int d, float y, float sum) {
-  const uint16_t g = a.gate ? ((const uint16_t*)a.gate)[t * a.gate_token + head * a.gate_head + d] : (uint16_t)0;
-  ((uint16_t*)a.out)[t * a.out_token + head * a.out_head + d] = f_elem<BF>(finish_value<BF>(a, y, sum, g));
-}
-
 template <int D, bool BF, int NT>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
+__global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
   using L = AttnLds<D, NT>;
   constexpr int G = L::G;
   extern __shared__ __align__(16) unsigned char lds[];
   float* s_m = reinterpret_cast<float*>(lds + L::MAIN);
-  float* s_l = s_m + AT_WAVES * 16 * NT;
+  float *s_l = s_m + AT_WAVES * 16 * NT, *s_qsum = s_l + AT_WAVES * 16 * NT, *s_mul = s_qsum + G * 16 * NT;
+  int* s_lim = reinterpret_cast<int*>(s_mul + 16 * NT);
   int* s_first = reinterpret_cast<int*>(lds + L::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kg = lane >> 4;
   unsigned char* s_wave = lds + wave * L::WAVE;
@@ -479,7 +475,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
   uint16_t *s_kb = s_ks + AT_STEP * G, *s_vs = s_kb + AT_STEP * G, *s_vb = s_vs + AT_STEP * G;
   uint4* s_q = reinterpret_cast<uint4*>(lds + AT_WAVES * L::WAVE);
   const int group = a.n_heads / pool.n_kv, shift = pool.page_shift, page_mask = (1 << shift) - 1;
-  const size_t hb = head_bytes<D>(pool);
+  const uint32_t page_stride = (uint32_t)(pool.n_kv * (int)head_bytes<D>(pool));
   const int part_c = (D / 2) << shift, part_sb = (D / 16) << shift;
 
   // ---- this workgroup's run of rounds ----
@@ -540,64 +536,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
       if (cut.splits > 1) slot = (((long)r * pool.n_kv + h) * cut.tiles + tile) * cut.splits + split;
     }
 
-    // ---- queries: operands in fp16, their sums per group, the factor back to scores in units of log2 ----
-    __syncthreads();                                     // (LDS of the item before)
-    h8 q[NT > 1 ? 1 : D / 32];
-    float qsum[NT][G], mul[NT];
-    int limit[NT];                                       // keys that row n16 of tile nt sees
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int row = row0 + nt * 16 + n16, tok = row / group, head = h * group + (row - tok * group);
-      const bool valid = nt * 16 + n16 < rows_here;
-      limit[nt] = valid ? (int)max(0l, keys - n + tok + 1) : 0x7fffffff;      // (the columns behind the last row are never written)
-      float x[D / 4], top = 0.0f;
-      const uint16_t* src = (const uint16_t*)a.q + (long)(start + (valid ? tok : 0)) * a.q_token + (long)(valid ? head : h * group) * a.q_head + 16 * kg;
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint4 w = ld16(src + 64 * g + 8 * c);
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float* y = x + 16 * g + 8 * c + 2 * j;
-            y[0] = valid ? elem_f<BF>((uint16_t)ws[j]) : 0.0f; y[1] = valid ? elem_f<BF>((uint16_t)(ws[j] >> 16)) : 0.0f;
-            top = fmaxf(top, fmaxf(fabsf(y[0]), fabsf(y[1])));
-          }
-        }
-      top = rows4_max(top);
-      const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 100);
-      const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
-      mul[nt] = a.scale * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23));
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { x[16 * g + i] = x[16 * g + i] * f; sum = sum + x[16 * g + i]; }
-        qsum[nt][g] = rows4_sum(sum) * 5.9604644775390625e-8f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float* y = x + 16 * g + 8 * c;
-          const uint4 w = make_uint4(half_pair(y[0], y[4]), half_pair(y[1] * 0.0625f, y[5] * 0.0625f), half_pair(y[2], y[6]), half_pair(y[3] * 0.0625f, y[7] * 0.0625f));
-          if constexpr (NT == 1) q[2 * g + c] = __builtin_bit_cast(h8, w);
-          else if (wave == nt % AT_WAVES) s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane] = w;
-        }
-      }
-    }
-    if (NT > 1) __syncthreads();
-
-    f4 o[NT][G][4], ob[NT];
-    float m[NT], l[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = -__builtin_inff(); l[nt] = 0.0f; ob[nt] = f4{0, 0, 0, 0};
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[nt][g][i] = f4{0, 0, 0, 0};
-    }
-
-    // ---- keys ----
+    // ---- the first step's bytes are asked for before anything else ----
     const int32_t* table = a.table + (size_t)r * a.table_width;
     const int end_page = key1 > 0 ? (key1 - 1) >> shift : 0;
     auto pages = [&](int k0) {
@@ -610,7 +549,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
       }
       return p;
     };
-    auto base = [&](int page) { return pool.pages + ((size_t)((unsigned)page < (unsigned)pool.n_pages ? page : 0) * pool.n_kv + h) * hb; };
+    const unsigned char* head_base = pool.pages + (size_t)h * head_bytes<D>(pool);
+    auto base = [&](int page) { return head_base + (uint64_t)((unsigned)page < (unsigned)pool.n_pages ? (uint32_t)page : 0u) * page_stride; };
     auto load_keys = [&](int k0, const KvPages& p, KvStep<D>& s) {
       const int ok = (k0 + 8 * (n16 >> 2) + (n16 & 3)) & page_mask;
       const unsigned char* bk = base(p.k) + ok * (D / 2) + kg * (D / 8);
@@ -628,7 +568,84 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
     int k0 = key0 + wave * AT_STEP;
     KvStep<D> cur;
     KvPages ahead{};
-    if (k0 < key1) { const KvPages p = pages(k0); load_rest(k0, p, cur); load_keys(k0, p, cur); ahead = pages(k0 + AT_UNIT); }
+    if (k0 < key1) { const KvPages p = pages(k0); ahead = pages(k0 + AT_UNIT); load_rest(k0, p, cur); load_keys(k0, p, cur); }
+
+    // ---- queries: operands in fp16, their sums per group, the factor back to scores in units of log2; 16 lanes a row ----
+    __syncthreads();                                     // (LDS of the item before)
+#pragma unroll
+    for (int pass = 0; pass < NT; ++pass) {
+      constexpr int PER = D / 16;                        // dims of a lane
+      const int in = pass * 16 + (tid >> 4), l16 = tid & 15, row = row0 + in, tok = row / group, head = h * group + (row - tok * group);
+      if (in - (in & 15) >= rows_here && pass > 0) break;        // (operands of an empty tile are not used)
+      const bool valid = in < rows_here;
+      float x[PER], top = 0.0f;
+      const uint16_t* src = (const uint16_t*)a.q + (long)(start + (valid ? tok : 0)) * a.q_token + (long)(valid ? head : h * group) * a.q_head + PER * l16;
+#pragma unroll
+      for (int c = 0; c < PER / 4; ++c) {
+        load4<BF>(src + 4 * c, x + 4 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[4 * c + j] = valid ? x[4 * c + j] : 0.0f; top = fmaxf(top, fabsf(x[4 * c + j])); }
+      }
+      top = fmaxf(top, dpp_f<DPP_XOR1>(top)); top = fmaxf(top, dpp_f<DPP_XOR2>(top));
+      top = fmaxf(top, dpp_f<DPP_HALF_MIRROR>(top)); top = fmaxf(top, dpp_f<DPP_MIRROR>(top));
+      const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 100);
+      const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) { x[i] = x[i] * f; sum = sum + x[i]; }
+      sum = tree_sum<16 / G>(sum) * 5.9604644775390625e-8f;
+      if (l16 % (16 / G) == 0) s_qsum[in * G + l16 / (16 / G)] = sum;
+      if (l16 == 0) {
+        s_mul[in] = a.scale * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23));
+        s_lim[in] = valid ? (int)max(0l, keys - n + tok + 1) : 0x7fffffff;      // (the columns behind the last row are never written)
+      }
+      // operand word w of quarter kg in group g: dims 64 g + 16 kg + 8 w + (0 4 | 1 5 | 2 6 | 3 7), the odd ones / 16
+      if constexpr (PER >= 8) {
+#pragma unroll
+        for (int c = 0; c < PER / 8; ++c) {
+          const int d = PER * l16 + 8 * c, to = (pass * (D / 32) + 2 * (d / 64) + (d / 8) % 2) * 64 + (d % 64) / 16 * 16 + (in & 15);
+          const float* y = x + 8 * c;
+          s_q[to] = make_uint4(half_pair(y[0], y[4]), half_pair(y[1] * 0.0625f, y[5] * 0.0625f), half_pair(y[2], y[6]), half_pair(y[3] * 0.0625f, y[7] * 0.0625f));
+        }
+      } else {
+        const int d = 4 * l16, to = (pass * (D / 32) + (d / 8) % 2) * 64 + d / 16 * 16 + (in & 15);
+        uint16_t* w = reinterpret_cast<uint16_t*>(s_q + to) + (l16 & 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[2 * j] = f2h(j & 1 ? x[j] * 0.0625f : x[j]);
+      }
+    }
+    __syncthreads();
+    h8 q[NT > 1 ? 1 : D / 32];
+    float qsum[NT][G], mul[NT];
+    int limit[NT];                                       // keys that row n16 of tile nt sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if constexpr (NT == 1) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) q[i] = __builtin_bit_cast(h8, s_q[i * 64 + lane]);
+      }
+      mul[nt] = s_mul[nt * 16 + n16]; limit[nt] = s_lim[nt * 16 + n16];
+#pragma unroll
+      for (int g = 0; g < G; ++g) qsum[nt][g] = s_qsum[(nt * 16 + n16) * G + g];
+    }
+    const int live = NT == 1 ? 1 : (rows_here + 15) / 16;       // row tiles that have rows
+
+    // 1024 in both halves, kept in a register: with the mask as a scalar, (x & mask) | 1024 is one instruction
+    uint32_t ones = 0x64006400u, mask_lo = 0x000F000Fu, mask_hi = 0x00F000F0u;
+    asm volatile("" : "+v"(ones));
+    asm volatile("" : "+s"(mask_lo), "+s"(mask_hi));
+    f4 o[NT][G][4], ob[NT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = -__builtin_inff(); l[nt] = 0.0f; ob[nt] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][g][i] = f4{0, 0, 0, 0};
+    }
+
+    // ---- keys ----
     for (; k0 < key1; k0 += AT_UNIT) {
       const bool more = k0 + AT_UNIT < key1;
       // scales and biases; a key that is not there gets zeros, a value bias that is not finite leaves its NaN to the scale
@@ -674,37 +691,40 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
         wave_lds_order();
       }
       if (more) load_rest(k0 + AT_UNIT, ahead, cur);
-      // scores
+      // scores: all products of the step first, so that no scale waits for the product before it
       float s[NT][8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t ks[2 * G], kb[2 * G];
-        load_words<2 * G>(ks, (const unsigned char*)(s_ks + (8 * kg + 4 * i) * G));
-        load_words<2 * G>(kb, (const unsigned char*)(s_kb + (8 * kg + 4 * i) * G));
+      for (int nt = 0; nt < NT; ++nt) {
+        if (nt >= live) break;
+        f4 acc[2][G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            f4 acc[NT];
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+          for (int g = 0; g < G; ++g) {
+            h8 qf;
+            if constexpr (NT == 1) qf = q[2 * g + c];
+            else qf = __builtin_bit_cast(h8, s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
               const uint32_t w = cur.k[i][2 * g + c], w8 = w >> 8;
-              const h8 kf = __builtin_bit_cast(h8, make_uint4(w & 0x000F000Fu, w & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                h8 qf;
-                if constexpr (NT == 1) qf = q[2 * g + c];
-                else qf = __builtin_bit_cast(h8, s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane]);
-                acc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf, c ? acc[nt] : f4{0, 0, 0, 0}, 0, 0, 0);
-              }
+              const h8 kf = __builtin_bit_cast(h8, make_uint4(w & mask_lo, w & mask_hi, w8 & mask_lo, w8 & mask_hi));
+              acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf, c ? acc[i][g] : f4{0, 0, 0, 0}, 0, 0, 0);
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int t = 4 * i + j;
-                const float before = g ? s[nt][t] : 0.0f;
-                s[nt][t] = fmaf(nth_half(kb, j * G + g), qsum[nt][g], fmaf(nth_half(ks, j * G + g), acc[nt][j], before));
-              }
           }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t ks[2 * G], kb[2 * G];
+          load_words<2 * G>(ks, (const unsigned char*)(s_ks + (8 * kg + 4 * i) * G));
+          load_words<2 * G>(kb, (const unsigned char*)(s_kb + (8 * kg + 4 * i) * G));
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int t = 4 * i + j;
+              const float before = g ? s[nt][t] : 0.0f;
+              s[nt][t] = fmaf(nth_half(kb, j * G + g), qsum[nt][g], fmaf(nth_half(ks, j * G + g), acc[i][g][j], before));
+            }
+        }
       }
       if (more) { load_keys(k0 + AT_UNIT, ahead, cur); ahead = pages(k0 + 2 * AT_UNIT); }
       // softmax: in units of log2, the running maximum per row, p relative to it
@@ -714,40 +734,47 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
         load_words<4 * G>(vs, (const unsigned char*)(s_vs + 8 * kg * G));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          unsigned hidden = 0;         // bit t: this lane's key t is not seen by its row
-          const int first = k0 + 8 * kg;
-          if (there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP)) {
+          if (nt >= live) break;
+          // only the step at the end of a row's keys, and one with a page that is not there, has keys to hide
+          const bool hides = there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP);
+          uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
 #pragma unroll
-            for (int t = 0; t < 8; ++t) if (!((there >> (8 * kg + t)) & 1u) || first + t >= limit[nt]) hidden |= 1u << t;
+          for (int t = 0; t < 8; ++t) s[nt][t] = s[nt][t] * mul[nt];
+          if (hides) {
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) { s[nt][t] = -__builtin_inff(); keep[t / 2] &= t & 1 ? 0x0000ffffu : 0xffff0000u; }
           }
           float top = m[nt];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            s[nt][t] = (hidden >> t) & 1u ? -__builtin_inff() : s[nt][t] * mul[nt];
-            top = fmaxf(top, s[nt][t]);
-          }
+          for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t]);
           top = rows4_max(top);
-          const float ref = top == -__builtin_inff() ? 0.0f : top, back = __builtin_amdgcn_exp2f(m[nt] - ref);
+          const float ref = top == -__builtin_inff() ? 0.0f : top;
           if (__any(top != m[nt])) {
+            const float back = __builtin_amdgcn_exp2f(m[nt] - ref);
             l[nt] = l[nt] * back; ob[nt] = ob[nt] * back;
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
               for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
+            m[nt] = top;
           }
-          m[nt] = top;
           float p[8];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) { p[t] = __builtin_amdgcn_exp2f(s[nt][t] - ref); l[nt] = l[nt] + p[t]; }
+          for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(s[nt][t] - ref);
+          l[nt] = l[nt] + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
 #pragma unroll
-          for (int t = 0; t < 4; ++t) pw[nt][G][t] = half_pair(p[2 * t], p[2 * t + 1]);
+          for (int t = 0; t < 4; ++t) pw[nt][G][t] = pair_of(p[2 * t], p[2 * t + 1]);
 #pragma unroll
           for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const float sa = (hidden >> (2 * t)) & 1u ? 0.0f : nth_half(vs, 2 * t * G + g), sb = (hidden >> (2 * t + 1)) & 1u ? 0.0f : nth_half(vs, (2 * t + 1) * G + g);
-              pw[nt][g][t] = half_pair(p[2 * t] * sa, p[2 * t + 1] * sb);
-            }
+            for (int t = 0; t < 4; ++t) pw[nt][g][t] = pair_of(fmaf(p[2 * t], nth_half(vs, 2 * t * G + g), 0.0f), fmaf(p[2 * t + 1], nth_half(vs, (2 * t + 1) * G + g), 0.0f));   // (fma: takes the half as it is)
+          if (hides) {                 // a hidden key's scale may be NaN
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+              for (int t = 0; t < 4; ++t) pw[nt][g][t] &= keep[t];
+          }
         }
       }
       // values
@@ -768,7 +795,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
               const uint32_t y = i & 2 ? x[t] >> 8 : x[t];
-              w[t] = __builtin_bit_cast(uint32_t, as_h2((y & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u) + off);
+              w[t] = __builtin_bit_cast(uint32_t, as_h2((y & (i & 1 ? mask_hi : mask_lo)) | ones) + off);
             }
             const h8 vf = __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
@@ -837,10 +864,15 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void k_kv4_attn(Pool pool, sl
   }
 }
 
-// Partial sums of a row joined: a workgroup of one wave per (row, head, request).
+// Partial sums of a row joined: a workgroup per (row, head, request).  A wave reads 256 / D partial rows at once, 16 bytes a
+// lane, four such loads in flight; the waves' sums meet in LDS.
 template <int D, bool BF>
-__global__ __launch_bounds__(64) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut, int main_grid, int tile_rows) {
-  const int row = blockIdx.x, h = blockIdx.y, r = blockIdx.z, lane = threadIdx.x, group = a.n_heads / pool.n_kv;
+__global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut, int main_grid, int tile_rows) {
+  constexpr int LANES = D / 4, PER_WAVE = 64 / LANES, PER = 4 * PER_WAVE;
+  __shared__ float s_red[4];
+  __shared__ float4 s_y[PER][LANES];
+  __shared__ float s_sum[PER];
+  const int row = blockIdx.x, h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.n_heads / pool.n_kv;
   int start, n;
   const int rows = rows_of(a, r, start, n);
   if (row >= rows * group) return;
@@ -860,20 +892,45 @@ __global__ __launch_bounds__(64) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_ar
   const float* stat = cut.part + cut.slots * cut.rows * D;
   auto slot_of = [&](long i) { return i == 0 && first_slot >= 0 ? first_slot : slot0 + i * step; };
   float best = -__builtin_inff();
-  for (long i = lane; i < count; i += 64) best = fmaxf(best, stat[slot_of(i) * cut.rows + in]);
+  for (long i = tid; i < count; i += 256) best = fmaxf(best, stat[slot_of(i) * cut.rows + in]);
   best = tree_max<64>(best);
-  float y[D / 64] = {}, sum = 0.0f;
-  for (long i = 0; i < count; ++i) {
-    const long slot = slot_of(i);
-    const float ms = stat[slot * cut.rows + in], f = ms == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ms - best);
-    sum += f * stat[(cut.slots + slot) * cut.rows + in];
-    const float* p = cut.part + (slot * cut.rows + in) * D;
+  if (lane == 0) s_red[wave] = best;
+  const int d = 4 * (lane % LANES), mine = wave * PER_WAVE + lane / LANES;
+  float4 y = make_float4(0, 0, 0, 0);
+  float sum = 0.0f;
+  __syncthreads();
+  best = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  for (long i = mine; i < count; i += 4 * PER) {
+    float4 p[4];
+    float m[4], l[4];
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) y[j] = fmaf(f, p[lane + 64 * j], y[j]);
+    for (int u = 0; u < 4; ++u) {
+      const bool in_range = i + u * PER < count;
+      const long slot = slot_of(in_range ? i + u * PER : i);
+      p[u] = *reinterpret_cast<const float4*>(cut.part + (slot * cut.rows + in) * D + d);
+      m[u] = in_range ? stat[slot * cut.rows + in] : -__builtin_inff();
+      l[u] = stat[(cut.slots + slot) * cut.rows + in];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (m[u] == -__builtin_inff()) continue;           // (a part in which the row sees no key)
+      const float f = __builtin_amdgcn_exp2f(m[u] - best);
+      sum = fmaf(f, l[u], sum);
+      y.x = fmaf(f, p[u].x, y.x); y.y = fmaf(f, p[u].y, y.y); y.z = fmaf(f, p[u].z, y.z); y.w = fmaf(f, p[u].w, y.w);
+    }
   }
-  const int tok = row / group, head = h * group + (row - tok * group);
+  s_y[mine][lane % LANES] = y;
+  if (lane % LANES == 0) s_sum[mine] = sum;
+  __syncthreads();
+  if (tid >= LANES) return;
+  sum = 0.0f; y = make_float4(0, 0, 0, 0);
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j) finish_dim<BF>(a, start + tok, head, lane + 64 * j, y[j], sum);
+  for (int i = 0; i < PER; ++i) {
+    const float4 x = s_y[i][tid];
+    sum += s_sum[i]; y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+  }
+  const int tok = row / group;
+  finish_row<BF>(a, start + tok, h * group + (row - tok * group), 4 * tid, y, sum);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -951,7 +1008,7 @@ void launch_attn(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut
   else launch_attn_nt<D, BF, 4>(pool, a, cut, sh, st);
   if (cut.slots == 0) return;
   const int rows = cut.tiles ? cut.tiles * cut.rows : cut.rows;
-  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(64), 0, st, pool, a, cut, sh.grid, cut.rows);
+  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut, sh.grid, cut.rows);
 }
 // f<D, BF>() for the pool's head_dim and an element type
 #define KV4_BY_LAYOUT(dim, bf, CALL)                                        \
