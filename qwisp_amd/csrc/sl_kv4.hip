@@ -365,17 +365,17 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr int AT_WAVES = 4, AT_STEP = 32, AT_UNIT = AT_WAVES * AT_STEP;   // keys of a workgroup's round
 constexpr int AT_MAX_REQ = 4096;
 
-// How the work of a call is cut.  Few rows (one row tile per request and head): the rounds of all requests and heads, in order,
-// are dealt to the workgroups in equal runs of `share`... of the total over the grid; a run that covers a head's rounds
-// only in part leaves a partial sum (a workgroup has at most two: its first item and its last).  Many rows: a workgroup
-// per (row tile, head, request, split).
+// How the work of a call is cut.  An item is a row tile of a request and a key/value head; its rounds of 128 keys are shared
+// out to ceil(rounds / share) workgroups, share = rounds of the whole call over `want` workgroups.  So every workgroup has one
+// part of one item: runs of equal length across items would need fewer workgroups, but one that ends an item and begins
+// another pays the start and the end twice, and the call waits for it (32 lanes: 47 us where the others end at 35).
+// The host launches want + items workgroups, which is enough whatever the lengths are; those behind the last part leave at once.
 struct AttnCut {
-  int tiles;          // 0: runs of rounds; else row tiles per request
-  int splits;         // parts of the key axis per row tile
+  int want;           // workgroups to share the rounds out to
   int rows;           // rows of a partial sum
-  int32_t* first;     // [n_req + 1] rounds before each request (written by the first workgroup, for the merge)
-  float* part;        // partial sums: [slot][rows][D], then [slot][rows] maximum, [slot][rows] sum
-  long slots;
+  int32_t* first;     // [n_req + 1] parts before each request, then share (written by the first workgroup, for the merge)
+  float* part;        // partial sums by workgroup: [grid][rows][D], then maxima [grid][rows], sums [grid][rows]
+  long slots;         // = grid
 };
 SL_DEV long seen_keys(const sl_kv4_attn_args& a, const Pool& pool, int r) {
   const long cap = (long)a.table_width << pool.page_shift;
@@ -389,9 +389,88 @@ SL_DEV int rows_of(const sl_kv4_attn_args& a, int r, int& start, int& n) {
   return min(min(n, a.max_rows), a.n_tokens - start);
 }
 SL_DEV int rounds_of(const sl_kv4_attn_args& a, const Pool& pool, int r) {
-  int start, n;
-  if (rows_of(a, r, start, n) <= 0) return 0;
   return max(1, (int)((seen_keys(a, pool, r) + AT_UNIT - 1) / AT_UNIT));
+}
+// rounds of a part: total / want, rounded up (a quotient of doubles is exact where it is whole)
+SL_DEV int share_of(long total, int want) { return max(1, (int)fmin(ceil((double)total / (double)want), 2147483647.0)); }
+SL_DEV int parts_of(int rounds, int share) { return (int)(((unsigned)rounds + (unsigned)share - 1u) / (unsigned)share); }
+struct AttnPart { int r, tile, h, part, parts, share, rounds; };
+// The part that workgroup `idx` has; false if there is none.  Up to 64 requests: every wave finds it by itself, a request
+// per lane; more: the workgroup with running sums in LDS (s_first: n_req + 1 words, s_tmp: 12 words).
+template <int TILE>
+SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut& cut, int idx, int* s_first, int* s_tmp, AttnPart& out) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.n_heads / pool.n_kv, n = a.n_req;
+  auto of = [&](int r, int& items, int& rounds) {
+    int start, nn;
+    const int rows = rows_of(a, r, start, nn);
+    items = rows > 0 ? (rows * group + TILE - 1) / TILE * pool.n_kv : 0;
+    rounds = rows > 0 ? rounds_of(a, pool, r) : 0;
+  };
+  int before, items, rounds, share;
+  if (n <= 64) {
+    items = rounds = 0;
+    if (lane < n) of(lane, items, rounds);
+    long total = (long)items * rounds;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    share = share_of(total, cut.want);
+    const int own = items * parts_of(rounds, share);
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; }
+    if (idx == 0 && wave == 0) {
+      if (lane < n) cut.first[lane] = upto - own;
+      if (lane == 63) { cut.first[n] = upto; cut.first[n + 1] = share; }
+    }
+    const int r = __popcll(__ballot(upto <= idx));
+    if (r >= n) return false;                      // (lanes behind n hold the total as well)
+    out.r = r;
+    before = __builtin_amdgcn_readlane(upto - own, r); items = __builtin_amdgcn_readlane(items, r); rounds = __builtin_amdgcn_readlane(rounds, r);
+  } else {
+    const int per = (n + 255) / 256;
+    long total = 0;
+    for (int j = 0; j < per; ++j) {
+      const int r = tid * per + j;
+      if (r < n) { of(r, items, rounds); total += (long)items * rounds; }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    long* s_total = reinterpret_cast<long*>(s_tmp);
+    if (lane == 0) s_total[wave] = total;
+    __syncthreads();
+    total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
+    share = share_of(total, cut.want);
+    int own = 0;
+    for (int j = 0; j < per; ++j) {
+      const int r = tid * per + j;
+      if (r < n) { of(r, items, rounds); own += items * parts_of(rounds, share); }
+    }
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; }
+    if (lane == 63) s_tmp[8 + wave] = upto;
+    __syncthreads();
+    int at = upto - own, all = 0;
+#pragma unroll
+    for (int w = 0; w < AT_WAVES; ++w) { if (w < wave) at += s_tmp[8 + w]; all += s_tmp[8 + w]; }
+    for (int j = 0; j < per; ++j) {
+      const int r = tid * per + j;
+      if (r < n) { of(r, items, rounds); s_first[r] = at; at += items * parts_of(rounds, share); }
+    }
+    if (tid == 0) s_first[n] = all;
+    __syncthreads();
+    if (idx == 0) for (int i = tid; i <= n + 1; i += 256) cut.first[i] = i <= n ? s_first[i] : share;
+    if (idx >= all) return false;
+    out.r = __builtin_amdgcn_readfirstlane(owner_of(s_first, n, idx));
+    before = s_first[out.r];
+    of(out.r, items, rounds);
+  }
+  out.share = share; out.rounds = rounds;
+  out.parts = parts_of(rounds, share);
+  const int in = idx - before, item = in / out.parts;
+  out.part = in - item * out.parts;
+  out.tile = item / pool.n_kv; out.h = item - out.tile * pool.n_kv;
+  return true;
 }
 
 template <int D, int NT>
@@ -478,65 +557,17 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
   const uint32_t page_stride = (uint32_t)(pool.n_kv * (int)head_bytes<D>(pool));
   const int part_c = (D / 2) << shift, part_sb = (D / 16) << shift;
 
-  // ---- this workgroup's run of rounds ----
-  long run0 = 0, run1 = 1;
-  if (cut.tiles == 0) {
-    // rounds before each request, in chunks of a workgroup's threads
-    int carry = 0;
-    for (int base = 0; base < a.n_req; base += 256) {
-      const int r = base + tid;
-      int x = r < a.n_req ? rounds_of(a, pool, r) : 0;
-      const int own = x;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(x, d); if (lane >= d) x += y; }
-      if (lane == 63) reinterpret_cast<int*>(s_m)[wave] = x;
-      __syncthreads();
-      int before = carry, all = 0;
-#pragma unroll
-      for (int w = 0; w < AT_WAVES; ++w) { const int v = reinterpret_cast<int*>(s_m)[w]; if (w < wave) before += v; all += v; }
-      if (r < a.n_req) s_first[r] = before + x - own;
-      carry += all;
-      __syncthreads();
-    }
-    if (tid == 0) s_first[a.n_req] = carry;
-    __syncthreads();
-    if (blockIdx.x == 0) for (int r = tid; r <= a.n_req; r += 256) cut.first[r] = s_first[r];
-    const long total = (long)carry * pool.n_kv, share = (total + gridDim.x - 1) / gridDim.x;
-    run0 = blockIdx.x * share;
-    run1 = min(total, run0 + share);
-  }
-
-  for (long at = run0; at < run1;) {
-    int r, h, tile, round0, round1, start, n;
-    long slot = -1;
-    if (cut.tiles == 0) {
-      r = owner_of(s_first, a.n_req, (int)(at / pool.n_kv));
-      const int rounds = s_first[r + 1] - s_first[r];
-      const long in = at - (long)s_first[r] * pool.n_kv;
-      h = (int)(in / rounds); round0 = (int)(in - (long)h * rounds); round1 = (int)min((long)rounds, round0 + (run1 - at));
-      tile = 0;
-      if (round0 > 0 || round1 < rounds) slot = 2l * blockIdx.x + (at == run0 ? 0 : 1);
-      at += round1 - round0;
-    } else {
-      tile = cut.tiles - 1 - (int)blockIdx.x; h = blockIdx.y; r = blockIdx.z / cut.splits;
-      at = run1;
-    }
-    const int rows = rows_of(a, r, start, n);
-    const int row0 = tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);
-    if (rows_here <= 0) continue;
-    const long keys = seen_keys(a, pool, r);
+  AttnPart at;
+  if (!find_part<16 * NT>(a, pool, cut, blockIdx.x, s_first, reinterpret_cast<int*>(s_m), at)) return;
+  {
+    const int r = at.r, h = at.h;
+    int start, n;
+    const int rows = rows_of(a, r, start, n), row0 = at.tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);
+    const long keys = seen_keys(a, pool, r), slot = at.parts > 1 ? (long)blockIdx.x : -1;
     // keys that the tile's last row sees
-    const long last = min(keys, keys - n + (row0 + rows_here - 1) / group + 1);
-    int key0, key1;
-    if (cut.tiles == 0) { key0 = round0 * AT_UNIT; key1 = (int)min((long)round1 * AT_UNIT, max(last, 0l)); }
-    else {
-      const int rounds = (int)((max(last, 0l) + AT_UNIT - 1) / AT_UNIT), split = blockIdx.z % cut.splits;
-      const int per = (rounds + cut.splits - 1) / cut.splits;
-      key0 = split * per * AT_UNIT; key1 = (int)min((long)(split + 1) * per * AT_UNIT, max(last, 0l));
-      if (cut.splits > 1) slot = (((long)r * pool.n_kv + h) * cut.tiles + tile) * cut.splits + split;
-    }
+    const long last = max(0l, min(keys, keys - n + (row0 + rows_here - 1) / group + 1));
+    const int key0 = at.part * at.share * AT_UNIT, key1 = (int)min((long)min(at.rounds, (at.part + 1) * at.share) * AT_UNIT, last);
 
-    // ---- the first step's bytes are asked for before anything else ----
     const int32_t* table = a.table + (size_t)r * a.table_width;
     const int end_page = key1 > 0 ? (key1 - 1) >> shift : 0;
     auto pages = [&](int k0) {
@@ -568,23 +599,31 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
     int k0 = key0 + wave * AT_STEP;
     KvStep<D> cur;
     KvPages ahead{};
-    if (k0 < key1) { const KvPages p = pages(k0); ahead = pages(k0 + AT_UNIT); load_rest(k0, p, cur); load_keys(k0, p, cur); }
-
-    // ---- queries: operands in fp16, their sums per group, the factor back to scores in units of log2; 16 lanes a row ----
-    __syncthreads();                                     // (LDS of the item before)
+    // Queries are asked for first, then the first step's bytes, which are on their way while the queries are laid out.
+    constexpr int QPER = D / 16;                         // 16 lanes a row
+    uint2 raw[NT][QPER / 4];
 #pragma unroll
     for (int pass = 0; pass < NT; ++pass) {
-      constexpr int PER = D / 16;                        // dims of a lane
-      const int in = pass * 16 + (tid >> 4), l16 = tid & 15, row = row0 + in, tok = row / group, head = h * group + (row - tok * group);
-      if (in - (in & 15) >= rows_here && pass > 0) break;        // (operands of an empty tile are not used)
+      const int in = pass * 16 + (tid >> 4), row = row0 + (in < rows_here ? in : 0), tok = row / group, head = h * group + (row - tok * group);
+      const uint16_t* src = (const uint16_t*)a.q + (long)(start + tok) * a.q_token + (long)head * a.q_head + QPER * (tid & 15);
+#pragma unroll
+      for (int c = 0; c < QPER / 4; ++c) raw[pass][c] = *reinterpret_cast<const uint2*>(src + 4 * c);
+    }
+    if (k0 < key1) { const KvPages p = pages(k0); ahead = pages(k0 + AT_UNIT); load_rest(k0, p, cur); load_keys(k0, p, cur); }
+
+    // ---- queries: operands in fp16, their sums per group, the factor back to scores in units of log2 ----
+#pragma unroll
+    for (int pass = 0; pass < NT; ++pass) {
+      constexpr int PER = QPER;
+      const int in = pass * 16 + (tid >> 4), l16 = tid & 15, row = row0 + in, tok = row / group;
+      if (pass * 16 >= rows_here) break;                 // (operands of an empty tile are not used)
       const bool valid = in < rows_here;
       float x[PER], top = 0.0f;
-      const uint16_t* src = (const uint16_t*)a.q + (long)(start + (valid ? tok : 0)) * a.q_token + (long)(valid ? head : h * group) * a.q_head + PER * l16;
 #pragma unroll
       for (int c = 0; c < PER / 4; ++c) {
-        load4<BF>(src + 4 * c, x + 4 * c);
+        const uint16_t e4[4] = {(uint16_t)raw[pass][c].x, (uint16_t)(raw[pass][c].x >> 16), (uint16_t)raw[pass][c].y, (uint16_t)(raw[pass][c].y >> 16)};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { x[4 * c + j] = valid ? x[4 * c + j] : 0.0f; top = fmaxf(top, fabsf(x[4 * c + j])); }
+        for (int j = 0; j < 4; ++j) { x[4 * c + j] = valid ? elem_f<BF>(e4[j]) : 0.0f; top = fmaxf(top, fabsf(x[4 * c + j])); }
       }
       top = fmaxf(top, dpp_f<DPP_XOR1>(top)); top = fmaxf(top, dpp_f<DPP_XOR2>(top));
       top = fmaxf(top, dpp_f<DPP_HALF_MIRROR>(top)); top = fmaxf(top, dpp_f<DPP_MIRROR>(top));
@@ -614,7 +653,7 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
         for (int j = 0; j < 4; ++j) w[2 * j] = f2h(j & 1 ? x[j] * 0.0625f : x[j]);
       }
     }
-    __syncthreads();
+    lds_barrier();
     h8 q[NT > 1 ? 1 : D / 32];
     float qsum[NT][G], mul[NT];
     int limit[NT];                                       // keys that row n16 of tile nt sees
@@ -815,7 +854,7 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
     float* s_o = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      __syncthreads();
+      lds_barrier();
       if (nt * 16 >= rows_here) continue;                // (the same for the whole workgroup)
       float top = -__builtin_inff();
 #pragma unroll
@@ -833,7 +872,7 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
           y.z = (o[nt][g][2][rr] + bias[g]) * f; y.w = fmaf(o[nt][g][3][rr], 0.0625f, bias[g]) * f;
           *reinterpret_cast<float4*>(s_o + (wave * 16 + n16) * (D + 4) + 64 * g + 16 * kg + 4 * rr) = y;
         }
-      __syncthreads();
+      lds_barrier();
       // a thread per four dims of a row
       for (int i = tid; i < 16 * (D / 4); i += 256) {
         const int row = i / (D / 4), d = 4 * (i % (D / 4)), in = nt * 16 + row;
@@ -867,7 +906,7 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
 // Partial sums of a row joined: a workgroup per (row, head, request).  A wave reads 256 / D partial rows at once, 16 bytes a
 // lane, four such loads in flight; the waves' sums meet in LDS.
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut, int main_grid, int tile_rows) {
+__global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut, int tile_rows) {
   constexpr int LANES = D / 4, PER_WAVE = 64 / LANES, PER = 4 * PER_WAVE;
   __shared__ float s_red[4];
   __shared__ float4 s_y[PER][LANES];
@@ -876,23 +915,14 @@ __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_a
   int start, n;
   const int rows = rows_of(a, r, start, n);
   if (row >= rows * group) return;
-  long slot0, count, step = 1, first_slot = -1;
-  int in = row;
-  if (cut.tiles == 0) {
-    const long rounds = cut.first[r + 1] - cut.first[r], total = (long)cut.first[a.n_req] * pool.n_kv, share = (total + main_grid - 1) / main_grid;
-    const long begin = (long)cut.first[r] * pool.n_kv + h * rounds, end = begin + rounds, w0 = begin / share, w1 = (end - 1) / share;
-    if (w0 == w1) return;                               // one workgroup had it all and wrote the row
-    slot0 = 2 * w0; count = w1 - w0 + 1; step = 2;
-    if (w0 * share < begin) first_slot = 2 * w0 + 1;    // the item was not that workgroup's first
-  } else {
-    const int tile = row / tile_rows;
-    in = row - tile * tile_rows;
-    slot0 = (((long)r * pool.n_kv + h) * cut.tiles + tile) * cut.splits; count = cut.splits;
-  }
+  const int tile = row / tile_rows, in = row - tile * tile_rows, share = cut.first[a.n_req + 1];
+  const int count = parts_of(rounds_of(a, pool, r), share);
+  if (count == 1) return;                               // one workgroup had all of it and wrote the row
+  const long slot0 = cut.first[r] + (long)(tile * pool.n_kv + h) * count;
+  if (slot0 + count > cut.slots) return;                // (row offsets that overlap: more parts than rows allow)
   const float* stat = cut.part + cut.slots * cut.rows * D;
-  auto slot_of = [&](long i) { return i == 0 && first_slot >= 0 ? first_slot : slot0 + i * step; };
   float best = -__builtin_inff();
-  for (long i = tid; i < count; i += 256) best = fmaxf(best, stat[slot_of(i) * cut.rows + in]);
+  for (int i = tid; i < count; i += 256) best = fmaxf(best, stat[(slot0 + i) * cut.rows + in]);
   best = tree_max<64>(best);
   if (lane == 0) s_red[wave] = best;
   const int d = 4 * (lane % LANES), mine = wave * PER_WAVE + lane / LANES;
@@ -900,13 +930,13 @@ __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_a
   float sum = 0.0f;
   __syncthreads();
   best = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  for (long i = mine; i < count; i += 4 * PER) {
+  for (int i = mine; i < count; i += 4 * PER) {
     float4 p[4];
     float m[4], l[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const bool in_range = i + u * PER < count;
-      const long slot = slot_of(in_range ? i + u * PER : i);
+      const long slot = slot0 + (in_range ? i + u * PER : i);
       p[u] = *reinterpret_cast<const float4*>(cut.part + (slot * cut.rows + in) * D + d);
       m[u] = in_range ? stat[slot * cut.rows + in] : -__builtin_inff();
       l[u] = stat[(cut.slots + slot) * cut.rows + in];
@@ -954,7 +984,7 @@ int pool_of(const sl_kv4_pool* p, Pool& out) {
 struct AttnShape {
   AttnCut cut{};
   int nt = 1;                 // row tiles of 16 in a workgroup
-  int grid = 0;               // workgroups of runs (cut.tiles == 0)
+  int grid = 0;
   int64_t part_bytes = 0, bytes = 0;
 };
 int compute_units() {         // of the current device
@@ -972,43 +1002,35 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   if (!p || !a || a->n_heads < 1 || p->n_kv < 1 || a->n_heads % p->n_kv || a->n_req < 1 || a->max_rows < 1 || !layout_ok(p->page_size, p->n_kv, p->head_dim)) return SL_ERR_ARG;
   const int64_t group = a->n_heads / p->n_kv, rows = (int64_t)std::min(a->max_rows, std::max(a->n_tokens, 1)) * group;
   const int64_t widest = (int64_t)a->table_width * p->page_size;
-  if (a->n_req > AT_MAX_REQ || a->n_heads > 65535 || rows > (1ll << 30) || widest > 0x7fffffffLL - 4096 ||
-      a->n_req * (widest / AT_UNIT + 2) * p->n_kv > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
-  const int cus = compute_units();
-  sh.nt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+  if (a->n_req > AT_MAX_REQ || a->n_heads > 65535 || rows > (1ll << 30) || widest > 0x7fffffffLL - 4096) return SL_ERR_TOO_LARGE;
+  sh.nt = rows <= 16 ? 1 : 2;
   const int tile = 16 * sh.nt;
-  if (rows <= tile) {
-    const int64_t rounds = a->n_req * (std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1) * p->n_kv;
-    sh.grid = (int)std::min<int64_t>(rounds, cus * (sh.nt == 1 ? 2 : 1));
-    sh.cut.slots = 2ll * sh.grid; sh.cut.rows = (int)rows; sh.cut.splits = 1;
-  } else {
-    sh.cut.tiles = (int)((rows + tile - 1) / tile);
-    const int64_t items = (int64_t)sh.cut.tiles * p->n_kv * a->n_req;
-    const int64_t rounds = std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1;
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>(cus / std::max<int64_t>(items, 1), rounds / 4));
-    splits = std::min<int64_t>(splits, std::max<int64_t>(1, 65535 / a->n_req));
-    sh.cut.splits = (int)splits; sh.cut.rows = tile; sh.cut.slots = splits > 1 ? items * splits : 0;
-  }
+  // items: by the most rows of a request, and by all rows of the call
+  const int64_t items = p->n_kv * std::min(a->n_req * ((rows + tile - 1) / tile), a->n_tokens * group / tile + a->n_req);
+  const int64_t resident = (int64_t)compute_units() * (sh.nt * p->head_dim <= 256 ? 2 : 1);
+  const int64_t rounds = items * (std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1);
+  if (p->n_kv * a->n_req * ((rows + tile - 1) / tile) + resident > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
+  // with few items they and the parts together fill the chip once; more than half the places are shared out in any case
+  sh.cut.want = (int)std::min(std::max(resident - items, resident / 2), std::max<int64_t>(rounds, 1));
+  sh.grid = (int)(sh.cut.want + items);
+  sh.cut.slots = sh.grid; sh.cut.rows = (int)std::min<int64_t>(rows, tile);
   sh.part_bytes = sh.cut.slots * sh.cut.rows * (p->head_dim + 2) * 4;
   sh.part_bytes = (sh.part_bytes + 15) & ~15ll;
-  sh.bytes = sh.part_bytes + ((a->n_req + 1) * 4 + 15) / 16 * 16;
+  sh.bytes = sh.part_bytes + ((a->n_req + 2) * 4 + 15) / 16 * 16;
   return SL_OK;
 }
 template <int D, bool BF, int NT>
 void launch_attn_nt(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, const AttnShape& sh, hipStream_t st) {
-  const int lds = AttnLds<D, NT>::BYTES + (cut.tiles ? 0 : (a.n_req + 1) * 4);
+  const int lds = AttnLds<D, NT>::BYTES + (a.n_req <= 64 ? 0 : (a.n_req + 1) * 4);
   if (lds > 65536) (void)hipFuncSetAttribute((const void*)k_kv4_attn<D, BF, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  const dim3 grid = cut.tiles ? dim3(cut.tiles, pool.n_kv, a.n_req * cut.splits) : dim3(sh.grid);
-  hipLaunchKernelGGL((k_kv4_attn<D, BF, NT>), grid, dim3(256), lds, st, pool, a, cut);
+  hipLaunchKernelGGL((k_kv4_attn<D, BF, NT>), dim3(sh.grid), dim3(256), lds, st, pool, a, cut);
 }
 template <int D, bool BF>
 void launch_attn(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, const AttnShape& sh, hipStream_t st) {
   if (sh.nt == 1) launch_attn_nt<D, BF, 1>(pool, a, cut, sh, st);
-  else if (sh.nt == 2) launch_attn_nt<D, BF, 2>(pool, a, cut, sh, st);
-  else launch_attn_nt<D, BF, 4>(pool, a, cut, sh, st);
-  if (cut.slots == 0) return;
-  const int rows = cut.tiles ? cut.tiles * cut.rows : cut.rows;
-  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut, sh.grid, cut.rows);
+  else launch_attn_nt<D, BF, 2>(pool, a, cut, sh, st);
+  const int rows = std::min(a.max_rows, a.n_tokens) * (a.n_heads / pool.n_kv);
+  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut, 16 * sh.nt);
 }
 // f<D, BF>() for the pool's head_dim and an element type
 #define KV4_BY_LAYOUT(dim, bf, CALL)                                        \
