@@ -7,6 +7,7 @@
 #include "../../include/seedless_hip.h"
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 using namespace sl;
 
@@ -482,7 +483,7 @@ struct AttnLds {
   static constexpr int Q = NT * (D / 32) * 64 * 16;                   // query operands in the order of the lanes
   static constexpr int JOIN = AT_WAVES * 16 * (D + 4) * 4;            // one row tile of every wave
   static constexpr int MAIN = AT_WAVES * WAVE + Q > JOIN ? AT_WAVES * WAVE + Q : JOIN;
-  static constexpr int STAT = (2 * AT_WAVES + G + 2) * 16 * NT * 4;   // maximum and sum per wave and row; per row sums of q, factor, keys seen
+  static constexpr int STAT = (2 * AT_WAVES + 2 + 4) * 16 * NT * 4;   // maximum and sum per wave and row; per row factor, keys seen, sums of q
   static constexpr int BYTES = MAIN + STAT;
 };
 
@@ -545,13 +546,14 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
   constexpr int G = L::G;
   extern __shared__ __align__(16) unsigned char lds[];
   float* s_m = reinterpret_cast<float*>(lds + L::MAIN);
-  float *s_l = s_m + AT_WAVES * 16 * NT, *s_qsum = s_l + AT_WAVES * 16 * NT, *s_mul = s_qsum + G * 16 * NT;
+  float *s_l = s_m + AT_WAVES * 16 * NT, *s_mul = s_l + AT_WAVES * 16 * NT;
   int* s_lim = reinterpret_cast<int*>(s_mul + 16 * NT);
+  uint4* s_qsum = reinterpret_cast<uint4*>(s_lim + 16 * NT);
   int* s_first = reinterpret_cast<int*>(lds + L::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kg = lane >> 4;
   unsigned char* s_wave = lds + wave * L::WAVE;
   uint16_t* s_ks = reinterpret_cast<uint16_t*>(s_wave + G * L::V_STRIDE);
-  uint16_t *s_kb = s_ks + AT_STEP * G, *s_vs = s_kb + AT_STEP * G, *s_vb = s_vs + AT_STEP * G;
+  uint16_t *s_vs = s_ks + AT_STEP * G, *s_kb = s_vs + AT_STEP * G, *s_vb = s_kb + AT_STEP * G;
   uint4* s_q = reinterpret_cast<uint4*>(lds + AT_WAVES * L::WAVE);
   const int group = a.n_heads / pool.n_kv, shift = pool.page_shift, page_mask = (1 << shift) - 1;
   const uint32_t page_stride = (uint32_t)(pool.n_kv * (int)head_bytes<D>(pool));
@@ -628,14 +630,23 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
       top = fmaxf(top, dpp_f<DPP_XOR1>(top)); top = fmaxf(top, dpp_f<DPP_XOR2>(top));
       top = fmaxf(top, dpp_f<DPP_HALF_MIRROR>(top)); top = fmaxf(top, dpp_f<DPP_MIRROR>(top));
       const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 100);
-      const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+      const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f);
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < PER; ++i) { x[i] = x[i] * f; sum = sum + x[i]; }
-      sum = tree_sum<16 / G>(sum) * 5.9604644775390625e-8f;
-      if (l16 % (16 / G) == 0) s_qsum[in * G + l16 / (16 / G)] = sum;
+      sum = tree_sum<16 / G>(sum) * 0.25f;               // at most 64 * 2^11 / 4
+      if (l16 % (16 / G) == 0) {                         // as two halves, behind each other for G > 1: operand [hi of the groups | lo of the groups]
+        uint16_t* w = reinterpret_cast<uint16_t*>(s_qsum + in) + l16 / (16 / G);
+        const uint16_t hi = f2h(sum);
+        w[0] = hi; w[G] = f2h(sum - h2f(hi));
+        if (G < 4) {
+#pragma unroll
+          for (int i = 2; i < 8 / G; ++i) w[i * G] = 0;
+        }
+      }
       if (l16 == 0) {
-        s_mul[in] = a.scale * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23));
+        // (a factor of zero would leave hidden keys without their minus infinity)
+        s_mul[in] = fmaxf(fabsf(a.scale) * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23)), 1e-30f);
         s_lim[in] = valid ? (int)max(0l, keys - n + tok + 1) : 0x7fffffff;      // (the columns behind the last row are never written)
       }
       // operand word w of quarter kg in group g: dims 64 g + 16 kg + 8 w + (0 4 | 1 5 | 2 6 | 3 7), the odd ones / 16
@@ -654,27 +665,27 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
       }
     }
     lds_barrier();
-    h8 q[NT > 1 ? 1 : D / 32];
-    float qsum[NT][G], mul[NT];
+    // (dims of 256 and several row tiles leave no room for the operands in registers)
+    constexpr bool Q_REGS = NT == 1 && D < 256;
+    h8 q[Q_REGS ? D / 32 : 1], qs[NT];
+    float mul[NT];
     int limit[NT];                                       // keys that row n16 of tile nt sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if constexpr (NT == 1) {
+      if constexpr (Q_REGS) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) q[i] = __builtin_bit_cast(h8, s_q[i * 64 + lane]);
       }
       mul[nt] = s_mul[nt * 16 + n16]; limit[nt] = s_lim[nt * 16 + n16];
-#pragma unroll
-      for (int g = 0; g < G; ++g) qsum[nt][g] = s_qsum[(nt * 16 + n16) * G + g];
+      qs[nt] = __builtin_bit_cast(h8, kg == 0 ? s_qsum[nt * 16 + n16] : make_uint4(0, 0, 0, 0));
     }
-    const int live = NT == 1 ? 1 : (rows_here + 15) / 16;       // row tiles that have rows
 
     // 1024 in both halves, kept in a register: with the mask as a scalar, (x & mask) | 1024 is one instruction
     uint32_t ones = 0x64006400u, mask_lo = 0x000F000Fu, mask_hi = 0x00F000F0u;
     asm volatile("" : "+v"(ones));
     asm volatile("" : "+s"(mask_lo), "+s"(mask_hi));
     f4 o[NT][G][4], ob[NT];
-    float m[NT], l[NT];
+    float m[NT], l[NT];                                  // running maximum (of scores before the factor) and this lane's sum of p
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt] = -__builtin_inff(); l[nt] = 0.0f; ob[nt] = f4{0, 0, 0, 0};
@@ -684,144 +695,171 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
         for (int i = 0; i < 4; ++i) o[nt][g][i] = f4{0, 0, 0, 0};
     }
 
-    // ---- keys ----
-    for (; k0 < key1; k0 += AT_UNIT) {
-      const bool more = k0 + AT_UNIT < key1;
-      // scales and biases; a key that is not there gets zeros, a value bias that is not finite leaves its NaN to the scale
-      const unsigned there = (unsigned)__ballot(cur.there);
-      {
-        uint16_t sc[G], bi[G];
+    // ---- keys: a step of 32 for the first LIVE row tiles ----
+    auto keys_loop = [&](auto live_tiles) {
+      constexpr int LIVE = decltype(live_tiles)::value;
+      for (; k0 < key1; k0 += AT_UNIT) {
+        const bool more = k0 + AT_UNIT < key1;
+        // scales and biases; a key that is not there gets zeros.  Value lanes turn b into b + 8 s; one that is not finite
+        // is left to the scale as NaN, which the weights carry only where the key is seen.
+        const unsigned there = (unsigned)__ballot(cur.there);
+        {
+          constexpr int W = (G + 1) / 2;
+          uint32_t sc[W], bi[W];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const uint32_t w = cur.there ? cur.sb[g] : 0u;
-          sc[g] = (uint16_t)w; bi[g] = (uint16_t)(w >> 16);
+          for (int g = 0; g < W; ++g) {
+            const uint32_t w0 = cur.there ? cur.sb[G == 1 ? 0 : 2 * g] : 0u, w1 = G == 1 ? 0u : (cur.there ? cur.sb[G == 1 ? 0 : 2 * g + 1] : 0u);
+            sc[g] = __builtin_amdgcn_perm(w1, w0, 0x05040100u); bi[g] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+          }
+          h2_t odd = {(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+          for (int g = 0; g < W; ++g) {
+            const h2_t eight = {(_Float16)8.0f, (_Float16)8.0f}, zero = {(_Float16)0.0f, (_Float16)0.0f};
+            const h2_t b = __builtin_elementwise_fma(as_h2(sc[g]), eight, as_h2(bi[g]));
+            odd = __builtin_elementwise_fma(b, zero, odd);
+            bi[g] = lane < 32 ? bi[g] : __builtin_bit_cast(uint32_t, b);
+          }
+          const _Float16 none = odd.x + odd.y;
+          if (__any(none != none && lane >= 32)) {
+#pragma unroll
+            for (int g = 0; g < W; ++g)
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                if (lane >= 32 && ((bi[g] >> (16 * u)) & 0x7c00u) == 0x7c00u) { bi[g] &= u ? 0x0000ffffu : 0xffff0000u; sc[g] = (sc[g] & (u ? 0x0000ffffu : 0xffff0000u)) | (0x7e00u << (16 * u)); }
+          }
+          wave_lds_order();
+          if constexpr (G == 4) {
+            *reinterpret_cast<uint2*>(s_ks + lane * G) = make_uint2(sc[0], sc[1]);
+            if (lane < 32) *reinterpret_cast<uint2*>(s_kb + lane * G) = make_uint2(bi[0], bi[1]);
+          } else if constexpr (G == 2) {
+            *reinterpret_cast<uint32_t*>(s_ks + lane * G) = sc[0];
+            if (lane < 32) *reinterpret_cast<uint32_t*>(s_kb + lane * G) = bi[0];
+          } else {
+            s_ks[lane] = (uint16_t)sc[0];
+            if (lane < 32) s_kb[lane] = (uint16_t)bi[0];
+          }
           if (lane >= 32) {
-            const float b = fmaf(8.0f, h2f(sc[g]), h2f(bi[g]));
-            bi[g] = f2h(b);
-            if ((bi[g] & 0x7c00u) == 0x7c00u) { bi[g] = 0; sc[g] = 0x7e00; }
+#pragma unroll
+            for (int g = 0; g < G; ++g) s_vb[g * AT_STEP + (lane & 31)] = (uint16_t)(bi[g / 2] >> (16 * (g & 1)));
           }
-        }
-        wave_lds_order();
-        const int key = lane & 31;
-        uint16_t* to = (lane < 32 ? s_ks : s_vs) + key * G;
-        if constexpr (G == 4) *reinterpret_cast<uint2*>(to) = make_uint2((uint32_t)sc[0] | ((uint32_t)sc[1] << 16), (uint32_t)sc[2] | ((uint32_t)sc[3] << 16));
-        else if constexpr (G == 2) *reinterpret_cast<uint32_t*>(to) = (uint32_t)sc[0] | ((uint32_t)sc[1] << 16);
-        else to[0] = sc[0];
-        if (lane < 32) {
+          // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
 #pragma unroll
-          for (int g = 0; g < G; ++g) s_kb[key * G + g] = bi[g];
-        } else {
+          for (int c = 0; c < G; ++c) {
+            uint32_t x[4];
 #pragma unroll
-          for (int g = 0; g < G; ++g) s_vb[g * AT_STEP + key] = bi[g];
-        }
-        // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
-#pragma unroll
-        for (int c = 0; c < G; ++c) {
-          uint32_t x[4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            if constexpr (G == 4) x[t] = __builtin_amdgcn_perm(cur.v[4 * t + 2 + c / 2], cur.v[4 * t + c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-            else if constexpr (G == 2) x[t] = __builtin_amdgcn_perm(cur.v[2 * t + 1], cur.v[2 * t], c & 1 ? 0x07060302u : 0x05040100u);
-            else x[t] = cur.v[t];
-          }
-          const int to_m = G * (n16 % (16 / G)) + c, to_g = n16 / (16 / G);
-          st16(s_wave + to_g * L::V_STRIDE + (kg * 16 + to_m) * 16, make_uint4(x[0], x[1], x[2], x[3]));
-        }
-        wave_lds_order();
-      }
-      if (more) load_rest(k0 + AT_UNIT, ahead, cur);
-      // scores: all products of the step first, so that no scale waits for the product before it
-      float s[NT][8];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (nt >= live) break;
-        f4 acc[2][G];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            h8 qf;
-            if constexpr (NT == 1) qf = q[2 * g + c];
-            else qf = __builtin_bit_cast(h8, s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t w = cur.k[i][2 * g + c], w8 = w >> 8;
-              const h8 kf = __builtin_bit_cast(h8, make_uint4(w & mask_lo, w & mask_hi, w8 & mask_lo, w8 & mask_hi));
-              acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf, c ? acc[i][g] : f4{0, 0, 0, 0}, 0, 0, 0);
+            for (int t = 0; t < 4; ++t) {
+              if constexpr (G == 4) x[t] = __builtin_amdgcn_perm(cur.v[4 * t + 2 + c / 2], cur.v[4 * t + c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+              else if constexpr (G == 2) x[t] = __builtin_amdgcn_perm(cur.v[2 * t + 1], cur.v[2 * t], c & 1 ? 0x07060302u : 0x05040100u);
+              else x[t] = cur.v[t];
             }
+            const int to_m = G * (n16 % (16 / G)) + c, to_g = n16 / (16 / G);
+            st16(s_wave + to_g * L::V_STRIDE + (kg * 16 + to_m) * 16, make_uint4(x[0], x[1], x[2], x[3]));
           }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t ks[2 * G], kb[2 * G];
-          load_words<2 * G>(ks, (const unsigned char*)(s_ks + (8 * kg + 4 * i) * G));
-          load_words<2 * G>(kb, (const unsigned char*)(s_kb + (8 * kg + 4 * i) * G));
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int t = 4 * i + j;
-              const float before = g ? s[nt][t] : 0.0f;
-              s[nt][t] = fmaf(nth_half(kb, j * G + g), qsum[nt][g], fmaf(nth_half(ks, j * G + g), acc[i][g][j], before));
-            }
+          wave_lds_order();
         }
-      }
-      if (more) { load_keys(k0 + AT_UNIT, ahead, cur); ahead = pages(k0 + 2 * AT_UNIT); }
-      // softmax: in units of log2, the running maximum per row, p relative to it
-      uint32_t pw[NT][G + 1][4];       // operands p s_g, and p itself
-      {
-        uint32_t vs[4 * G];
-        load_words<4 * G>(vs, (const unsigned char*)(s_vs + 8 * kg * G));
+        if (more) load_rest(k0 + AT_UNIT, ahead, cur);
+        // scores: all products of the step first, so that no scale waits for the product before it
+        float s[LIVE][8];
+        {
+          f4 acc[LIVE][2][G], accb[LIVE][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (nt >= live) break;
-          // only the step at the end of a row's keys, and one with a page that is not there, has keys to hide
-          const bool hides = there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP);
-          uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int t = 0; t < 8; ++t) s[nt][t] = s[nt][t] * mul[nt];
-          if (hides) {
+            for (int g = 0; g < G; ++g) {
+              h8 qf[LIVE];
 #pragma unroll
-            for (int t = 0; t < 8; ++t)
-              if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) { s[nt][t] = -__builtin_inff(); keep[t / 2] &= t & 1 ? 0x0000ffffu : 0xffff0000u; }
+              for (int nt = 0; nt < LIVE; ++nt) {
+                if constexpr (Q_REGS) qf[nt] = q[2 * g + c];
+                else qf[nt] = __builtin_bit_cast(h8, s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane]);
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t w = cur.k[i][2 * g + c], w8 = w >> 8;
+                const h8 kf = __builtin_bit_cast(h8, make_uint4(w & mask_lo, w & mask_hi, w8 & mask_lo, w8 & mask_hi));
+#pragma unroll
+                for (int nt = 0; nt < LIVE; ++nt) acc[nt][i][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[nt], c ? acc[nt][i][g] : f4{0, 0, 0, 0}, 0, 0, 0);
+              }
+            }
+          // sum over groups of b_g * (sum q), the sum in two halves
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = 8 * (n16 >> 2) + 4 * i + (n16 & 3);
+            uint4 b;
+            if constexpr (G == 4) { const uint2 x = *reinterpret_cast<const uint2*>(s_kb + key * G); b = make_uint4(x.x, x.y, x.x, x.y); }
+            else if constexpr (G == 2) { const uint32_t x = *reinterpret_cast<const uint32_t*>(s_kb + key * G); b = make_uint4(x, x, 0, 0); }
+            else { const uint32_t x = s_kb[key]; b = make_uint4(x | (x << 16), 0, 0, 0); }
+#pragma unroll
+            for (int nt = 0; nt < LIVE; ++nt) accb[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, b), qs[nt], f4{0, 0, 0, 0}, 0, 0, 0);
           }
-          float top = m[nt];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t]);
-          top = rows4_max(top);
-          const float ref = top == -__builtin_inff() ? 0.0f : top;
-          if (__any(top != m[nt])) {
-            const float back = __builtin_amdgcn_exp2f(m[nt] - ref);
-            l[nt] = l[nt] * back; ob[nt] = ob[nt] * back;
+          for (int i = 0; i < 2; ++i) {
+            uint32_t ks[2 * G];
+            load_words<2 * G>(ks, (const unsigned char*)(s_ks + (8 * kg + 4 * i) * G));
+#pragma unroll
+            for (int nt = 0; nt < LIVE; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float x = accb[nt][i][j] * 2.384185791015625e-7f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) x = fmaf(nth_half(ks, j * G + g), acc[nt][i][g][j], x);
+                s[nt][4 * i + j] = x;
+              }
+          }
+        }
+        if (more) { load_keys(k0 + AT_UNIT, ahead, cur); ahead = pages(k0 + 2 * AT_UNIT); }
+        // softmax: the running maximum per row, p relative to it
+        uint32_t pw[LIVE][G + 1][4];       // operands p s_g, and p itself
+        {
+          uint32_t vs[4 * G];
+          load_words<4 * G>(vs, (const unsigned char*)(s_vs + 8 * kg * G));
+#pragma unroll
+          for (int nt = 0; nt < LIVE; ++nt) {
+            // only the step at the end of a row's keys, and one with a page that is not there, has keys to hide
+            const bool hides = there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP);
+            uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+            if (hides) {
+#pragma unroll
+              for (int t = 0; t < 8; ++t)
+                if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) { s[nt][t] = -__builtin_inff(); keep[t / 2] &= t & 1 ? 0x0000ffffu : 0xffff0000u; }
+            }
+            float top = m[nt];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t]);
+            top = rows4_max(top);
+            const float ref = top == -__builtin_inff() ? 0.0f : top;
+            if (__any(top != m[nt])) {
+              const float back = __builtin_amdgcn_exp2f((m[nt] - ref) * mul[nt]);
+              l[nt] = l[nt] * back; ob[nt] = ob[nt] * back;
+#pragma unroll
+              for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
+              m[nt] = top;
+            }
+            const float from = -ref * mul[nt];
+            float p[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(fmaf(s[nt][t], mul[nt], from));
+            l[nt] = l[nt] + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+#pragma unroll
+            for (int t = 0; t < 4; ++t) pw[nt][G][t] = pair_of(p[2 * t], p[2 * t + 1]);
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
-            m[nt] = top;
-          }
-          float p[8];
+              for (int t = 0; t < 4; ++t) pw[nt][g][t] = pair_of(fmaf(p[2 * t], nth_half(vs, 2 * t * G + g), 0.0f), fmaf(p[2 * t + 1], nth_half(vs, (2 * t + 1) * G + g), 0.0f));   // (fma: takes the half as it is)
+            if (hides) {                 // a hidden key's scale may be NaN
 #pragma unroll
-          for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(s[nt][t] - ref);
-          l[nt] = l[nt] + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+              for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) pw[nt][G][t] = pair_of(p[2 * t], p[2 * t + 1]);
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) pw[nt][g][t] = pair_of(fmaf(p[2 * t], nth_half(vs, 2 * t * G + g), 0.0f), fmaf(p[2 * t + 1], nth_half(vs, (2 * t + 1) * G + g), 0.0f));   // (fma: takes the half as it is)
-          if (hides) {                 // a hidden key's scale may be NaN
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-              for (int t = 0; t < 4; ++t) pw[nt][g][t] &= keep[t];
+                for (int t = 0; t < 4; ++t) pw[nt][g][t] &= keep[t];
+            }
           }
         }
-      }
-      // values
-      {
+        // values
         uint4 vb = make_uint4(0, 0, 0, 0);
         if (n16 < G) vb = *reinterpret_cast<const uint4*>(s_vb + n16 * AT_STEP + 8 * kg);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < LIVE; ++nt)
           ob[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vb), __builtin_bit_cast(h8, make_uint4(pw[nt][G][0], pw[nt][G][1], pw[nt][G][2], pw[nt][G][3])), ob[nt], 0, 0, 0);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -838,12 +876,16 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
             }
             const h8 vf = __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < LIVE; ++nt)
               o[nt][g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(h8, make_uint4(pw[nt][g][0], pw[nt][g][1], pw[nt][g][2], pw[nt][g][3])), o[nt][g][i], 0, 0, 0);
           }
         }
       }
-    }
+    };
+    if (NT == 1 || rows_here <= 16) keys_loop(std::integral_constant<int, 1>{});
+    else keys_loop(std::integral_constant<int, NT>{});
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt] = m[nt] * mul[nt];        // in units of log2 from here on
 
     // ---- the four waves' sums together; lane (n16, kg) holds dims 64 g + 16 kg + 4 r + i of row n16 ----
 #pragma unroll
