@@ -474,19 +474,6 @@ SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut
   return true;
 }
 
-template <int D, int NT>
-struct AttnLds {
-  static constexpr int G = D / 64;                                    // groups of a row
-  static constexpr int V_STRIDE = 64 * 16 + 16;                       // a group's value pieces
-  static constexpr int SB = 4 * AT_STEP * G * 2;                      // key s, key b, value s [32][G] and value b' [G][32], fp16
-  static constexpr int WAVE = G * V_STRIDE + SB;
-  static constexpr int Q = NT * (D / 32) * 64 * 16;                   // query operands in the order of the lanes
-  static constexpr int JOIN = AT_WAVES * 16 * (D + 4) * 4;            // one row tile of every wave
-  static constexpr int MAIN = AT_WAVES * WAVE + Q > JOIN ? AT_WAVES * WAVE + Q : JOIN;
-  static constexpr int STAT = (2 * AT_WAVES + 2 + 4) * 16 * NT * 4;   // maximum and sum per wave and row; per row factor, keys seen, sums of q
-  static constexpr int BYTES = MAIN + STAT;
-};
-
 SL_DEV float swap16_max(float v) {
   const unsigned u = __float_as_uint(v);
   const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
@@ -525,6 +512,262 @@ SL_DEV void load_words(uint32_t* to, const unsigned char* p) {
 // Page ids for a step's three uses by this lane.
 struct KvPages { int k, v, sb; };
 
+// ---- one step of 32 keys: the parts that the kernels share ----
+constexpr int V_STRIDE = 64 * 16 + 16;        // bytes of a group's value pieces: [quarter of the keys][16 lanes][8 keys x 4 dims], padded against bank conflicts
+// LDS of a step as the lanes read it.
+struct StepLds {
+  uint16_t *ks, *vs, *kb, *vb;                // key s, value s, key b [32][G], value b + 8 s [G][32]; vs follows ks
+  unsigned char* v;                           // value pieces [G][V_STRIDE]
+  template <int D>
+  static SL_DEV StepLds at(unsigned char* p) {
+    constexpr int G = D / 64;
+    uint16_t* h = reinterpret_cast<uint16_t*>(p + G * V_STRIDE);
+    return StepLds{h, h + AT_STEP * G, h + 2 * AT_STEP * G, h + 3 * AT_STEP * G, p};
+  }
+  template <int D>
+  static constexpr int bytes() { return (D / 64) * (V_STRIDE + 4 * AT_STEP * 2); }
+};
+// Scales and biases (lanes 0..31: key `lane`, lanes 32..63: value of key lane - 32) into LDS; a key that is not there gets
+// zeros.  Value lanes turn b into b + 8 s; one that is not finite is left to the scale as NaN, which the weights carry only
+// where the key is seen.
+template <int D>
+SL_DEV void put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& st) {
+  constexpr int G = D / 64, W = (G + 1) / 2;
+  const int lane = threadIdx.x & 63;
+  uint32_t sc[W], bi[W];
+#pragma unroll
+  for (int g = 0; g < W; ++g) {
+    const uint32_t w0 = there ? sb[G == 1 ? 0 : 2 * g] : 0u, w1 = G == 1 ? 0u : (there ? sb[G == 1 ? 0 : 2 * g + 1] : 0u);
+    sc[g] = __builtin_amdgcn_perm(w1, w0, 0x05040100u); bi[g] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+  }
+  h2_t odd = {(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+  for (int g = 0; g < W; ++g) {
+    const h2_t eight = {(_Float16)8.0f, (_Float16)8.0f}, zero = {(_Float16)0.0f, (_Float16)0.0f};
+    const h2_t b = __builtin_elementwise_fma(as_h2(sc[g]), eight, as_h2(bi[g]));
+    odd = __builtin_elementwise_fma(b, zero, odd);
+    bi[g] = lane < 32 ? bi[g] : __builtin_bit_cast(uint32_t, b);
+  }
+  const _Float16 none = odd.x + odd.y;
+  if (__any(none != none && lane >= 32)) {
+#pragma unroll
+    for (int g = 0; g < W; ++g)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (lane >= 32 && ((bi[g] >> (16 * u)) & 0x7c00u) == 0x7c00u) { bi[g] &= u ? 0x0000ffffu : 0xffff0000u; sc[g] = (sc[g] & (u ? 0x0000ffffu : 0xffff0000u)) | (0x7e00u << (16 * u)); }
+  }
+  if constexpr (G == 4) {
+    *reinterpret_cast<uint2*>(st.ks + lane * G) = make_uint2(sc[0], sc[1]);
+    if (lane < 32) *reinterpret_cast<uint2*>(st.kb + lane * G) = make_uint2(bi[0], bi[1]);
+  } else if constexpr (G == 2) {
+    *reinterpret_cast<uint32_t*>(st.ks + lane * G) = sc[0];
+    if (lane < 32) *reinterpret_cast<uint32_t*>(st.kb + lane * G) = bi[0];
+  } else {
+    st.ks[lane] = (uint16_t)sc[0];
+    if (lane < 32) st.kb[lane] = (uint16_t)bi[0];
+  }
+  if (lane >= 32) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) st.vb[g * AT_STEP + (lane & 31)] = (uint16_t)(bi[g / 2] >> (16 * (g & 1)));
+  }
+}
+// s[row tile][8]: this lane's keys 8 kg .. 8 kg + 7 against row n16.  All products of the step first, so that no scale waits for
+// the product before it.  `query(nt, i)`: the operand of dims word i; k: the two key operands' words.
+template <int D, int LIVE, class Q, int NT>
+SL_DEV void step_scores(const uint32_t (&k)[2][D / 32], Q query, const h8 (&qs)[NT], const StepLds& st, uint32_t mask_lo, uint32_t mask_hi, float (&s)[LIVE][8]) {
+  constexpr int G = D / 64;
+  const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
+  f4 acc[LIVE][2][G], accb[LIVE][2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      h8 qf[LIVE];
+#pragma unroll
+      for (int nt = 0; nt < LIVE; ++nt) qf[nt] = query(nt, 2 * g + c);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w = k[i][2 * g + c], w8 = w >> 8;
+        const h8 kf = __builtin_bit_cast(h8, make_uint4(w & mask_lo, w & mask_hi, w8 & mask_lo, w8 & mask_hi));
+#pragma unroll
+        for (int nt = 0; nt < LIVE; ++nt) acc[nt][i][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[nt], c ? acc[nt][i][g] : f4{0, 0, 0, 0}, 0, 0, 0);
+      }
+    }
+  // sum over groups of b_g * (sum q), the sum in two halves
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int key = 8 * (n16 >> 2) + 4 * i + (n16 & 3);
+    uint4 b;
+    if constexpr (G == 4) { const uint2 x = *reinterpret_cast<const uint2*>(st.kb + key * G); b = make_uint4(x.x, x.y, x.x, x.y); }
+    else if constexpr (G == 2) { const uint32_t x = *reinterpret_cast<const uint32_t*>(st.kb + key * G); b = make_uint4(x, x, 0, 0); }
+    else { const uint32_t x = st.kb[key]; b = make_uint4(x | (x << 16), 0, 0, 0); }
+#pragma unroll
+    for (int nt = 0; nt < LIVE; ++nt) accb[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, b), qs[nt], f4{0, 0, 0, 0}, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t ks[2 * G];
+    load_words<2 * G>(ks, (const unsigned char*)(st.ks + (8 * kg + 4 * i) * G));
+#pragma unroll
+    for (int nt = 0; nt < LIVE; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = accb[nt][i][j] * 2.384185791015625e-7f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) x = fmaf(nth_half(ks, j * G + g), acc[nt][i][g][j], x);
+        s[nt][4 * i + j] = x;
+      }
+  }
+}
+// The running maximum per row, p relative to it; pw: the operands p s_g of each group, then p itself.
+template <int D, int LIVE, int NT>
+SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int (&limit)[NT], const float (&mul)[NT], const StepLds& st, float (&m)[NT],
+                         float (&l)[NT], f4 (&o)[NT][D / 64][4], f4 (&ob)[NT], uint32_t (&pw)[LIVE][D / 64 + 1][4]) {
+  constexpr int G = D / 64;
+  const int lane = threadIdx.x & 63, kg = lane >> 4;
+  uint32_t vs[4 * G];
+  load_words<4 * G>(vs, (const unsigned char*)(st.vs + 8 * kg * G));
+#pragma unroll
+  for (int nt = 0; nt < LIVE; ++nt) {
+    // only the step at the end of a row's keys, and one with a page that is not there, has keys to hide
+    const bool hides = there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP);
+    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    if (hides) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) { s[nt][t] = -__builtin_inff(); keep[t / 2] &= t & 1 ? 0x0000ffffu : 0xffff0000u; }
+    }
+    float top = m[nt];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t]);
+    top = rows4_max(top);
+    const float ref = top == -__builtin_inff() ? 0.0f : top;
+    if (__any(top != m[nt])) {
+      const float back = __builtin_amdgcn_exp2f((m[nt] - ref) * mul[nt]);
+      l[nt] = l[nt] * back; ob[nt] = ob[nt] * back;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
+      m[nt] = top;
+    }
+    const float from = -ref * mul[nt];
+    float p[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(fmaf(s[nt][t], mul[nt], from));
+    l[nt] = l[nt] + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+#pragma unroll
+    for (int t = 0; t < 4; ++t) pw[nt][G][t] = pair_of(p[2 * t], p[2 * t + 1]);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) pw[nt][g][t] = pair_of(fmaf(p[2 * t], nth_half(vs, 2 * t * G + g), 0.0f), fmaf(p[2 * t + 1], nth_half(vs, (2 * t + 1) * G + g), 0.0f));   // (fma: takes the half as it is)
+    if (hides) {                 // a hidden key's scale may be NaN
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) pw[nt][g][t] &= keep[t];
+    }
+  }
+}
+template <int D, int LIVE, int NT>
+SL_DEV void step_values(const uint32_t (&pw)[LIVE][D / 64 + 1][4], const StepLds& st, uint32_t ones, uint32_t mask_lo, uint32_t mask_hi, f4 (&o)[NT][D / 64][4], f4 (&ob)[NT]) {
+  constexpr int G = D / 64;
+  const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
+  uint4 vb = make_uint4(0, 0, 0, 0);
+  if (n16 < G) vb = *reinterpret_cast<const uint4*>(st.vb + n16 * AT_STEP + 8 * kg);
+#pragma unroll
+  for (int nt = 0; nt < LIVE; ++nt)
+    ob[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vb), __builtin_bit_cast(h8, make_uint4(pw[nt][G][0], pw[nt][G][1], pw[nt][G][2], pw[nt][G][3])), ob[nt], 0, 0, 0);
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const uint4 raw = ld16(st.v + g * V_STRIDE + lane * 16);
+    const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w[4];
+      const h2_t off = i & 1 ? h2_t{(_Float16)-1152.0f, (_Float16)-1152.0f} : h2_t{(_Float16)-1032.0f, (_Float16)-1032.0f};
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint32_t y = i & 2 ? x[t] >> 8 : x[t];
+        w[t] = __builtin_bit_cast(uint32_t, as_h2((y & (i & 1 ? mask_hi : mask_lo)) | ones) + off);
+      }
+      const h8 vf = __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+      for (int nt = 0; nt < LIVE; ++nt)
+        o[nt][g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(h8, make_uint4(pw[nt][g][0], pw[nt][g][1], pw[nt][g][2], pw[nt][g][3])), o[nt][g][i], 0, 0, 0);
+    }
+  }
+        
+}
+
+template <int D, int NT>
+struct AttnLds {
+  static constexpr int G = D / 64;                                    // groups of a row
+  static constexpr int WAVE = StepLds::bytes<D>();
+  static constexpr int Q = NT * (D / 32) * 64 * 16;                   // query operands in the order of the lanes
+  static constexpr int JOIN = AT_WAVES * 16 * (D + 4) * 4;            // one row tile of every wave
+  static constexpr int MAIN = AT_WAVES * WAVE + Q > JOIN ? AT_WAVES * WAVE + Q : JOIN;
+  static constexpr int STAT = (2 * AT_WAVES + 2 + 4) * 16 * NT * 4;   // maximum and sum per wave and row; per row factor, keys seen, sums of q
+  static constexpr int BYTES = MAIN + STAT;
+};
+
+constexpr int NO_LIMIT = 0x7fffffff;          // of the columns behind the last row, which are never written
+struct QueryLds {
+  uint4 *word, *sum;                          // operands [row tile][D/32][64 lanes], the groups' sums of a row as halves
+  float* mul;                                 // factor from a row's scores to units of log2
+  int* limit;                                 // keys that a row sees
+};
+// Row `in` of the workgroup, 16 lanes a row, D/16 dims a lane (bits in `raw`).
+template <int D, bool BF>
+SL_DEV void put_query(const uint2 (&raw)[D / 64], int in, bool valid, int limit, float scale, const QueryLds& q) {
+  constexpr int G = D / 64, PER = D / 16;
+  const int l16 = threadIdx.x & 15;
+  float x[PER], top = 0.0f;
+#pragma unroll
+  for (int c = 0; c < PER / 4; ++c) {
+    const uint16_t e4[4] = {(uint16_t)raw[c].x, (uint16_t)(raw[c].x >> 16), (uint16_t)raw[c].y, (uint16_t)(raw[c].y >> 16)};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[4 * c + j] = valid ? elem_f<BF>(e4[j]) : 0.0f; top = fmaxf(top, fabsf(x[4 * c + j])); }
+  }
+  top = fmaxf(top, dpp_f<DPP_XOR1>(top)); top = fmaxf(top, dpp_f<DPP_XOR2>(top));
+  top = fmaxf(top, dpp_f<DPP_HALF_MIRROR>(top)); top = fmaxf(top, dpp_f<DPP_MIRROR>(top));
+  const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 100);
+  const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23) * (scale < 0.0f ? -1.0f : 1.0f);
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) { x[i] = x[i] * f; sum = sum + x[i]; }
+  sum = tree_sum<16 / G>(sum) * 0.25f;               // at most 64 * 2^11 / 4
+  if (l16 % (16 / G) == 0) {                         // as two halves, behind each other for G > 1: operand [hi of the groups | lo of the groups]
+    uint16_t* w = reinterpret_cast<uint16_t*>(q.sum + in) + l16 / (16 / G);
+    const uint16_t hi = f2h(sum);
+    w[0] = hi; w[G] = f2h(sum - h2f(hi));
+    if (G < 4) {
+#pragma unroll
+      for (int i = 2; i < 8 / G; ++i) w[i * G] = 0;
+    }
+  }
+  if (l16 == 0) {
+    // (a factor of zero would leave hidden keys without their minus infinity)
+    q.mul[in] = fmaxf(fabsf(scale) * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23)), 1e-30f);
+    q.limit[in] = limit;
+  }
+  // operand word w of quarter kg in group g: dims 64 g + 16 kg + 8 w + (0 4 | 1 5 | 2 6 | 3 7), the odd ones / 16
+  if constexpr (PER >= 8) {
+#pragma unroll
+    for (int c = 0; c < PER / 8; ++c) {
+      const int d = PER * l16 + 8 * c, to = (in / 16 * (D / 32) + 2 * (d / 64) + (d / 8) % 2) * 64 + (d % 64) / 16 * 16 + (in & 15);
+      const float* y = x + 8 * c;
+      q.word[to] = make_uint4(half_pair(y[0], y[4]), half_pair(y[1] * 0.0625f, y[5] * 0.0625f), half_pair(y[2], y[6]), half_pair(y[3] * 0.0625f, y[7] * 0.0625f));
+    }
+  } else {
+    const int d = 4 * l16, to = (in / 16 * (D / 32) + (d / 8) % 2) * 64 + d / 16 * 16 + (in & 15);
+    uint16_t* w = reinterpret_cast<uint16_t*>(q.word + to) + (l16 & 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[2 * j] = f2h(j & 1 ? x[j] * 0.0625f : x[j]);
+  }
+}
+
 // Normalised, gated, rounded: the last step of a row (sum 0: the row saw no key).
 template <bool BF>
 SL_DEV float finish_value(const sl_kv4_attn_args& a, float y, float sum, uint16_t gate) {
@@ -540,6 +783,34 @@ SL_DEV void finish_row(const sl_kv4_attn_args& a, int t, int head, int d, float4
   *reinterpret_cast<uint2*>((uint16_t*)a.out + t * a.out_token + head * a.out_head + d) =
       make_uint2((uint32_t)f_elem<BF>(x0) | ((uint32_t)f_elem<BF>(x1) << 16), (uint32_t)f_elem<BF>(x2) | ((uint32_t)f_elem<BF>(x3) << 16));
 }
+// A wave's sums of one row tile to LDS [16 rows][D + 4], times f: lane (n16, kg) holds dims 64 g + 16 kg + 4 r + i of row n16.
+template <int D>
+SL_DEV void put_sums(const f4 (&o)[D / 64][4], const f4& ob, float f, float* to) {
+  const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
+  float bias[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) bias[g] = __shfl(ob[g], n16);
+#pragma unroll
+  for (int g = 0; g < D / 64; ++g)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float4 y;
+      y.x = (o[g][0][r] + bias[g]) * f; y.y = fmaf(o[g][1][r], 0.0625f, bias[g]) * f;
+      y.z = (o[g][2][r] + bias[g]) * f; y.w = fmaf(o[g][3][r], 0.0625f, bias[g]) * f;
+      *reinterpret_cast<float4*>(to + n16 * (D + 4) + 64 * g + 16 * kg + 4 * r) = y;
+    }
+}
+// Four dims of a row: to the output, or as a partial sum (slot >= 0) with its maximum and sum.
+template <int D, bool BF>
+SL_DEV void put_row(const sl_kv4_attn_args& a, const AttnCut& cut, long slot, int in, int t, int head, int d, float4 y, float best, float sum) {
+  if (slot < 0) { finish_row<BF>(a, t, head, d, y, sum); return; }
+  *reinterpret_cast<float4*>(cut.part + (slot * cut.rows + in) * D + d) = y;
+  if (d == 0) {
+    float* stat = cut.part + cut.slots * cut.rows * D;
+    stat[slot * cut.rows + in] = best; stat[(cut.slots + slot) * cut.rows + in] = sum;
+  }
+}
+
 template <int D, bool BF, int NT>
 __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
   using L = AttnLds<D, NT>;
@@ -551,10 +822,9 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
   uint4* s_qsum = reinterpret_cast<uint4*>(s_lim + 16 * NT);
   int* s_first = reinterpret_cast<int*>(lds + L::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kg = lane >> 4;
-  unsigned char* s_wave = lds + wave * L::WAVE;
-  uint16_t* s_ks = reinterpret_cast<uint16_t*>(s_wave + G * L::V_STRIDE);
-  uint16_t *s_vs = s_ks + AT_STEP * G, *s_kb = s_vs + AT_STEP * G, *s_vb = s_kb + AT_STEP * G;
+  const StepLds st = StepLds::at<D>(lds + wave * L::WAVE);
   uint4* s_q = reinterpret_cast<uint4*>(lds + AT_WAVES * L::WAVE);
+  const QueryLds sq{s_q, s_qsum, s_mul, s_lim};
   const int group = a.n_heads / pool.n_kv, shift = pool.page_shift, page_mask = (1 << shift) - 1;
   const uint32_t page_stride = (uint32_t)(pool.n_kv * (int)head_bytes<D>(pool));
   const int part_c = (D / 2) << shift, part_sb = (D / 16) << shift;
@@ -616,53 +886,9 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
     // ---- queries: operands in fp16, their sums per group, the factor back to scores in units of log2 ----
 #pragma unroll
     for (int pass = 0; pass < NT; ++pass) {
-      constexpr int PER = QPER;
-      const int in = pass * 16 + (tid >> 4), l16 = tid & 15, row = row0 + in, tok = row / group;
       if (pass * 16 >= rows_here) break;                 // (operands of an empty tile are not used)
-      const bool valid = in < rows_here;
-      float x[PER], top = 0.0f;
-#pragma unroll
-      for (int c = 0; c < PER / 4; ++c) {
-        const uint16_t e4[4] = {(uint16_t)raw[pass][c].x, (uint16_t)(raw[pass][c].x >> 16), (uint16_t)raw[pass][c].y, (uint16_t)(raw[pass][c].y >> 16)};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { x[4 * c + j] = valid ? elem_f<BF>(e4[j]) : 0.0f; top = fmaxf(top, fabsf(x[4 * c + j])); }
-      }
-      top = fmaxf(top, dpp_f<DPP_XOR1>(top)); top = fmaxf(top, dpp_f<DPP_XOR2>(top));
-      top = fmaxf(top, dpp_f<DPP_HALF_MIRROR>(top)); top = fmaxf(top, dpp_f<DPP_MIRROR>(top));
-      const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 100);
-      const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f);
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) { x[i] = x[i] * f; sum = sum + x[i]; }
-      sum = tree_sum<16 / G>(sum) * 0.25f;               // at most 64 * 2^11 / 4
-      if (l16 % (16 / G) == 0) {                         // as two halves, behind each other for G > 1: operand [hi of the groups | lo of the groups]
-        uint16_t* w = reinterpret_cast<uint16_t*>(s_qsum + in) + l16 / (16 / G);
-        const uint16_t hi = f2h(sum);
-        w[0] = hi; w[G] = f2h(sum - h2f(hi));
-        if (G < 4) {
-#pragma unroll
-          for (int i = 2; i < 8 / G; ++i) w[i * G] = 0;
-        }
-      }
-      if (l16 == 0) {
-        // (a factor of zero would leave hidden keys without their minus infinity)
-        s_mul[in] = fmaxf(fabsf(a.scale) * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23)), 1e-30f);
-        s_lim[in] = valid ? (int)max(0l, keys - n + tok + 1) : 0x7fffffff;      // (the columns behind the last row are never written)
-      }
-      // operand word w of quarter kg in group g: dims 64 g + 16 kg + 8 w + (0 4 | 1 5 | 2 6 | 3 7), the odd ones / 16
-      if constexpr (PER >= 8) {
-#pragma unroll
-        for (int c = 0; c < PER / 8; ++c) {
-          const int d = PER * l16 + 8 * c, to = (pass * (D / 32) + 2 * (d / 64) + (d / 8) % 2) * 64 + (d % 64) / 16 * 16 + (in & 15);
-          const float* y = x + 8 * c;
-          s_q[to] = make_uint4(half_pair(y[0], y[4]), half_pair(y[1] * 0.0625f, y[5] * 0.0625f), half_pair(y[2], y[6]), half_pair(y[3] * 0.0625f, y[7] * 0.0625f));
-        }
-      } else {
-        const int d = 4 * l16, to = (pass * (D / 32) + (d / 8) % 2) * 64 + d / 16 * 16 + (in & 15);
-        uint16_t* w = reinterpret_cast<uint16_t*>(s_q + to) + (l16 & 1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[2 * j] = f2h(j & 1 ? x[j] * 0.0625f : x[j]);
-      }
+      const int in = pass * 16 + (tid >> 4);
+      put_query<D, BF>(raw[pass], in, in < rows_here, in < rows_here ? (int)max(0l, keys - n + (row0 + in) / group + 1) : NO_LIMIT, a.scale, sq);
     }
     lds_barrier();
     // (dims of 256 and several row tiles leave no room for the operands in registers)
@@ -700,186 +926,32 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
       constexpr int LIVE = decltype(live_tiles)::value;
       for (; k0 < key1; k0 += AT_UNIT) {
         const bool more = k0 + AT_UNIT < key1;
-        // scales and biases; a key that is not there gets zeros.  Value lanes turn b into b + 8 s; one that is not finite
-        // is left to the scale as NaN, which the weights carry only where the key is seen.
         const unsigned there = (unsigned)__ballot(cur.there);
-        {
-          constexpr int W = (G + 1) / 2;
-          uint32_t sc[W], bi[W];
+        wave_lds_order();
+        put_scales<D>(cur.sb, cur.there, st);
+        // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
 #pragma unroll
-          for (int g = 0; g < W; ++g) {
-            const uint32_t w0 = cur.there ? cur.sb[G == 1 ? 0 : 2 * g] : 0u, w1 = G == 1 ? 0u : (cur.there ? cur.sb[G == 1 ? 0 : 2 * g + 1] : 0u);
-            sc[g] = __builtin_amdgcn_perm(w1, w0, 0x05040100u); bi[g] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+        for (int c = 0; c < G; ++c) {
+          uint32_t x[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if constexpr (G == 4) x[t] = __builtin_amdgcn_perm(cur.v[4 * t + 2 + c / 2], cur.v[4 * t + c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+            else if constexpr (G == 2) x[t] = __builtin_amdgcn_perm(cur.v[2 * t + 1], cur.v[2 * t], c & 1 ? 0x07060302u : 0x05040100u);
+            else x[t] = cur.v[t];
           }
-          h2_t odd = {(_Float16)0.0f, (_Float16)0.0f};
-#pragma unroll
-          for (int g = 0; g < W; ++g) {
-            const h2_t eight = {(_Float16)8.0f, (_Float16)8.0f}, zero = {(_Float16)0.0f, (_Float16)0.0f};
-            const h2_t b = __builtin_elementwise_fma(as_h2(sc[g]), eight, as_h2(bi[g]));
-            odd = __builtin_elementwise_fma(b, zero, odd);
-            bi[g] = lane < 32 ? bi[g] : __builtin_bit_cast(uint32_t, b);
-          }
-          const _Float16 none = odd.x + odd.y;
-          if (__any(none != none && lane >= 32)) {
-#pragma unroll
-            for (int g = 0; g < W; ++g)
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-                if (lane >= 32 && ((bi[g] >> (16 * u)) & 0x7c00u) == 0x7c00u) { bi[g] &= u ? 0x0000ffffu : 0xffff0000u; sc[g] = (sc[g] & (u ? 0x0000ffffu : 0xffff0000u)) | (0x7e00u << (16 * u)); }
-          }
-          wave_lds_order();
-          if constexpr (G == 4) {
-            *reinterpret_cast<uint2*>(s_ks + lane * G) = make_uint2(sc[0], sc[1]);
-            if (lane < 32) *reinterpret_cast<uint2*>(s_kb + lane * G) = make_uint2(bi[0], bi[1]);
-          } else if constexpr (G == 2) {
-            *reinterpret_cast<uint32_t*>(s_ks + lane * G) = sc[0];
-            if (lane < 32) *reinterpret_cast<uint32_t*>(s_kb + lane * G) = bi[0];
-          } else {
-            s_ks[lane] = (uint16_t)sc[0];
-            if (lane < 32) s_kb[lane] = (uint16_t)bi[0];
-          }
-          if (lane >= 32) {
-#pragma unroll
-            for (int g = 0; g < G; ++g) s_vb[g * AT_STEP + (lane & 31)] = (uint16_t)(bi[g / 2] >> (16 * (g & 1)));
-          }
-          // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
-#pragma unroll
-          for (int c = 0; c < G; ++c) {
-            uint32_t x[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              if constexpr (G == 4) x[t] = __builtin_amdgcn_perm(cur.v[4 * t + 2 + c / 2], cur.v[4 * t + c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-              else if constexpr (G == 2) x[t] = __builtin_amdgcn_perm(cur.v[2 * t + 1], cur.v[2 * t], c & 1 ? 0x07060302u : 0x05040100u);
-              else x[t] = cur.v[t];
-            }
-            const int to_m = G * (n16 % (16 / G)) + c, to_g = n16 / (16 / G);
-            st16(s_wave + to_g * L::V_STRIDE + (kg * 16 + to_m) * 16, make_uint4(x[0], x[1], x[2], x[3]));
-          }
-          wave_lds_order();
+          st16(st.v + (n16 / (16 / G)) * V_STRIDE + (kg * 16 + G * (n16 % (16 / G)) + c) * 16, make_uint4(x[0], x[1], x[2], x[3]));
         }
+        wave_lds_order();
         if (more) load_rest(k0 + AT_UNIT, ahead, cur);
-        // scores: all products of the step first, so that no scale waits for the product before it
         float s[LIVE][8];
-        {
-          f4 acc[LIVE][2][G], accb[LIVE][2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-              h8 qf[LIVE];
-#pragma unroll
-              for (int nt = 0; nt < LIVE; ++nt) {
-                if constexpr (Q_REGS) qf[nt] = q[2 * g + c];
-                else qf[nt] = __builtin_bit_cast(h8, s_q[(nt * (D / 32) + 2 * g + c) * 64 + lane]);
-              }
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t w = cur.k[i][2 * g + c], w8 = w >> 8;
-                const h8 kf = __builtin_bit_cast(h8, make_uint4(w & mask_lo, w & mask_hi, w8 & mask_lo, w8 & mask_hi));
-#pragma unroll
-                for (int nt = 0; nt < LIVE; ++nt) acc[nt][i][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[nt], c ? acc[nt][i][g] : f4{0, 0, 0, 0}, 0, 0, 0);
-              }
-            }
-          // sum over groups of b_g * (sum q), the sum in two halves
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int key = 8 * (n16 >> 2) + 4 * i + (n16 & 3);
-            uint4 b;
-            if constexpr (G == 4) { const uint2 x = *reinterpret_cast<const uint2*>(s_kb + key * G); b = make_uint4(x.x, x.y, x.x, x.y); }
-            else if constexpr (G == 2) { const uint32_t x = *reinterpret_cast<const uint32_t*>(s_kb + key * G); b = make_uint4(x, x, 0, 0); }
-            else { const uint32_t x = s_kb[key]; b = make_uint4(x | (x << 16), 0, 0, 0); }
-#pragma unroll
-            for (int nt = 0; nt < LIVE; ++nt) accb[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, b), qs[nt], f4{0, 0, 0, 0}, 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t ks[2 * G];
-            load_words<2 * G>(ks, (const unsigned char*)(s_ks + (8 * kg + 4 * i) * G));
-#pragma unroll
-            for (int nt = 0; nt < LIVE; ++nt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float x = accb[nt][i][j] * 2.384185791015625e-7f;
-#pragma unroll
-                for (int g = 0; g < G; ++g) x = fmaf(nth_half(ks, j * G + g), acc[nt][i][g][j], x);
-                s[nt][4 * i + j] = x;
-              }
-          }
-        }
+        step_scores<D, LIVE>(cur.k, [&](int nt, int i) {
+          if constexpr (Q_REGS) return q[i];
+          else return __builtin_bit_cast(h8, s_q[(nt * (D / 32) + i) * 64 + lane]);
+        }, qs, st, mask_lo, mask_hi, s);
         if (more) { load_keys(k0 + AT_UNIT, ahead, cur); ahead = pages(k0 + 2 * AT_UNIT); }
-        // softmax: the running maximum per row, p relative to it
-        uint32_t pw[LIVE][G + 1][4];       // operands p s_g, and p itself
-        {
-          uint32_t vs[4 * G];
-          load_words<4 * G>(vs, (const unsigned char*)(s_vs + 8 * kg * G));
-#pragma unroll
-          for (int nt = 0; nt < LIVE; ++nt) {
-            // only the step at the end of a row's keys, and one with a page that is not there, has keys to hide
-            const bool hides = there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP);
-            uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-            if (hides) {
-#pragma unroll
-              for (int t = 0; t < 8; ++t)
-                if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) { s[nt][t] = -__builtin_inff(); keep[t / 2] &= t & 1 ? 0x0000ffffu : 0xffff0000u; }
-            }
-            float top = m[nt];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t]);
-            top = rows4_max(top);
-            const float ref = top == -__builtin_inff() ? 0.0f : top;
-            if (__any(top != m[nt])) {
-              const float back = __builtin_amdgcn_exp2f((m[nt] - ref) * mul[nt]);
-              l[nt] = l[nt] * back; ob[nt] = ob[nt] * back;
-#pragma unroll
-              for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
-              m[nt] = top;
-            }
-            const float from = -ref * mul[nt];
-            float p[8];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(fmaf(s[nt][t], mul[nt], from));
-            l[nt] = l[nt] + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
-#pragma unroll
-            for (int t = 0; t < 4; ++t) pw[nt][G][t] = pair_of(p[2 * t], p[2 * t + 1]);
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-              for (int t = 0; t < 4; ++t) pw[nt][g][t] = pair_of(fmaf(p[2 * t], nth_half(vs, 2 * t * G + g), 0.0f), fmaf(p[2 * t + 1], nth_half(vs, (2 * t + 1) * G + g), 0.0f));   // (fma: takes the half as it is)
-            if (hides) {                 // a hidden key's scale may be NaN
-#pragma unroll
-              for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) pw[nt][g][t] &= keep[t];
-            }
-          }
-        }
-        // values
-        uint4 vb = make_uint4(0, 0, 0, 0);
-        if (n16 < G) vb = *reinterpret_cast<const uint4*>(s_vb + n16 * AT_STEP + 8 * kg);
-#pragma unroll
-        for (int nt = 0; nt < LIVE; ++nt)
-          ob[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vb), __builtin_bit_cast(h8, make_uint4(pw[nt][G][0], pw[nt][G][1], pw[nt][G][2], pw[nt][G][3])), ob[nt], 0, 0, 0);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const uint4 raw = ld16(s_wave + g * L::V_STRIDE + lane * 16);
-          const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
-            const h2_t off = i & 1 ? h2_t{(_Float16)-1152.0f, (_Float16)-1152.0f} : h2_t{(_Float16)-1032.0f, (_Float16)-1032.0f};
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const uint32_t y = i & 2 ? x[t] >> 8 : x[t];
-              w[t] = __builtin_bit_cast(uint32_t, as_h2((y & (i & 1 ? mask_hi : mask_lo)) | ones) + off);
-            }
-            const h8 vf = __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3]));
-#pragma unroll
-            for (int nt = 0; nt < LIVE; ++nt)
-              o[nt][g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(h8, make_uint4(pw[nt][g][0], pw[nt][g][1], pw[nt][g][2], pw[nt][g][3])), o[nt][g][i], 0, 0, 0);
-          }
-        }
+        uint32_t pw[LIVE][G + 1][4];
+        step_weights<D, LIVE, NT>(s, there, k0, limit, mul, st, m, l, o, ob, pw);
+        step_values<D, LIVE, NT>(pw, st, ones, mask_lo, mask_hi, o, ob);
       }
     };
     if (NT == 1 || rows_here <= 16) keys_loop(std::integral_constant<int, 1>{});
@@ -902,18 +974,7 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
 #pragma unroll
       for (int w = 0; w < AT_WAVES; ++w) top = fmaxf(top, s_m[w * 16 * NT + nt * 16 + n16]);
       const float f = m[nt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - top);
-      float bias[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) bias[g] = __shfl(ob[nt][g], n16);
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int rr = 0; rr < 4; ++rr) {
-          float4 y;
-          y.x = (o[nt][g][0][rr] + bias[g]) * f; y.y = fmaf(o[nt][g][1][rr], 0.0625f, bias[g]) * f;
-          y.z = (o[nt][g][2][rr] + bias[g]) * f; y.w = fmaf(o[nt][g][3][rr], 0.0625f, bias[g]) * f;
-          *reinterpret_cast<float4*>(s_o + (wave * 16 + n16) * (D + 4) + 64 * g + 16 * kg + 4 * rr) = y;
-        }
+      put_sums<D>(o[nt], ob[nt], f, s_o + wave * 16 * (D + 4));
       lds_barrier();
       // a thread per four dims of a row
       for (int i = tid; i < 16 * (D / 4); i += 256) {
@@ -930,17 +991,210 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
           const float mw = s_m[w * 16 * NT + in];
           sum += s_l[w * 16 * NT + in] * (mw == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw - best));
         }
-        if (slot >= 0) {
-          *reinterpret_cast<float4*>(cut.part + (slot * cut.rows + in) * D + d) = y;
-          if (d == 0) {
-            float* stat = cut.part + cut.slots * cut.rows * D;
-            stat[slot * cut.rows + in] = best; stat[(cut.slots + slot) * cut.rows + in] = sum;
-          }
-        } else {
-          const int tok = (row0 + in) / group, head = h * group + (row0 + in - tok * group);
-          finish_row<BF>(a, start + tok, head, d, y, sum);
-        }
+        const int row_of = row0 + in, tok = row_of / group;
+        put_row<D, BF>(a, cut, slot, in, start + tok, h * group + (row_of - tok * group), d, y, best, sum);
       }
+    }
+  }
+}
+
+// Many rows: a workgroup takes 64 rows.  Its waves lay a step's bytes out in LDS together, a step ahead of its use, so the registers
+// hold no bytes but those on their way.  Dims of 256: each wave has 16 rows (the sums of 32 would not leave room for two waves a
+// SIMD) and all keys.  Fewer dims: two waves of 32 rows each take every second step, two the others, and a step is unpacked
+// for 32 rows at once; the two key groups' sums are joined at the end.
+template <int D>
+struct TileLds {
+  static constexpr int KEYS = 16 * D;                                  // key words in the order of the lanes
+  static constexpr int STEP = KEYS + StepLds::bytes<D>();
+  static constexpr int KS = D == 256 ? 1 : 2;                          // key groups
+  static constexpr int Q = 4 * (D / 32) * 64 * 16;
+  static constexpr int JOIN = 4 * 16 * (D + 4) * 4;
+  static constexpr int MAIN = 2 * KS * STEP + Q > JOIN ? 2 * KS * STEP + Q : JOIN;
+  static constexpr int STAT = (2 * KS + 2 + 4) * 64 * 4;
+  static constexpr int BYTES = MAIN + STAT;
+};
+template <int D, bool BF>
+__global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
+  using L = TileLds<D>;
+  constexpr int G = D / 64, KS = L::KS, RS = 4 / KS, NT = KS, KW = D >= 128 ? 4 : 2, HALVES = D == 256 ? 2 : 1;     // KW: words that a thread brings of keys and of values
+  extern __shared__ __align__(16) unsigned char lds[];
+  float* s_m = reinterpret_cast<float*>(lds + L::MAIN);
+  float *s_l = s_m + KS * 64, *s_mul = s_l + KS * 64;
+  int* s_lim = reinterpret_cast<int*>(s_mul + 64);
+  uint4* s_qsum = reinterpret_cast<uint4*>(s_lim + 64);
+  int* s_first = reinterpret_cast<int*>(lds + L::BYTES);
+  uint4* s_q = reinterpret_cast<uint4*>(lds + 2 * KS * L::STEP);
+  const QueryLds sq{s_q, s_qsum, s_mul, s_lim};
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kg = lane >> 4, rg = wave % RS, ks = wave / RS, t2 = tid % (RS * 64);
+  const int group = a.n_heads / pool.n_kv, shift = pool.page_shift, page_mask = (1 << shift) - 1;
+  const uint32_t page_stride = (uint32_t)(pool.n_kv * (int)head_bytes<D>(pool));
+  const int part_c = (D / 2) << shift, part_sb = (D / 16) << shift;
+
+  AttnPart at;
+  if (!find_part<64>(a, pool, cut, blockIdx.x, s_first, reinterpret_cast<int*>(s_m), at)) return;
+  const int r = at.r, h = at.h;
+  int start, n;
+  const int rows = rows_of(a, r, start, n), tiles = (rows * group + 63) / 64;
+  const int row0 = (tiles - 1 - at.tile) * 64, rows_here = min(64, rows * group - row0);      // the tiles that see most keys first
+  const long keys = seen_keys(a, pool, r), slot = at.parts > 1 ? (long)blockIdx.x : -1;
+  const long last = max(0l, min(keys, keys - n + (row0 + rows_here - 1) / group + 1));
+  const int key0 = at.part * at.share * AT_UNIT, key1 = (int)min((long)min(at.rounds, (at.part + 1) * at.share) * AT_UNIT, last);
+
+  uint2 raw[4][D / 64];
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int in = pass * 16 + (tid >> 4), row = row0 + (in < rows_here ? in : 0), tok = row / group, head = h * group + (row - tok * group);
+    const uint16_t* src = (const uint16_t*)a.q + (long)(start + tok) * a.q_token + (long)head * a.q_head + (D / 16) * (tid & 15);
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) raw[pass][c] = *reinterpret_cast<const uint2*>(src + 4 * c);
+  }
+
+  // A step's bytes by the key group's threads: 16 bytes each of keys and values (8 for dims of 64).
+  const int32_t* table = a.table + (size_t)r * a.table_width;
+  const int end_page = key1 > 0 ? (key1 - 1) >> shift : 0;
+  const unsigned char* head_base = pool.pages + (size_t)h * head_bytes<D>(pool);
+  auto base = [&](int page) { return head_base + (uint64_t)((unsigned)page < (unsigned)pool.n_pages ? (uint32_t)page : 0u) * page_stride; };
+  auto page_of = [&](int key) { return table[min(key >> shift, end_page)]; };
+  uint32_t wk[KW], wv[KW], sb[G];
+  bool there = false;
+  const int key_token = t2 & 31, key_part = t2 >> 5;
+  constexpr int V_UNITS = D / 16 / KW;                                 // threads to a lane's 8 keys
+  const int v_blk = t2 / (16 * V_UNITS), v_m = (t2 / V_UNITS) & 15, v_sub = t2 % V_UNITS;
+  auto pages = [&](int k0) {
+    KvPages p;
+    p.k = page_of(k0 + key_token); p.v = page_of(k0 + 8 * v_blk); p.sb = rg == 0 ? page_of(k0 + (lane & 31)) : 0;
+    return p;
+  };
+  auto load = [&](int k0, const KvPages& p) {
+    load_words<KW>(wk, base(p.k) + ((k0 + key_token) & page_mask) * (D / 2) + 4 * KW * key_part);
+    load_words<KW>(wv, base(p.v) + part_c + part_sb + (((k0 + 8 * v_blk) & page_mask) >> 3) * (4 * D) + (t2 % (16 * V_UNITS)) * (4 * KW));
+    if (rg == 0) {
+      load_words<G>(sb, base(p.sb) + (lane < 32 ? part_c : 2 * part_c + part_sb) + ((k0 + (lane & 31)) & page_mask) * (D / 16));
+      there = (unsigned)p.sb < (unsigned)pool.n_pages && k0 + (lane & 31) < key1;
+    }
+  };
+  auto step_lds = [&](int buf) { return lds + (2 * ks + buf) * L::STEP; };
+  unsigned* s_there = reinterpret_cast<unsigned*>(s_m);                // [key group][buffer], free until the end
+  // keys: [operand][half of the row's quarter][quarter][row of the operand]; values: pieces of 4 dims, two keys a word
+  const int k_to = ((((key_token >> 2) & 1) * HALVES + key_part % HALVES) * 64 + key_part / HALVES * 16 + (key_token >> 3) * 4 + (key_token & 3)) * 4 * KW;
+  const int v_to = v_m / (16 / G) * V_STRIDE + (v_blk * 16 + G * (v_m % (16 / G))) * 16 + v_sub * (D == 256 ? 4 : 8);
+  auto put = [&](int buf) {
+    unsigned char* to = step_lds(buf);
+    const StepLds st = StepLds::at<D>(to + L::KEYS);
+    if constexpr (KW == 4) st16(to + k_to, make_uint4(wk[0], wk[1], wk[2], wk[3]));
+    else *reinterpret_cast<uint2*>(to + k_to) = make_uint2(wk[0], wk[1]);
+    unsigned char* v = st.v + v_to;
+    if constexpr (D == 256) {              // two keys of 8 bytes: a word of four pieces
+#pragma unroll
+      for (int c = 0; c < 4; ++c) *reinterpret_cast<uint32_t*>(v + 16 * c) = __builtin_amdgcn_perm(wv[2 + c / 2], wv[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+    } else if constexpr (D == 128) {       // four keys of 4 bytes: two words of two pieces
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<uint2*>(v + 16 * c) = make_uint2(__builtin_amdgcn_perm(wv[1], wv[0], c ? 0x07060302u : 0x05040100u), __builtin_amdgcn_perm(wv[3], wv[2], c ? 0x07060302u : 0x05040100u));
+    } else *reinterpret_cast<uint2*>(v) = make_uint2(wv[0], wv[1]);
+    if (rg == 0) {
+      put_scales<D>(sb, there, st);
+      const unsigned mask = (unsigned)__ballot(there);
+      if (lane == 0) s_there[2 * ks + buf] = mask;
+    }
+  };
+
+  const int steps = key1 > key0 ? (key1 - key0 + KS * AT_STEP - 1) / (KS * AT_STEP) : 0;
+  int k0 = key0 + ks * AT_STEP;
+  KvPages ahead{};
+  if (steps > 0) { load(k0, pages(k0)); ahead = pages(k0 + KS * AT_STEP); }
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int in = pass * 16 + (tid >> 4);
+    put_query<D, BF>(raw[pass], in, in < rows_here, in < rows_here ? (int)max(0l, keys - n + (row0 + in) / group + 1) : NO_LIMIT, a.scale, sq);
+  }
+  lds_barrier();
+  if (steps > 0) put(0);
+  if (steps > 1) { load(k0 + KS * AT_STEP, ahead); ahead = pages(k0 + 2 * KS * AT_STEP); }
+  h8 qs[NT];
+  float mul[NT];
+  int limit[NT], most = 0;                             // keys that row n16 of tile nt sees, and that any row of this wave sees
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int in = rg * 16 * NT + nt * 16 + n16;
+    mul[nt] = s_mul[in]; limit[nt] = s_lim[in];
+    qs[nt] = __builtin_bit_cast(h8, kg == 0 ? s_qsum[in] : make_uint4(0, 0, 0, 0));
+  }
+  if (rg * 16 * NT < rows_here) most = (int)max(0l, min(keys, keys - n + (row0 + min((rg + 1) * 16 * NT, rows_here) - 1) / group + 1));
+  uint32_t ones = 0x64006400u, mask_lo = 0x000F000Fu, mask_hi = 0x00F000F0u;
+  asm volatile("" : "+v"(ones));
+  asm volatile("" : "+s"(mask_lo), "+s"(mask_hi));
+  f4 o[NT][G][4], ob[NT];
+  float m[NT], l[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt] = -__builtin_inff(); l[nt] = 0.0f; ob[nt] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[nt][g][i] = f4{0, 0, 0, 0};
+  }
+  lds_barrier();
+  for (int i = 0; i < steps; ++i, k0 += KS * AT_STEP) {
+    const int buf = i & 1;
+    if (k0 < most) {                                   // (the other key group may still have keys, and so may the rows of the other wave)
+      const unsigned char* from = step_lds(buf);
+      const StepLds st = StepLds::at<D>((unsigned char*)from + L::KEYS);
+      uint32_t k[2][D / 32];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int half = 0; half < HALVES; ++half) {
+          uint32_t w[KW];
+          load_words<KW>(w, from + ((c * HALVES + half) * 64 + lane) * 4 * KW);
+#pragma unroll
+          for (int j = 0; j < KW; ++j) k[c][half * KW + j] = w[j];
+        }
+      const unsigned here = s_there[2 * ks + buf];
+      float s[NT][8];
+      step_scores<D, NT>(k, [&](int nt, int w) { return __builtin_bit_cast(h8, s_q[((NT * rg + nt) * (D / 32) + w) * 64 + lane]); }, qs, st, mask_lo, mask_hi, s);
+      uint32_t pw[NT][G + 1][4];
+      step_weights<D, NT, NT>(s, here, k0, limit, mul, st, m, l, o, ob, pw);
+      step_values<D, NT, NT>(pw, st, ones, mask_lo, mask_hi, o, ob);
+    }
+    if (i + 1 < steps) put(buf ^ 1);
+    if (i + 2 < steps) { load(k0 + 2 * KS * AT_STEP, ahead); ahead = pages(k0 + 3 * KS * AT_STEP); }
+    lds_barrier();
+  }
+
+  // ---- the key groups' sums together ----
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt] = m[nt] * mul[nt];
+    l[nt] = rows4_sum(l[nt]);
+    const int in = (ks * RS + rg) * 16 * NT + nt * 16 + n16;
+    if (kg == 0) { s_m[in] = m[nt]; s_l[in] = l[nt]; }
+  }
+  float* s_o = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    lds_barrier();
+    float f = 1.0f;
+    if constexpr (KS == 2) {
+      const int in = rg * 16 * NT + nt * 16 + n16;
+      f = m[nt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - fmaxf(s_m[in], s_m[64 + in]));
+    }
+    put_sums<D>(o[nt], ob[nt], f, s_o + wave * 16 * (D + 4));
+    lds_barrier();
+    for (int i = tid; i < RS * 16 * (D / 4); i += 256) {
+      const int row = i / (D / 4), d = 4 * (i % (D / 4)), side = row >> 4, in = side * 16 * NT + nt * 16 + (row & 15);
+      if (in >= rows_here) continue;
+      float4 y = *reinterpret_cast<const float4*>(s_o + row * (D + 4) + d);
+      float best = s_m[in], sum = s_l[in];
+      if constexpr (KS == 2) {
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (RS * 16 + row) * (D + 4) + d);
+        y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+        const float m0 = best, m1 = s_m[64 + in];
+        best = fmaxf(m0, m1);
+        sum = sum * (m0 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m0 - best)) + s_l[64 + in] * (m1 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m1 - best));
+      }
+      const int row_of = row0 + in, tok = row_of / group;
+      put_row<D, BF>(a, cut, slot, in, start + tok, h * group + (row_of - tok * group), d, y, best, sum);
     }
   }
 }
@@ -957,7 +1211,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_a
   int start, n;
   const int rows = rows_of(a, r, start, n);
   if (row >= rows * group) return;
-  const int tile = row / tile_rows, in = row - tile * tile_rows, share = cut.first[a.n_req + 1];
+  const int in = row % tile_rows, tile = tile_rows == 64 ? (rows * group + 63) / 64 - 1 - row / 64 : row / tile_rows, share = cut.first[a.n_req + 1];
   const int count = parts_of(rounds_of(a, pool, r), share);
   if (count == 1) return;                               // one workgroup had all of it and wrote the row
   const long slot0 = cut.first[r] + (long)(tile * pool.n_kv + h) * count;
@@ -1025,7 +1279,7 @@ int pool_of(const sl_kv4_pool* p, Pool& out) {
 // How a call is cut, from what the host knows.
 struct AttnShape {
   AttnCut cut{};
-  int nt = 1;                 // row tiles of 16 in a workgroup
+  int tile = 16;              // rows of a workgroup
   int grid = 0;
   int64_t part_bytes = 0, bytes = 0;
 };
@@ -1045,11 +1299,11 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   const int64_t group = a->n_heads / p->n_kv, rows = (int64_t)std::min(a->max_rows, std::max(a->n_tokens, 1)) * group;
   const int64_t widest = (int64_t)a->table_width * p->page_size;
   if (a->n_req > AT_MAX_REQ || a->n_heads > 65535 || rows > (1ll << 30) || widest > 0x7fffffffLL - 4096) return SL_ERR_TOO_LARGE;
-  sh.nt = rows <= 16 ? 1 : 2;
-  const int tile = 16 * sh.nt;
+  sh.tile = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  const int tile = sh.tile;
   // items: by the most rows of a request, and by all rows of the call
   const int64_t items = p->n_kv * std::min(a->n_req * ((rows + tile - 1) / tile), a->n_tokens * group / tile + a->n_req);
-  const int64_t resident = (int64_t)compute_units() * (sh.nt * p->head_dim <= 256 ? 2 : 1);
+  const int64_t resident = (int64_t)compute_units() * (tile != 32 || p->head_dim <= 128 ? 2 : 1);
   const int64_t rounds = items * (std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1);
   if (p->n_kv * a->n_req * ((rows + tile - 1) / tile) + resident > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
   // with few items they and the parts together fill the chip once; more than half the places are shared out in any case
@@ -1061,18 +1315,19 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   sh.bytes = sh.part_bytes + ((a->n_req + 2) * 4 + 15) / 16 * 16;
   return SL_OK;
 }
-template <int D, bool BF, int NT>
-void launch_attn_nt(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, const AttnShape& sh, hipStream_t st) {
-  const int lds = AttnLds<D, NT>::BYTES + (a.n_req <= 64 ? 0 : (a.n_req + 1) * 4);
-  if (lds > 65536) (void)hipFuncSetAttribute((const void*)k_kv4_attn<D, BF, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL((k_kv4_attn<D, BF, NT>), dim3(sh.grid), dim3(256), lds, st, pool, a, cut);
+template <class K>
+void launch_attn_kernel(K kernel, int lds, const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, int grid, hipStream_t st) {
+  lds += a.n_req <= 64 ? 0 : (a.n_req + 1) * 4;
+  if (lds > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, st, pool, a, cut);
 }
 template <int D, bool BF>
 void launch_attn(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, const AttnShape& sh, hipStream_t st) {
-  if (sh.nt == 1) launch_attn_nt<D, BF, 1>(pool, a, cut, sh, st);
-  else launch_attn_nt<D, BF, 2>(pool, a, cut, sh, st);
+  if (sh.tile == 16) launch_attn_kernel(k_kv4_attn<D, BF, 1>, AttnLds<D, 1>::BYTES, pool, a, cut, sh.grid, st);
+  else if (sh.tile == 32) launch_attn_kernel(k_kv4_attn<D, BF, 2>, AttnLds<D, 2>::BYTES, pool, a, cut, sh.grid, st);
+  else launch_attn_kernel(k_kv4_attn_tile<D, BF>, TileLds<D>::BYTES, pool, a, cut, sh.grid, st);
   const int rows = std::min(a.max_rows, a.n_tokens) * (a.n_heads / pool.n_kv);
-  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut, 16 * sh.nt);
+  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut, sh.tile);
 }
 // f<D, BF>() for the pool's head_dim and an element type
 #define KV4_BY_LAYOUT(dim, bf, CALL)                                        \
