@@ -367,12 +367,13 @@ constexpr int AT_WAVES = 4, AT_STEP = 32, AT_UNIT = AT_WAVES * AT_STEP;   // key
 constexpr int AT_MAX_REQ = 4096;
 
 // How the work of a call is cut.  An item is a row tile of a request and a key/value head; its rounds of 128 keys are shared
-// out to ceil(rounds / share) workgroups, share = rounds of the whole call over `want` workgroups.  So every workgroup has one
-// part of one item: runs of equal length across items would need fewer workgroups, but one that ends an item and begins
-// another pays the start and the end twice, and the call waits for it (32 lanes: 47 us where the others end at 35).
-// The host launches want + items workgroups, which is enough whatever the lengths are; those behind the last part leave at once.
+// out to as many workgroups as its cost (rounds, weighted by the row tile's width) holds shares, a share being the cost of the
+// whole call over `want` workgroups.  So every workgroup has one part of one item: runs of equal length across items would need
+// fewer workgroups, but one that ends an item and begins another pays the start and the end twice, and the call
+// waits for it (32 lanes: 47 us where the others end at 35).  The host launches enough workgroups whatever the lengths are; those
+// behind the last part leave at once, as do those whose rows see fewer keys than the request has.
 struct AttnCut {
-  int want;           // workgroups to share the rounds out to
+  int want;           // workgroups to share the cost out to
   int rows;           // rows of a partial sum
   int32_t* first;     // [n_req + 1] parts before each request, then share (written by the first workgroup, for the merge)
   float* part;        // partial sums by workgroup: [grid][rows][D], then maxima [grid][rows], sums [grid][rows]
@@ -389,33 +390,50 @@ SL_DEV int rows_of(const sl_kv4_attn_args& a, int r, int& start, int& n) {
   if (start < 0 || n <= 0 || start >= a.n_tokens) return 0;
   return min(min(n, a.max_rows), a.n_tokens - start);
 }
-SL_DEV int rounds_of(const sl_kv4_attn_args& a, const Pool& pool, int r) {
-  return max(1, (int)((seen_keys(a, pool, r) + AT_UNIT - 1) / AT_UNIT));
-}
-// rounds of a part: total / want, rounded up (a quotient of doubles is exact where it is whole)
+SL_DEV int rounds_for(long keys) { return max(1, (int)((keys + AT_UNIT - 1) / AT_UNIT)); }
+// Cost of a round: a workgroup of 32 rows takes 4/3 of the time where more than 16 of them are there (measured 72 against 55 us).
+SL_DEV int round_cost(int tile_rows, int rows) { return tile_rows == 32 ? (rows > 16 ? 4 : 3) : 1; }
+SL_DEV int parts_of(int rounds, int cost, int share) { return (int)(((unsigned)rounds * (unsigned)cost + (unsigned)share - 1u) / (unsigned)share); }
+// cost of a part: total / want, rounded up (a quotient of doubles is exact where it is whole)
 SL_DEV int share_of(long total, int want) { return max(1, (int)fmin(ceil((double)total / (double)want), 2147483647.0)); }
-SL_DEV int parts_of(int rounds, int share) { return (int)(((unsigned)rounds + (unsigned)share - 1u) / (unsigned)share); }
-struct AttnPart { int r, tile, h, part, parts, share, rounds; };
+struct AttnPart { int r, tile, h, part, share; };
+// What a request asks for: its items, its most rounds, their cost, and the sum of its items' costs (row tiles further up see
+// fewer keys: their rounds lie evenly between the first tile's and the last's).
+template <int TILE>
+SL_DEV void request_work(const sl_kv4_attn_args& a, const Pool& pool, int r, int& items, int& rounds, int& cost, long& all) {
+  int start, n;
+  const int rows = rows_of(a, r, start, n), group = a.n_heads / pool.n_kv;
+  items = rounds = 0; cost = 1; all = 0;
+  if (rows <= 0) return;
+  const int tiles = (rows * group + TILE - 1) / TILE;
+  const long keys = seen_keys(a, pool, r);
+  items = tiles * pool.n_kv; rounds = rounds_for(min(keys, keys - n + rows)); cost = round_cost(TILE, rows * group);
+  const int least = rounds_for(keys - n + min(rows, TILE / group + 1));
+  all = (long)items * (rounds + (tiles > 1 ? least : rounds)) * cost / 2;
+}
+// Rounds of a row tile and how they are cut: `parts` of `per` rounds (at most parts_of() of the request's most rounds).
+template <int TILE>
+SL_DEV void tile_cut(long keys, int n, int rows_total, int tile, int group, int share, long& last, int& parts, int& per) {
+  const int end = min((tile + 1) * TILE, rows_total);             // rows in front of the tile's end
+  last = max(0l, min(keys, keys - n + (end - 1) / group + 1));    // keys that its last row sees
+  const int rounds = rounds_for(last);
+  parts = parts_of(rounds, round_cost(TILE, rows_total), share);
+  per = (rounds + parts - 1) / parts;
+}
 // The part that workgroup `idx` has; false if there is none.  Up to 64 requests: every wave finds it by itself, a request
 // per lane; more: the workgroup with running sums in LDS (s_first: n_req + 1 words, s_tmp: 12 words).
 template <int TILE>
 SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut& cut, int idx, int* s_first, int* s_tmp, AttnPart& out) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.n_heads / pool.n_kv, n = a.n_req;
-  auto of = [&](int r, int& items, int& rounds) {
-    int start, nn;
-    const int rows = rows_of(a, r, start, nn);
-    items = rows > 0 ? (rows * group + TILE - 1) / TILE * pool.n_kv : 0;
-    rounds = rows > 0 ? rounds_of(a, pool, r) : 0;
-  };
-  int before, items, rounds, share;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n_req;
+  int before, items, rounds, cost, share;
+  long all;
   if (n <= 64) {
-    items = rounds = 0;
-    if (lane < n) of(lane, items, rounds);
-    long total = (long)items * rounds;
+    items = rounds = 0; cost = 1; all = 0;
+    if (lane < n) request_work<TILE>(a, pool, lane, items, rounds, cost, all);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
-    share = share_of(total, cut.want);
-    const int own = items * parts_of(rounds, share);
+    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+    share = share_of(all, cut.want);
+    const int parts = parts_of(rounds, cost, share), own = items * parts;
     int upto = own;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; }
@@ -426,13 +444,13 @@ SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut
     const int r = __popcll(__ballot(upto <= idx));
     if (r >= n) return false;                      // (lanes behind n hold the total as well)
     out.r = r;
-    before = __builtin_amdgcn_readlane(upto - own, r); items = __builtin_amdgcn_readlane(items, r); rounds = __builtin_amdgcn_readlane(rounds, r);
+    before = __builtin_amdgcn_readlane(upto - own, r); rounds = __builtin_amdgcn_readlane(parts, r); items = __builtin_amdgcn_readlane(items, r);
   } else {
     const int per = (n + 255) / 256;
     long total = 0;
     for (int j = 0; j < per; ++j) {
       const int r = tid * per + j;
-      if (r < n) { of(r, items, rounds); total += (long)items * rounds; }
+      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, cost, all); total += all; }
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
@@ -444,32 +462,35 @@ SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut
     int own = 0;
     for (int j = 0; j < per; ++j) {
       const int r = tid * per + j;
-      if (r < n) { of(r, items, rounds); own += items * parts_of(rounds, share); }
+      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, cost, all); own += items * parts_of(rounds, cost, share); }
     }
     int upto = own;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; }
     if (lane == 63) s_tmp[8 + wave] = upto;
     __syncthreads();
-    int at = upto - own, all = 0;
+    int at = upto - own, sum = 0;
 #pragma unroll
-    for (int w = 0; w < AT_WAVES; ++w) { if (w < wave) at += s_tmp[8 + w]; all += s_tmp[8 + w]; }
+    for (int w = 0; w < AT_WAVES; ++w) { if (w < wave) at += s_tmp[8 + w]; sum += s_tmp[8 + w]; }
     for (int j = 0; j < per; ++j) {
       const int r = tid * per + j;
-      if (r < n) { of(r, items, rounds); s_first[r] = at; at += items * parts_of(rounds, share); }
+      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, cost, all); s_first[r] = at; at += items * parts_of(rounds, cost, share); }
     }
-    if (tid == 0) s_first[n] = all;
+    if (tid == 0) s_first[n] = sum;
     __syncthreads();
     if (idx == 0) for (int i = tid; i <= n + 1; i += 256) cut.first[i] = i <= n ? s_first[i] : share;
-    if (idx >= all) return false;
+    if (idx >= sum) return false;
     out.r = __builtin_amdgcn_readfirstlane(owner_of(s_first, n, idx));
     before = s_first[out.r];
-    of(out.r, items, rounds);
+    request_work<TILE>(a, pool, out.r, items, rounds, cost, all);
+    rounds = parts_of(rounds, cost, share);
   }
-  out.share = share; out.rounds = rounds;
-  out.parts = parts_of(rounds, share);
-  const int in = idx - before, item = in / out.parts;
-  out.part = in - item * out.parts;
+  // (rounds: from here on the most parts of an item.)  Workgroups go round the eight XCDs in turn: eight items side by side, part
+  // after part, so that every XCD gets items of all lengths and their later parts, which the shorter items lack, alike.
+  const int in = idx - before, full = items & ~7, side = in < full * rounds ? 8 : items - full;
+  const int from = in < full * rounds ? in / (8 * rounds) * 8 : full, rest = in - from * rounds, item = from + rest % side;
+  out.share = share;
+  out.part = rest / side;
   out.tile = item / pool.n_kv; out.h = item - out.tile * pool.n_kv;
   return true;
 }
@@ -485,7 +506,6 @@ SL_DEV float swap32_max(float v) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 SL_DEV float rows4_max(float v) { return swap32_max(swap16_max(v)); }     // over the four rows of 16 lanes
-SL_DEV float rows4_sum(float v) { return swap32_sum(swap16_sum(v)); }
 SL_DEV float nth_half(const uint32_t* w, int i) { return i & 1 ? hi_h(w[i / 2]) : lo_h(w[i / 2]); }
 SL_DEV uint32_t half_pair(float a, float b) { return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16); }
 SL_DEV uint32_t pair_of(float a, float b) { return __builtin_bit_cast(uint32_t, h2_t{(_Float16)a, (_Float16)b}); }   // (a product and its rounding may become one instruction)
@@ -513,6 +533,7 @@ SL_DEV void load_words(uint32_t* to, const unsigned char* p) {
 struct KvPages { int k, v, sb; };
 
 // ---- one step of 32 keys: the parts that the kernels share ----
+constexpr uint32_t mask_lo = 0x000F000Fu, mask_hi = 0x00F000F0u;       // nibbles 0 | 4 and 1 | 5 of a word: as halves, code * 2^-24 and code * 2^-20
 constexpr int V_STRIDE = 64 * 16 + 16;        // bytes of a group's value pieces: [quarter of the keys][16 lanes][8 keys x 4 dims], padded against bank conflicts
 // LDS of a step as the lanes read it.
 struct StepLds {
@@ -574,7 +595,7 @@ SL_DEV void put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& 
 // s[row tile][8]: this lane's keys 8 kg .. 8 kg + 7 against row n16.  All products of the step first, so that no scale waits for
 // the product before it.  `query(nt, i)`: the operand of dims word i; k: the two key operands' words.
 template <int D, int LIVE, class Q, int NT>
-SL_DEV void step_scores(const uint32_t (&k)[2][D / 32], Q query, const h8 (&qs)[NT], const StepLds& st, uint32_t mask_lo, uint32_t mask_hi, float (&s)[LIVE][8]) {
+SL_DEV void step_scores(const uint32_t (&k)[2][D / 32], Q query, const h8 (&qs)[NT], const StepLds& st, float (&s)[LIVE][8]) {
   constexpr int G = D / 64;
   const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
   f4 acc[LIVE][2][G], accb[LIVE][2];
@@ -622,7 +643,7 @@ SL_DEV void step_scores(const uint32_t (&k)[2][D / 32], Q query, const h8 (&qs)[
 // The running maximum per row, p relative to it; pw: the operands p s_g of each group, then p itself.
 template <int D, int LIVE, int NT>
 SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int (&limit)[NT], const float (&mul)[NT], const StepLds& st, float (&m)[NT],
-                         float (&l)[NT], f4 (&o)[NT][D / 64][4], f4 (&ob)[NT], uint32_t (&pw)[LIVE][D / 64 + 1][4]) {
+                         f4 (&o)[NT][D / 64][4], f4 (&ob)[NT], uint32_t (&pw)[LIVE][D / 64 + 1][4]) {
   constexpr int G = D / 64;
   const int lane = threadIdx.x & 63, kg = lane >> 4;
   uint32_t vs[4 * G];
@@ -637,25 +658,25 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
       for (int t = 0; t < 8; ++t)
         if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) { s[nt][t] = -__builtin_inff(); keep[t / 2] &= t & 1 ? 0x0000ffffu : 0xffff0000u; }
     }
-    float top = m[nt];
+    float top = s[nt][0];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) top = fmaxf(top, s[nt][t]);
+    for (int t = 1; t < 8; ++t) top = fmaxf(top, s[nt][t]);
     top = rows4_max(top);
-    const float ref = top == -__builtin_inff() ? 0.0f : top;
-    if (__any(top != m[nt])) {
-      const float back = __builtin_amdgcn_exp2f((m[nt] - ref) * mul[nt]);
-      l[nt] = l[nt] * back; ob[nt] = ob[nt] * back;
+    // The reference moves only where a row's maximum has grown past it by a factor of 2^2.875 = 7.3: until then p lies above 1, and
+    // p s stays within fp16 (|s| < 8734.1, for no value lies beyond 65504).
+    if (__any((top - m[nt]) * mul[nt] > 2.875f)) {
+      const float next = fmaxf(m[nt], top), back = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m[nt] - next) * mul[nt]);
+      ob[nt] = ob[nt] * back;
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
-      m[nt] = top;
+      m[nt] = next;
     }
-    const float from = -ref * mul[nt];
+    const float from = m[nt] == -__builtin_inff() ? 0.0f : -m[nt] * mul[nt];
     float p[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(fmaf(s[nt][t], mul[nt], from));
-    l[nt] = l[nt] + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
 #pragma unroll
     for (int t = 0; t < 4; ++t) pw[nt][G][t] = pair_of(p[2 * t], p[2 * t + 1]);
 #pragma unroll
@@ -670,11 +691,26 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
     }
   }
 }
+// Values: o[group][i] gathers (p s_g) c of the dims 4 m' + i, in units of 2^-24 (odd i: 2^-20, the nibble standing four bits up).
+// Codes run from 0, so the rounding of p s_g is as large as c makes it; ob takes what brings it back to c - 8: row g of ob
+// is sum p (b_g + 8 s_g), row 8 + g the sum of the rounded p s_g (times 8 to be taken off), row G the sum of p, the softmax's own.
+template <int D>
+struct OnesRows { h8 at[D / 64]; };              // per group: an operand whose row 8 + g is ones
+template <int D>
+SL_DEV OnesRows<D> ones_rows() {
+  constexpr int G = D / 64;
+  const int n16 = threadIdx.x & 15;
+  OnesRows<D> r;
+#pragma unroll
+  for (int g = 0; g < G; ++g) { const uint32_t x = n16 == 8 + g ? 0x3c003c00u : 0u; r.at[g] = __builtin_bit_cast(h8, make_uint4(x, x, x, x)); }
+  return r;
+}
 template <int D, int LIVE, int NT>
-SL_DEV void step_values(const uint32_t (&pw)[LIVE][D / 64 + 1][4], const StepLds& st, uint32_t ones, uint32_t mask_lo, uint32_t mask_hi, f4 (&o)[NT][D / 64][4], f4 (&ob)[NT]) {
+SL_DEV void step_values(const uint32_t (&pw)[LIVE][D / 64 + 1][4], const StepLds& st, const OnesRows<D>& ones, f4 (&o)[NT][D / 64][4], f4 (&ob)[NT]) {
   constexpr int G = D / 64;
   const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
-  uint4 vb = make_uint4(0, 0, 0, 0);
+  const uint32_t one = n16 == G ? 0x3c003c00u : 0u;
+  uint4 vb = make_uint4(one, one, one, one);
   if (n16 < G) vb = *reinterpret_cast<const uint4*>(st.vb + n16 * AT_STEP + 8 * kg);
 #pragma unroll
   for (int nt = 0; nt < LIVE; ++nt)
@@ -683,23 +719,25 @@ SL_DEV void step_values(const uint32_t (&pw)[LIVE][D / 64 + 1][4], const StepLds
   for (int g = 0; g < G; ++g) {
     const uint4 raw = ld16(st.v + g * V_STRIDE + lane * 16);
     const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+    h8 weight[LIVE];
+#pragma unroll
+    for (int nt = 0; nt < LIVE; ++nt) weight[nt] = __builtin_bit_cast(h8, make_uint4(pw[nt][g][0], pw[nt][g][1], pw[nt][g][2], pw[nt][g][3]));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t w[4];
-      const h2_t off = i & 1 ? h2_t{(_Float16)-1152.0f, (_Float16)-1152.0f} : h2_t{(_Float16)-1032.0f, (_Float16)-1032.0f};
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t y = i & 2 ? x[t] >> 8 : x[t];
-        w[t] = __builtin_bit_cast(uint32_t, as_h2((y & (i & 1 ? mask_hi : mask_lo)) | ones) + off);
-      }
+      for (int t = 0; t < 4; ++t) w[t] = (i & 2 ? x[t] >> 8 : x[t]) & (i & 1 ? mask_hi : mask_lo);
       const h8 vf = __builtin_bit_cast(h8, make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-      for (int nt = 0; nt < LIVE; ++nt)
-        o[nt][g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(h8, make_uint4(pw[nt][g][0], pw[nt][g][1], pw[nt][g][2], pw[nt][g][3])), o[nt][g][i], 0, 0, 0);
+      for (int nt = 0; nt < LIVE; ++nt) o[nt][g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, weight[nt], o[nt][g][i], 0, 0, 0);
     }
+#pragma unroll
+    for (int nt = 0; nt < LIVE; ++nt) ob[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones.at[g], weight[nt], ob[nt], 0, 0, 0);
   }
-        
 }
+// The softmax's sum of row n16.
+template <int D>
+SL_DEV float sum_of(const f4& ob) { return __shfl(ob[D / 64 % 4], (int)(threadIdx.x & 15) + 16 * (D / 256)); }
 
 template <int D, int NT>
 struct AttnLds {
@@ -787,16 +825,16 @@ SL_DEV void finish_row(const sl_kv4_attn_args& a, int t, int head, int d, float4
 template <int D>
 SL_DEV void put_sums(const f4 (&o)[D / 64][4], const f4& ob, float f, float* to) {
   const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
-  float bias[4];
+  float bias[D / 64];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) bias[g] = __shfl(ob[g], n16);
+  for (int g = 0; g < D / 64; ++g) bias[g] = fmaf(-8.0f, __shfl(ob[g], n16 + 32), __shfl(ob[g], n16));
 #pragma unroll
   for (int g = 0; g < D / 64; ++g)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float4 y;
-      y.x = (o[g][0][r] + bias[g]) * f; y.y = fmaf(o[g][1][r], 0.0625f, bias[g]) * f;
-      y.z = (o[g][2][r] + bias[g]) * f; y.w = fmaf(o[g][3][r], 0.0625f, bias[g]) * f;
+      y.x = fmaf(o[g][0][r], 16777216.0f, bias[g]) * f; y.y = fmaf(o[g][1][r], 1048576.0f, bias[g]) * f;
+      y.z = fmaf(o[g][2][r], 16777216.0f, bias[g]) * f; y.w = fmaf(o[g][3][r], 1048576.0f, bias[g]) * f;
       *reinterpret_cast<float4*>(to + n16 * (D + 4) + 64 * g + 16 * kg + 4 * r) = y;
     }
 }
@@ -811,8 +849,10 @@ SL_DEV void put_row(const sl_kv4_attn_args& a, const AttnCut& cut, long slot, in
   }
 }
 
+// Workgroups on a compute unit: by the registers, of which the running sums alone take NT * D / 4.
+constexpr int attn_places(int dim, int nt) { return dim == 64 ? (nt == 1 ? 4 : 3) : (dim == 128 && nt == 1 ? 3 : 2); }
 template <int D, bool BF, int NT>
-__global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
+__global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
   using L = AttnLds<D, NT>;
   constexpr int G = L::G;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -821,7 +861,7 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
   int* s_lim = reinterpret_cast<int*>(s_mul + 16 * NT);
   uint4* s_qsum = reinterpret_cast<uint4*>(s_lim + 16 * NT);
   int* s_first = reinterpret_cast<int*>(lds + L::BYTES);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kg = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, kg = lane >> 4;
   const StepLds st = StepLds::at<D>(lds + wave * L::WAVE);
   uint4* s_q = reinterpret_cast<uint4*>(lds + AT_WAVES * L::WAVE);
   const QueryLds sq{s_q, s_qsum, s_mul, s_lim};
@@ -835,11 +875,13 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
     const int r = at.r, h = at.h;
     int start, n;
     const int rows = rows_of(a, r, start, n), row0 = at.tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);
-    const long keys = seen_keys(a, pool, r), slot = at.parts > 1 ? (long)blockIdx.x : -1;
-    // keys that the tile's last row sees
-    const long last = max(0l, min(keys, keys - n + (row0 + rows_here - 1) / group + 1));
-    const int key0 = at.part * at.share * AT_UNIT, key1 = (int)min((long)min(at.rounds, (at.part + 1) * at.share) * AT_UNIT, last);
-
+    const long keys = seen_keys(a, pool, r);
+    long last;
+    int parts, per;
+    tile_cut<16 * NT>(keys, n, rows * group, at.tile, group, at.share, last, parts, per);
+    if (at.part >= parts) return;
+    const long slot = parts > 1 ? (long)blockIdx.x : -1;
+    const int key0 = at.part * per * AT_UNIT, key1 = (int)min((long)(at.part + 1) * per * AT_UNIT, last);
     const int32_t* table = a.table + (size_t)r * a.table_width;
     const int end_page = key1 > 0 ? (key1 - 1) >> shift : 0;
     auto pages = [&](int k0) {
@@ -906,15 +948,12 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
       qs[nt] = __builtin_bit_cast(h8, kg == 0 ? s_qsum[nt * 16 + n16] : make_uint4(0, 0, 0, 0));
     }
 
-    // 1024 in both halves, kept in a register: with the mask as a scalar, (x & mask) | 1024 is one instruction
-    uint32_t ones = 0x64006400u, mask_lo = 0x000F000Fu, mask_hi = 0x00F000F0u;
-    asm volatile("" : "+v"(ones));
-    asm volatile("" : "+s"(mask_lo), "+s"(mask_hi));
+    const OnesRows<D> ones = ones_rows<D>();
     f4 o[NT][G][4], ob[NT];
-    float m[NT], l[NT];                                  // running maximum (of scores before the factor) and this lane's sum of p
+    float m[NT];                                         // the reference of p, in scores before the factor
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = -__builtin_inff(); l[nt] = 0.0f; ob[nt] = f4{0, 0, 0, 0};
+      m[nt] = -__builtin_inff(); ob[nt] = f4{0, 0, 0, 0};
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -947,11 +986,11 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
         step_scores<D, LIVE>(cur.k, [&](int nt, int i) {
           if constexpr (Q_REGS) return q[i];
           else return __builtin_bit_cast(h8, s_q[(nt * (D / 32) + i) * 64 + lane]);
-        }, qs, st, mask_lo, mask_hi, s);
+        }, qs, st, s);
         if (more) { load_keys(k0 + AT_UNIT, ahead, cur); ahead = pages(k0 + 2 * AT_UNIT); }
         uint32_t pw[LIVE][G + 1][4];
-        step_weights<D, LIVE, NT>(s, there, k0, limit, mul, st, m, l, o, ob, pw);
-        step_values<D, LIVE, NT>(pw, st, ones, mask_lo, mask_hi, o, ob);
+        step_weights<D, LIVE, NT>(s, there, k0, limit, mul, st, m, o, ob, pw);
+        step_values<D, LIVE, NT>(pw, st, ones, o, ob);
       }
     };
     if (NT == 1 || rows_here <= 16) keys_loop(std::integral_constant<int, 1>{});
@@ -962,8 +1001,8 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
     // ---- the four waves' sums together; lane (n16, kg) holds dims 64 g + 16 kg + 4 r + i of row n16 ----
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      l[nt] = rows4_sum(l[nt]);
-      if (kg == 0) { s_m[wave * 16 * NT + nt * 16 + n16] = m[nt]; s_l[wave * 16 * NT + nt * 16 + n16] = l[nt]; }
+      const float sum = sum_of<D>(ob[nt]);
+      if (kg == 0) { s_m[wave * 16 * NT + nt * 16 + n16] = m[nt]; s_l[wave * 16 * NT + nt * 16 + n16] = sum; }
     }
     float* s_o = reinterpret_cast<float*>(lds);
 #pragma unroll
@@ -998,34 +1037,34 @@ __global__ __launch_bounds__(256, NT * D <= 256 ? 2 : 1) void k_kv4_attn(Pool po
   }
 }
 
-// Many rows: a workgroup takes 64 rows.  Its waves lay a step's bytes out in LDS together, a step ahead of its use, so the registers
-// hold no bytes but those on their way.  Dims of 256: each wave has 16 rows (the sums of 32 would not leave room for two waves a
-// SIMD) and all keys.  Fewer dims: two waves of 32 rows each take every second step, two the others, and a step is unpacked
-// for 32 rows at once; the two key groups' sums are joined at the end.
+// Many rows of 256 dims: a workgroup takes 64 rows, each wave 16 of them and all keys (the sums of 32 rows would not leave room for two
+// waves a SIMD).  The waves lay a step's bytes out in LDS together, a step ahead of its use, so the registers hold no bytes but
+// those on their way.  (With fewer dims a wave has room for 32 rows, and waves that unpack their own keys are faster than
+// ones that meet at a barrier every step: 64 rows of 128 dims against 32K keys 121 us, with this kernel's scheme 190.)
 template <int D>
 struct TileLds {
   static constexpr int KEYS = 16 * D;                                  // key words in the order of the lanes
   static constexpr int STEP = KEYS + StepLds::bytes<D>();
-  static constexpr int KS = D == 256 ? 1 : 2;                          // key groups
   static constexpr int Q = 4 * (D / 32) * 64 * 16;
   static constexpr int JOIN = 4 * 16 * (D + 4) * 4;
-  static constexpr int MAIN = 2 * KS * STEP + Q > JOIN ? 2 * KS * STEP + Q : JOIN;
-  static constexpr int STAT = (2 * KS + 2 + 4) * 64 * 4;
+  static constexpr int MAIN = 2 * STEP + Q > JOIN ? 2 * STEP + Q : JOIN;
+  static constexpr int STAT = (2 + 2 + 4) * 64 * 4;
   static constexpr int BYTES = MAIN + STAT;
 };
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
   using L = TileLds<D>;
-  constexpr int G = D / 64, KS = L::KS, RS = 4 / KS, NT = KS, KW = D >= 128 ? 4 : 2, HALVES = D == 256 ? 2 : 1;     // KW: words that a thread brings of keys and of values
+  static_assert(D == 256, "a thread brings 16 bytes of keys and of values, half a lane's quarter row");
+  constexpr int G = D / 64, NT = 1, KW = 4, HALVES = 2;
   extern __shared__ __align__(16) unsigned char lds[];
   float* s_m = reinterpret_cast<float*>(lds + L::MAIN);
-  float *s_l = s_m + KS * 64, *s_mul = s_l + KS * 64;
+  float *s_l = s_m + 64, *s_mul = s_l + 64;
   int* s_lim = reinterpret_cast<int*>(s_mul + 64);
   uint4* s_qsum = reinterpret_cast<uint4*>(s_lim + 64);
   int* s_first = reinterpret_cast<int*>(lds + L::BYTES);
-  uint4* s_q = reinterpret_cast<uint4*>(lds + 2 * KS * L::STEP);
+  uint4* s_q = reinterpret_cast<uint4*>(lds + 2 * L::STEP);
   const QueryLds sq{s_q, s_qsum, s_mul, s_lim};
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, kg = lane >> 4, rg = wave % RS, ks = wave / RS, t2 = tid % (RS * 64);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, kg = lane >> 4;
   const int group = a.n_heads / pool.n_kv, shift = pool.page_shift, page_mask = (1 << shift) - 1;
   const uint32_t page_stride = (uint32_t)(pool.n_kv * (int)head_bytes<D>(pool));
   const int part_c = (D / 2) << shift, part_sb = (D / 16) << shift;
@@ -1035,10 +1074,14 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
   const int r = at.r, h = at.h;
   int start, n;
   const int rows = rows_of(a, r, start, n), tiles = (rows * group + 63) / 64;
-  const int row0 = (tiles - 1 - at.tile) * 64, rows_here = min(64, rows * group - row0);      // the tiles that see most keys first
-  const long keys = seen_keys(a, pool, r), slot = at.parts > 1 ? (long)blockIdx.x : -1;
-  const long last = max(0l, min(keys, keys - n + (row0 + rows_here - 1) / group + 1));
-  const int key0 = at.part * at.share * AT_UNIT, key1 = (int)min((long)min(at.rounds, (at.part + 1) * at.share) * AT_UNIT, last);
+  const int tile = tiles - 1 - at.tile, row0 = tile * 64, rows_here = min(64, rows * group - row0);      // the tiles that see most keys first
+  const long keys = seen_keys(a, pool, r);
+  long last;
+  int parts, per;
+  tile_cut<64>(keys, n, rows * group, tile, group, at.share, last, parts, per);
+  if (at.part >= parts) return;
+  const long slot = parts > 1 ? (long)blockIdx.x : -1;
+  const int key0 = at.part * per * AT_UNIT, key1 = (int)min((long)(at.part + 1) * per * AT_UNIT, last);
 
   uint2 raw[4][D / 64];
 #pragma unroll
@@ -1049,7 +1092,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
     for (int c = 0; c < D / 64; ++c) raw[pass][c] = *reinterpret_cast<const uint2*>(src + 4 * c);
   }
 
-  // A step's bytes by the key group's threads: 16 bytes each of keys and values (8 for dims of 64).
+  // A step's bytes: 16 each of keys and values by every thread, scales and biases by the first wave.
   const int32_t* table = a.table + (size_t)r * a.table_width;
   const int end_page = key1 > 0 ? (key1 - 1) >> shift : 0;
   const unsigned char* head_base = pool.pages + (size_t)h * head_bytes<D>(pool);
@@ -1057,52 +1100,45 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
   auto page_of = [&](int key) { return table[min(key >> shift, end_page)]; };
   uint32_t wk[KW], wv[KW], sb[G];
   bool there = false;
-  const int key_token = t2 & 31, key_part = t2 >> 5;
+  const int key_token = tid & 31, key_part = tid >> 5;
   constexpr int V_UNITS = D / 16 / KW;                                 // threads to a lane's 8 keys
-  const int v_blk = t2 / (16 * V_UNITS), v_m = (t2 / V_UNITS) & 15, v_sub = t2 % V_UNITS;
+  const int v_blk = tid / (16 * V_UNITS), v_m = (tid / V_UNITS) & 15, v_sub = tid % V_UNITS;
   auto pages = [&](int k0) {
     KvPages p;
-    p.k = page_of(k0 + key_token); p.v = page_of(k0 + 8 * v_blk); p.sb = rg == 0 ? page_of(k0 + (lane & 31)) : 0;
+    p.k = page_of(k0 + key_token); p.v = page_of(k0 + 8 * v_blk); p.sb = wave == 0 ? page_of(k0 + (lane & 31)) : 0;
     return p;
   };
   auto load = [&](int k0, const KvPages& p) {
     load_words<KW>(wk, base(p.k) + ((k0 + key_token) & page_mask) * (D / 2) + 4 * KW * key_part);
-    load_words<KW>(wv, base(p.v) + part_c + part_sb + (((k0 + 8 * v_blk) & page_mask) >> 3) * (4 * D) + (t2 % (16 * V_UNITS)) * (4 * KW));
-    if (rg == 0) {
+    load_words<KW>(wv, base(p.v) + part_c + part_sb + (((k0 + 8 * v_blk) & page_mask) >> 3) * (4 * D) + (tid % (16 * V_UNITS)) * (4 * KW));
+    if (wave == 0) {
       load_words<G>(sb, base(p.sb) + (lane < 32 ? part_c : 2 * part_c + part_sb) + ((k0 + (lane & 31)) & page_mask) * (D / 16));
       there = (unsigned)p.sb < (unsigned)pool.n_pages && k0 + (lane & 31) < key1;
     }
   };
-  auto step_lds = [&](int buf) { return lds + (2 * ks + buf) * L::STEP; };
-  unsigned* s_there = reinterpret_cast<unsigned*>(s_m);                // [key group][buffer], free until the end
+  auto step_lds = [&](int buf) { return lds + buf * L::STEP; };
+  unsigned* s_there = reinterpret_cast<unsigned*>(s_m);                // by buffer; free until the end
   // keys: [operand][half of the row's quarter][quarter][row of the operand]; values: pieces of 4 dims, two keys a word
   const int k_to = ((((key_token >> 2) & 1) * HALVES + key_part % HALVES) * 64 + key_part / HALVES * 16 + (key_token >> 3) * 4 + (key_token & 3)) * 4 * KW;
-  const int v_to = v_m / (16 / G) * V_STRIDE + (v_blk * 16 + G * (v_m % (16 / G))) * 16 + v_sub * (D == 256 ? 4 : 8);
+  const int v_to = v_m / (16 / G) * V_STRIDE + (v_blk * 16 + G * (v_m % (16 / G))) * 16 + v_sub * 4;
   auto put = [&](int buf) {
     unsigned char* to = step_lds(buf);
     const StepLds st = StepLds::at<D>(to + L::KEYS);
-    if constexpr (KW == 4) st16(to + k_to, make_uint4(wk[0], wk[1], wk[2], wk[3]));
-    else *reinterpret_cast<uint2*>(to + k_to) = make_uint2(wk[0], wk[1]);
-    unsigned char* v = st.v + v_to;
-    if constexpr (D == 256) {              // two keys of 8 bytes: a word of four pieces
+    st16(to + k_to, make_uint4(wk[0], wk[1], wk[2], wk[3]));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) *reinterpret_cast<uint32_t*>(v + 16 * c) = __builtin_amdgcn_perm(wv[2 + c / 2], wv[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
-    } else if constexpr (D == 128) {       // four keys of 4 bytes: two words of two pieces
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<uint2*>(v + 16 * c) = make_uint2(__builtin_amdgcn_perm(wv[1], wv[0], c ? 0x07060302u : 0x05040100u), __builtin_amdgcn_perm(wv[3], wv[2], c ? 0x07060302u : 0x05040100u));
-    } else *reinterpret_cast<uint2*>(v) = make_uint2(wv[0], wv[1]);
-    if (rg == 0) {
+    for (int c = 0; c < 4; ++c)            // two keys of 8 bytes: a word of four pieces
+      *reinterpret_cast<uint32_t*>(st.v + v_to + 16 * c) = __builtin_amdgcn_perm(wv[2 + c / 2], wv[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
+    if (wave == 0) {
       put_scales<D>(sb, there, st);
       const unsigned mask = (unsigned)__ballot(there);
-      if (lane == 0) s_there[2 * ks + buf] = mask;
+      if (lane == 0) s_there[buf] = mask;
     }
   };
 
-  const int steps = key1 > key0 ? (key1 - key0 + KS * AT_STEP - 1) / (KS * AT_STEP) : 0;
-  int k0 = key0 + ks * AT_STEP;
+  const int steps = key1 > key0 ? (key1 - key0 + AT_STEP - 1) / (AT_STEP) : 0;
+  int k0 = key0;
   KvPages ahead{};
-  if (steps > 0) { load(k0, pages(k0)); ahead = pages(k0 + KS * AT_STEP); }
+  if (steps > 0) { load(k0, pages(k0)); ahead = pages(k0 + AT_STEP); }
 #pragma unroll
   for (int pass = 0; pass < 4; ++pass) {
     const int in = pass * 16 + (tid >> 4);
@@ -1110,153 +1146,150 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
   }
   lds_barrier();
   if (steps > 0) put(0);
-  if (steps > 1) { load(k0 + KS * AT_STEP, ahead); ahead = pages(k0 + 2 * KS * AT_STEP); }
+  if (steps > 1) { load(k0 + AT_STEP, ahead); ahead = pages(k0 + 2 * AT_STEP); }
   h8 qs[NT];
   float mul[NT];
   int limit[NT], most = 0;                             // keys that row n16 of tile nt sees, and that any row of this wave sees
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int in = rg * 16 * NT + nt * 16 + n16;
+    const int in = wave * 16 + n16;
     mul[nt] = s_mul[in]; limit[nt] = s_lim[in];
     qs[nt] = __builtin_bit_cast(h8, kg == 0 ? s_qsum[in] : make_uint4(0, 0, 0, 0));
   }
-  if (rg * 16 * NT < rows_here) most = (int)max(0l, min(keys, keys - n + (row0 + min((rg + 1) * 16 * NT, rows_here) - 1) / group + 1));
-  uint32_t ones = 0x64006400u, mask_lo = 0x000F000Fu, mask_hi = 0x00F000F0u;
-  asm volatile("" : "+v"(ones));
-  asm volatile("" : "+s"(mask_lo), "+s"(mask_hi));
+  if (wave * 16 < rows_here) most = (int)max(0l, min(keys, keys - n + (row0 + min((wave + 1) * 16, rows_here) - 1) / group + 1));
+  const OnesRows<D> ones = ones_rows<D>();
   f4 o[NT][G][4], ob[NT];
-  float m[NT], l[NT];
+  float m[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m[nt] = -__builtin_inff(); l[nt] = 0.0f; ob[nt] = f4{0, 0, 0, 0};
+    m[nt] = -__builtin_inff(); ob[nt] = f4{0, 0, 0, 0};
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[nt][g][i] = f4{0, 0, 0, 0};
   }
   lds_barrier();
-  for (int i = 0; i < steps; ++i, k0 += KS * AT_STEP) {
+  auto turn = [&](int i) {                             // the next step's bytes into LDS, those of the one after it asked for
+    if (i + 1 < steps) put((i & 1) ^ 1);
+    if (i + 2 < steps) { load(k0 + 2 * AT_STEP, ahead); ahead = pages(k0 + 3 * AT_STEP); }
+    lds_barrier();
+  };
+  const int mine = min(steps, max(0, (most - key0 + AT_STEP - 1) / AT_STEP));     // steps that any row of this wave sees
+  int i = 0;
+  for (; i < mine; ++i, k0 += AT_STEP) {
     const int buf = i & 1;
-    if (k0 < most) {                                   // (the other key group may still have keys, and so may the rows of the other wave)
-      const unsigned char* from = step_lds(buf);
-      const StepLds st = StepLds::at<D>((unsigned char*)from + L::KEYS);
-      uint32_t k[2][D / 32];
+    const unsigned char* from = step_lds(buf);
+    const StepLds st = StepLds::at<D>((unsigned char*)from + L::KEYS);
+    uint32_t k[2][D / 32];
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int half = 0; half < HALVES; ++half) {
-          uint32_t w[KW];
-          load_words<KW>(w, from + ((c * HALVES + half) * 64 + lane) * 4 * KW);
+      for (int half = 0; half < HALVES; ++half) {
+        uint32_t w[KW];
+        load_words<KW>(w, from + ((c * HALVES + half) * 64 + lane) * 4 * KW);
 #pragma unroll
-          for (int j = 0; j < KW; ++j) k[c][half * KW + j] = w[j];
-        }
-      const unsigned here = s_there[2 * ks + buf];
-      float s[NT][8];
-      step_scores<D, NT>(k, [&](int nt, int w) { return __builtin_bit_cast(h8, s_q[((NT * rg + nt) * (D / 32) + w) * 64 + lane]); }, qs, st, mask_lo, mask_hi, s);
-      uint32_t pw[NT][G + 1][4];
-      step_weights<D, NT, NT>(s, here, k0, limit, mul, st, m, l, o, ob, pw);
-      step_values<D, NT, NT>(pw, st, ones, mask_lo, mask_hi, o, ob);
-    }
-    if (i + 1 < steps) put(buf ^ 1);
-    if (i + 2 < steps) { load(k0 + 2 * KS * AT_STEP, ahead); ahead = pages(k0 + 3 * KS * AT_STEP); }
-    lds_barrier();
-  }
-
-  // ---- the key groups' sums together ----
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt] = m[nt] * mul[nt];
-    l[nt] = rows4_sum(l[nt]);
-    const int in = (ks * RS + rg) * 16 * NT + nt * 16 + n16;
-    if (kg == 0) { s_m[in] = m[nt]; s_l[in] = l[nt]; }
-  }
-  float* s_o = reinterpret_cast<float*>(lds);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    lds_barrier();
-    float f = 1.0f;
-    if constexpr (KS == 2) {
-      const int in = rg * 16 * NT + nt * 16 + n16;
-      f = m[nt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - fmaxf(s_m[in], s_m[64 + in]));
-    }
-    put_sums<D>(o[nt], ob[nt], f, s_o + wave * 16 * (D + 4));
-    lds_barrier();
-    for (int i = tid; i < RS * 16 * (D / 4); i += 256) {
-      const int row = i / (D / 4), d = 4 * (i % (D / 4)), side = row >> 4, in = side * 16 * NT + nt * 16 + (row & 15);
-      if (in >= rows_here) continue;
-      float4 y = *reinterpret_cast<const float4*>(s_o + row * (D + 4) + d);
-      float best = s_m[in], sum = s_l[in];
-      if constexpr (KS == 2) {
-        const float4 x = *reinterpret_cast<const float4*>(s_o + (RS * 16 + row) * (D + 4) + d);
-        y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
-        const float m0 = best, m1 = s_m[64 + in];
-        best = fmaxf(m0, m1);
-        sum = sum * (m0 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m0 - best)) + s_l[64 + in] * (m1 == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m1 - best));
+        for (int j = 0; j < KW; ++j) k[c][half * KW + j] = w[j];
       }
-      const int row_of = row0 + in, tok = row_of / group;
-      put_row<D, BF>(a, cut, slot, in, start + tok, h * group + (row_of - tok * group), d, y, best, sum);
-    }
+    const unsigned here = s_there[buf];
+    float s[NT][8];
+    step_scores<D, NT>(k, [&](int nt, int w) { return __builtin_bit_cast(h8, s_q[(wave * (D / 32) + w) * 64 + lane]); }, qs, st, s);
+    uint32_t pw[NT][G + 1][4];
+    step_weights<D, NT, NT>(s, here, k0, limit, mul, st, m, o, ob, pw);
+    step_values<D, NT, NT>(pw, st, ones, o, ob);
+    turn(i);
+  }
+  for (; i < steps; ++i, k0 += AT_STEP) turn(i);
+
+  // ---- rows out through LDS ----
+  m[0] = m[0] * mul[0];
+  const float total = sum_of<D>(ob[0]);
+  if (kg == 0) { s_m[wave * 16 + n16] = m[0]; s_l[wave * 16 + n16] = total; }
+  float* s_o = reinterpret_cast<float*>(lds);
+  put_sums<D>(o[0], ob[0], 1.0f, s_o + wave * 16 * (D + 4));
+  lds_barrier();
+  for (int i = tid; i < 64 * (D / 4); i += 256) {
+    const int in = i / (D / 4), d = 4 * (i % (D / 4));
+    if (in >= rows_here) break;
+    const int row = row0 + in, tok = row / group;
+    put_row<D, BF>(a, cut, slot, in, start + tok, h * group + (row - tok * group), d, *reinterpret_cast<const float4*>(s_o + in * (D + 4) + d), s_m[in], s_l[in]);
   }
 }
 
-// Partial sums of a row joined: a workgroup per (row, head, request).  A wave reads 256 / D partial rows at once, 16 bytes a
-// lane, four such loads in flight; the waves' sums meet in LDS.
-template <int D, bool BF>
-__global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut, int tile_rows) {
-  constexpr int LANES = D / 4, PER_WAVE = 64 / LANES, PER = 4 * PER_WAVE;
+// Partial sums joined.  TILE 16 or 32: a workgroup per row (there are many parts); its waves read 256 / D partial rows at once, 16
+// bytes a lane, four such loads in flight, and meet in LDS.  TILE 64: a wave per row (few parts), 16 rows a workgroup.
+template <int D, bool BF, int TILE>
+__global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
+  constexpr int LANES = D / 4, PER_WAVE = 64 / LANES, WAVES = TILE == 64 ? 1 : 4, PER = WAVES * PER_WAVE;
   __shared__ float s_red[4];
-  __shared__ float4 s_y[PER][LANES];
-  __shared__ float s_sum[PER];
-  const int row = blockIdx.x, h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.n_heads / pool.n_kv;
+  __shared__ float4 s_y[4 * PER_WAVE][LANES];
+  __shared__ float s_sum[4 * PER_WAVE];
+  const int h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.n_heads / pool.n_kv;
   int start, n;
-  const int rows = rows_of(a, r, start, n);
-  if (row >= rows * group) return;
-  const int in = row % tile_rows, tile = tile_rows == 64 ? (rows * group + 63) / 64 - 1 - row / 64 : row / tile_rows, share = cut.first[a.n_req + 1];
-  const int count = parts_of(rounds_of(a, pool, r), share);
-  if (count == 1) return;                               // one workgroup had all of it and wrote the row
-  const long slot0 = cut.first[r] + (long)(tile * pool.n_kv + h) * count;
-  if (slot0 + count > cut.slots) return;                // (row offsets that overlap: more parts than rows allow)
+  const int rows = rows_of(a, r, start, n), row_first = TILE == 64 ? blockIdx.x * 16 : blockIdx.x;
+  if (row_first >= rows * group) return;
+  const int tile = row_first / TILE, tiles = (rows * group + TILE - 1) / TILE, share = cut.first[a.n_req + 1];
+  const long keys = seen_keys(a, pool, r);
+  long last;
+  int count, per;
+  tile_cut<TILE>(keys, n, rows * group, tile, group, share, last, count, per);
+  if (count == 1) return;                               // one workgroup had all of it and wrote the rows
+  const int most = parts_of(rounds_for(min(keys, keys - n + rows)), round_cost(TILE, rows * group), share);      // parts that each item is numbered with
+  // as find_part numbers them: part i of the item stands at first + i * side
+  const int items = tiles * pool.n_kv, item = (TILE == 64 ? tiles - 1 - tile : tile) * pool.n_kv + h, full = items & ~7, side = item < full ? 8 : items - full;
+  const long first = cut.first[r] + (item < full ? (long)(item & ~7) * most + (item & 7) : (long)full * most + (item - full));
+  if (cut.first[r] + (long)items * most > cut.slots) return;      // (row offsets that overlap: more parts than rows allow)
   const float* stat = cut.part + cut.slots * cut.rows * D;
-  float best = -__builtin_inff();
-  for (int i = tid; i < count; i += 256) best = fmaxf(best, stat[(slot0 + i) * cut.rows + in]);
-  best = tree_max<64>(best);
-  if (lane == 0) s_red[wave] = best;
-  const int d = 4 * (lane % LANES), mine = wave * PER_WAVE + lane / LANES;
-  float4 y = make_float4(0, 0, 0, 0);
-  float sum = 0.0f;
-  __syncthreads();
-  best = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  for (int i = mine; i < count; i += 4 * PER) {
-    float4 p[4];
-    float m[4], l[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool in_range = i + u * PER < count;
-      const long slot = slot0 + (in_range ? i + u * PER : i);
-      p[u] = *reinterpret_cast<const float4*>(cut.part + (slot * cut.rows + in) * D + d);
-      m[u] = in_range ? stat[slot * cut.rows + in] : -__builtin_inff();
-      l[u] = stat[(cut.slots + slot) * cut.rows + in];
+  const int d = 4 * (lane % LANES), mine = (TILE == 64 ? 0 : wave * PER_WAVE) + lane / LANES;
+  for (int j = 0; j < (TILE == 64 ? 4 : 1); ++j) {
+    const int row = TILE == 64 ? row_first + wave * 4 + j : row_first, in = row % TILE;
+    if (row >= rows * group) return;
+    float best = -__builtin_inff();
+    for (int i = TILE == 64 ? lane : tid; i < count; i += 64 * WAVES) best = fmaxf(best, stat[(first + (long)i * side) * cut.rows + in]);
+    best = tree_max<64>(best);
+    if constexpr (TILE != 64) {
+      if (lane == 0) s_red[wave] = best;
+      __syncthreads();
+      best = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     }
+    float4 y = make_float4(0, 0, 0, 0);
+    float sum = 0.0f;
+    for (int i = mine; i < count; i += 4 * PER) {
+      float4 p[4];
+      float m[4], l[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (m[u] == -__builtin_inff()) continue;           // (a part in which the row sees no key)
-      const float f = __builtin_amdgcn_exp2f(m[u] - best);
-      sum = fmaf(f, l[u], sum);
-      y.x = fmaf(f, p[u].x, y.x); y.y = fmaf(f, p[u].y, y.y); y.z = fmaf(f, p[u].z, y.z); y.w = fmaf(f, p[u].w, y.w);
+      for (int u = 0; u < 4; ++u) {
+        const bool in_range = i + u * PER < count;
+        const long slot = first + (long)(in_range ? i + u * PER : i) * side;
+        p[u] = *reinterpret_cast<const float4*>(cut.part + (slot * cut.rows + in) * D + d);
+        m[u] = in_range ? stat[slot * cut.rows + in] : -__builtin_inff();
+        l[u] = stat[(cut.slots + slot) * cut.rows + in];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (m[u] == -__builtin_inff()) continue;         // (a part in which the row sees no key)
+        const float f = __builtin_amdgcn_exp2f(m[u] - best);
+        sum = fmaf(f, l[u], sum);
+        y.x = fmaf(f, p[u].x, y.x); y.y = fmaf(f, p[u].y, y.y); y.z = fmaf(f, p[u].z, y.z); y.w = fmaf(f, p[u].w, y.w);
+      }
     }
-  }
-  s_y[mine][lane % LANES] = y;
-  if (lane % LANES == 0) s_sum[mine] = sum;
-  __syncthreads();
-  if (tid >= LANES) return;
-  sum = 0.0f; y = make_float4(0, 0, 0, 0);
+    const int slot_y = TILE == 64 ? wave * PER_WAVE + lane / LANES : mine;
+    s_y[slot_y][lane % LANES] = y;
+    if (lane % LANES == 0) s_sum[slot_y] = sum;
+    if constexpr (TILE != 64) __syncthreads(); else wave_lds_order();
+    const int lead = TILE == 64 ? lane : tid;
+    if (lead < LANES) {
+      sum = 0.0f; y = make_float4(0, 0, 0, 0);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const float4 x = s_y[i][tid];
-    sum += s_sum[i]; y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+      for (int i = 0; i < PER; ++i) {
+        const int from = (TILE == 64 ? wave * PER_WAVE : 0) + i;
+        const float4 x = s_y[from][lead];
+        sum += s_sum[from]; y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+      }
+      const int tok = row / group;
+      finish_row<BF>(a, start + tok, h * group + (row - tok * group), 4 * lead, y, sum);
+    }
+    if constexpr (TILE == 64) wave_lds_order();
   }
-  const int tok = row / group;
-  finish_row<BF>(a, start + tok, h * group + (row - tok * group), 4 * tid, y, sum);
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------
@@ -1299,16 +1332,21 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   const int64_t group = a->n_heads / p->n_kv, rows = (int64_t)std::min(a->max_rows, std::max(a->n_tokens, 1)) * group;
   const int64_t widest = (int64_t)a->table_width * p->page_size;
   if (a->n_req > AT_MAX_REQ || a->n_heads > 65535 || rows > (1ll << 30) || widest > 0x7fffffffLL - 4096) return SL_ERR_TOO_LARGE;
-  sh.tile = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  // 256 dims: 16 rows a workgroup, from 49 rows on 64 (32 lanes of 32 rows 66 against 98 us, of 64 rows 140 against 103); fewer dims: a
+  // second row tile as soon as there are rows for it (128 dims, six requests of 32 rows at 20-32K: 71 against 83 us).
+  sh.tile = p->head_dim == 256 ? (rows <= 48 ? 16 : 64) : (rows <= 16 ? 16 : 32);
   const int tile = sh.tile;
   // items: by the most rows of a request, and by all rows of the call
   const int64_t items = p->n_kv * std::min(a->n_req * ((rows + tile - 1) / tile), a->n_tokens * group / tile + a->n_req);
-  const int64_t resident = (int64_t)compute_units() * (tile != 32 || p->head_dim <= 128 ? 2 : 1);
+  const int64_t resident = (int64_t)compute_units() * (tile == 64 ? 2 : attn_places(p->head_dim, tile / 16));
   const int64_t rounds = items * (std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1);
-  if (p->n_kv * a->n_req * ((rows + tile - 1) / tile) + resident > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
-  // with few items they and the parts together fill the chip once; more than half the places are shared out in any case
-  sh.cut.want = (int)std::min(std::max(resident - items, resident / 2), std::max<int64_t>(rounds, 1));
-  sh.grid = (int)(sh.cut.want + items);
+  if (p->n_kv * a->n_req * ((rows + tile - 1) / tile) + 2 * resident > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
+  // 16 and 32 rows: parts are equally long, so with few items they and the parts together fill the chip once; with more, parts of half
+  // a turn.  64 rows: row tiles see different numbers of keys, the longest first, and the chip takes parts as it gets free; tiles that
+  // fill it by themselves are cut where they are twice the mean (2048 rows of a prompt 147 us, cut at the mean 168).
+  sh.cut.want = (int)std::min(tile == 64 ? (items >= resident ? resident / 2 : resident) : (items <= resident / 2 ? resident - items : 2 * resident), std::max<int64_t>(rounds, 1));
+  // a request's items are numbered with the parts of its longest row tile: at most twice the mean of longest and shortest
+  sh.grid = (int)(2 * sh.cut.want + items);
   sh.cut.slots = sh.grid; sh.cut.rows = (int)std::min<int64_t>(rows, tile);
   sh.part_bytes = sh.cut.slots * sh.cut.rows * (p->head_dim + 2) * 4;
   sh.part_bytes = (sh.part_bytes + 15) & ~15ll;
@@ -1323,11 +1361,16 @@ void launch_attn_kernel(K kernel, int lds, const Pool& pool, const sl_kv4_attn_a
 }
 template <int D, bool BF>
 void launch_attn(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut, const AttnShape& sh, hipStream_t st) {
-  if (sh.tile == 16) launch_attn_kernel(k_kv4_attn<D, BF, 1>, AttnLds<D, 1>::BYTES, pool, a, cut, sh.grid, st);
-  else if (sh.tile == 32) launch_attn_kernel(k_kv4_attn<D, BF, 2>, AttnLds<D, 2>::BYTES, pool, a, cut, sh.grid, st);
-  else launch_attn_kernel(k_kv4_attn_tile<D, BF>, TileLds<D>::BYTES, pool, a, cut, sh.grid, st);
   const int rows = std::min(a.max_rows, a.n_tokens) * (a.n_heads / pool.n_kv);
-  hipLaunchKernelGGL((k_kv4_attn_merge<D, BF>), dim3(rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut, sh.tile);
+#define KV4_ATTN(TILE, KERNEL, LDS)                                                                            \
+  do {                                                                                                         \
+    launch_attn_kernel(KERNEL, LDS, pool, a, cut, sh.grid, st);                                                \
+    hipLaunchKernelGGL((k_kv4_attn_merge<D, BF, TILE>), dim3(TILE == 64 ? (rows + 15) / 16 : rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut); \
+  } while (0)
+  if (sh.tile == 16) KV4_ATTN(16, (k_kv4_attn<D, BF, 1>), (AttnLds<D, 1>::BYTES));
+  else if constexpr (D == 256) KV4_ATTN(64, (k_kv4_attn_tile<D, BF>), TileLds<D>::BYTES);
+  else KV4_ATTN(32, (k_kv4_attn<D, BF, 2>), (AttnLds<D, 2>::BYTES));
+#undef KV4_ATTN
 }
 // f<D, BF>() for the pool's head_dim and an element type
 #define KV4_BY_LAYOUT(dim, bf, CALL)                                        \
