@@ -451,7 +451,7 @@ int64_t sl_kv4_page_bytes(int page_size, int n_kv, int head_dim);
  * more pages than table_width, fewer held than ctx_len needs) is not served: it keeps what it holds, kv_len 0, slots -1
  * (its rows then read no key and write none), counted in `unserved`; after the first request that finds too few pages no
  * later one gets new pages.  Outputs are written whole: -1 behind the used entries of table_out and free_out, slot -1 and
- * pos 0 behind the last row.  n_req <= 4096, n_req * table_width < 2^31. */
+ * pos 0 behind the last row.  n_req <= 4096, n_req * table_width + n_free < 2^31. */
 typedef struct {
   int32_t n_req, table_width, n_free, page_size, max_tokens;
   const int32_t* ctx_len;        /* [n_req] */

@@ -51,7 +51,6 @@ SL_DEV void load4(const uint16_t* p, float* x) {
 // ---- page tables, slots and row offsets -----------------------------------------------------------------------------------
 constexpr int PLAN_MAX_REQ = 4096;
 constexpr int PLAN_THREADS = 512;
-constexpr int PLAN_PER = PLAN_MAX_REQ / PLAN_THREADS;
 
 // Sums in front of the caller's value over the workgroup, with sums capped at `cap` (the cap of a sum of capped sums is
 // the cap of the sum).  Returns the sum before this thread; `total` the sum of all.
@@ -87,66 +86,106 @@ SL_DEV int owner_of(const int* first, int n, int x) {
   return lo;
 }
 
-// Every workgroup forms the three running sums over the requests (rows, pages missing, pages given back) for itself, in
-// LDS, and then fills its share of the outputs, an element per thread and step: one launch, no exchange between
-// workgroups.  The requests' numbers are 12 bytes each and come from L2.
+// Every workgroup forms the running sums over the requests (rows; pages missing and pages given back) for itself, in LDS, and then
+// fills its share of the outputs: one launch, no exchange between workgroups.  The requests' numbers are 12 bytes each and
+// come from L2; up to 64 requests are one wave's work, without a barrier.
 __global__ __launch_bounds__(PLAN_THREADS) void k_kv4_plan(sl_kv4_plan_args a, int page_shift) {
   __shared__ int s_row[PLAN_MAX_REQ + 1], s_need[PLAN_MAX_REQ + 1], s_give[PLAN_MAX_REQ + 1];
   __shared__ unsigned s_wave[PLAN_THREADS / 64];
   __shared__ unsigned s_fit[PLAN_MAX_REQ / 32];     // the request is served
-  const int tid = threadIdx.x, n = a.n_req, per = (n + PLAN_THREADS - 1) / PLAN_THREADS, page = 1 << page_shift;
+  __shared__ unsigned s_taken, s_unserved;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n_req, page = 1 << page_shift;
   const int W = a.table_width;
+  const unsigned cap = (unsigned)a.max_tokens;
+  const unsigned count = (unsigned)min(max(a.free_count_in[0], 0), a.n_free);
   for (int i = tid; i < (n + 31) / 32; i += PLAN_THREADS) s_fit[i] = 0;
+  if (tid == 0) s_taken = s_unserved = 0;
 
-  unsigned rows = 0, cap = (unsigned)a.max_tokens;
-  for (int j = 0; j < per; ++j) {
-    const int r = tid * per + j;
-    if (r < n) rows = min(cap, rows + min(cap, (unsigned)max(a.new_len[r], 0)));
-  }
-  unsigned all_rows;
-  unsigned row = scan_before(rows, cap, s_wave, all_rows);
-  int need[PLAN_PER], give[PLAN_PER];
-  bool sane[PLAN_PER];
-  unsigned need_sum = 0, give_sum = 0;
-  for (int j = 0; j < per; ++j) {
-    const int r = tid * per + j;
-    need[j] = give[j] = 0; sane[j] = false;
-    if (r >= n) continue;
-    const int ctx = a.ctx_len[r], nw = a.new_len[r], held = a.held_in[r];
-    s_row[r] = (int)row;
+  // pages that a request misses and gives back, as far as its numbers make sense
+  auto pages_of = [&](int ctx, int nw, int held, unsigned row, unsigned& need, unsigned& give) {
     const long total = (long)ctx + nw;
     const bool fits = (unsigned)max(nw, 0) <= cap - row;
-    sane[j] = ctx >= 0 && nw >= 0 && fits && held >= 0 && held <= W && total <= ((long)W << page_shift) && ctx <= ((long)held << page_shift);
-    if (sane[j]) {
-      const int want = (int)((total + page - 1) >> page_shift);
-      need[j] = max(want - held, 0); give[j] = max(held - want, 0);
+    need = give = 0;
+    if (!(ctx >= 0 && nw >= 0 && fits && held >= 0 && held <= W && total <= ((long)W << page_shift) && ctx <= ((long)held << page_shift))) return false;
+    const int want = (int)((total + page - 1) >> page_shift);
+    need = (unsigned)max(want - held, 0); give = (unsigned)max(held - want, 0);
+    return true;
+  };
+  unsigned all_rows, all_need, all_give;
+  if (n <= 64) {
+    __syncthreads();
+    if (wave == 0) {
+      const bool there = lane < n;
+      const int ctx = there ? a.ctx_len[lane] : 0, nw = there ? a.new_len[lane] : 0, held = there ? a.held_in[lane] : 0;
+      unsigned x = min(cap, (unsigned)max(nw, 0));
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) { const unsigned y = (unsigned)__shfl_up((int)x, d); if (lane >= d) x = min(cap, x + y); }
+      unsigned row = (unsigned)__shfl_up((int)x, 1);
+      if (lane == 0) row = 0;
+      unsigned need, give;
+      const bool sane = pages_of(ctx, nw, held, row, need, give) && there;
+      unsigned nb = need, gb = give;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const unsigned y = (unsigned)__shfl_up((int)nb, d), z = (unsigned)__shfl_up((int)gb, d);
+        if (lane >= d) { nb += y; gb += z; }
+      }
+      const unsigned give_all = (unsigned)__shfl((int)gb, 63), have = count + give_all;
+      const bool fit = sane && (need == 0 || nb <= have);
+      if (there) { s_row[lane] = (int)row; s_need[lane] = (int)(nb - need); s_give[lane] = (int)(gb - give); }
+      unsigned taken = fit ? need : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) taken += (unsigned)__shfl_xor((int)taken, d);
+      const unsigned long long fits = __ballot(fit);
+      if (lane == 63) {
+        s_row[n] = (int)x; s_need[n] = (int)nb; s_give[n] = (int)gb;
+        s_taken = taken; s_unserved = (unsigned)(n - __popcll(fits));
+        if (n > 0) s_fit[0] = (unsigned)fits;
+        if (n > 32) s_fit[1] = (unsigned)(fits >> 32);
+      }
     }
-    row = min(cap, row + min(cap, (unsigned)max(nw, 0)));
-    need_sum += need[j]; give_sum += give[j];
+    __syncthreads();
+    all_rows = (unsigned)s_row[n]; all_give = (unsigned)s_give[n];
+  } else {
+    const int per = (n + PLAN_THREADS - 1) / PLAN_THREADS;
+    unsigned rows = 0;
+    for (int j = 0; j < per; ++j) {
+      const int r = tid * per + j;
+      if (r < n) rows = min(cap, rows + min(cap, (unsigned)max(a.new_len[r], 0)));
+    }
+    unsigned row = scan_before(rows, cap, s_wave, all_rows);
+    unsigned need_sum = 0, give_sum = 0, need, give;
+    unsigned at_row = row;
+    for (int j = 0; j < per; ++j) {
+      const int r = tid * per + j;
+      if (r >= n) continue;
+      const int nw = a.new_len[r];
+      pages_of(a.ctx_len[r], nw, a.held_in[r], at_row, need, give);
+      at_row = min(cap, at_row + min(cap, (unsigned)max(nw, 0)));
+      need_sum += need; give_sum += give;
+    }
+    unsigned nb = scan_before(need_sum, 0x7fffffffu, s_wave, all_need);
+    unsigned gb = scan_before(give_sum, 0x7fffffffu, s_wave, all_give);
+    const unsigned have = count + all_give;
+    unsigned taken = 0, unserved = 0;
+    for (int j = 0; j < per; ++j) {
+      const int r = tid * per + j;
+      if (r >= n) continue;
+      const int nw = a.new_len[r];
+      const bool sane = pages_of(a.ctx_len[r], nw, a.held_in[r], row, need, give);
+      s_row[r] = (int)row; s_need[r] = (int)nb; s_give[r] = (int)gb;
+      if (sane && (need == 0 || nb + need <= have)) { atomicOr(&s_fit[r >> 5], 1u << (r & 31)); taken += need; }
+      else ++unserved;
+      row = min(cap, row + min(cap, (unsigned)max(nw, 0)));
+      nb += need; gb += give;
+    }
+    if (taken) atomicAdd(&s_taken, taken);               // (whole numbers: in any order)
+    if (unserved) atomicAdd(&s_unserved, unserved);
+    if (tid == 0) { s_row[n] = (int)all_rows; s_need[n] = (int)all_need; s_give[n] = (int)all_give; }
+    __syncthreads();
   }
-  unsigned all_need, all_give;
-  unsigned nb = scan_before(need_sum, 0x7fffffffu, s_wave, all_need);
-  unsigned gb = scan_before(give_sum, 0x7fffffffu, s_wave, all_give);
-  const unsigned count = (unsigned)min(max(a.free_count_in[0], 0), a.n_free), have = count + all_give;
-  // pages taken = what the served requests miss; they are the first ones of the running sum
-  unsigned taken = 0;
-  int unserved = 0;
-  for (int j = 0; j < per; ++j) {
-    const int r = tid * per + j;
-    if (r >= n) continue;
-    s_need[r] = (int)nb; s_give[r] = (int)gb;
-    const bool fit = sane[j] && (need[j] == 0 || nb + need[j] <= have);
-    if (fit) { atomicOr(&s_fit[r >> 5], 1u << (r & 31)); taken += need[j]; }
-    else ++unserved;
-    nb += need[j]; gb += give[j];
-  }
-  unsigned all_taken, all_unserved;
-  scan_before(taken, 0x7fffffffu, s_wave, all_taken);
-  scan_before((unsigned)unserved, 0x7fffffffu, s_wave, all_unserved);
-  if (tid == 0) { s_row[n] = (int)all_rows; s_need[n] = (int)all_need; s_give[n] = (int)all_give; }
-  __syncthreads();
 
-  const int left = (int)(have - all_taken);
+  const int have = (int)(count + all_give), left = have - (int)s_taken;
   auto fit = [&](int r) { return (s_fit[r >> 5] >> (r & 31)) & 1u; };
   // entry x of the free list with the pages given back behind it
   auto free_at = [&](int x) {
@@ -158,13 +197,27 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_kv4_plan(sl_kv4_plan_args a, i
   auto page_at = [&](int r, int c, int held) {
     const int need_r = s_need[r + 1] - s_need[r];
     if (c < held - (s_give[r + 1] - s_give[r])) return a.table_in[(size_t)r * W + c];
-    if (c >= held && c < held + need_r && fit(r)) return free_at((int)have - 1 - s_need[r] - (c - held));
+    if (c >= held && c < held + need_r && fit(r)) return free_at(have - 1 - s_need[r] - (c - held));
     return -1;
   };
   const int step = gridDim.x * PLAN_THREADS, at = blockIdx.x * PLAN_THREADS + tid;
-  for (long i = at; i < (long)n * W; i += step) {
-    const int r = (int)(i / W), c = (int)(i - (long)r * W), held = min(max(a.held_in[r], 0), W);
-    a.table_out[i] = page_at(r, c, held);
+  for (int r = blockIdx.x; r < n; r += gridDim.x) {      // a workgroup per row of the table
+    const int held = min(max(a.held_in[r], 0), W), need_r = fit(r) ? s_need[r + 1] - s_need[r] : 0, kept = held - (s_give[r + 1] - s_give[r]);
+    const int32_t* from = a.table_in + (size_t)r * W;
+    int32_t* to = a.table_out + (size_t)r * W;
+    const int top = have - 1 - s_need[r] + held;
+#pragma unroll 4
+    for (int c = tid; c < W; c += PLAN_THREADS) {
+      int id = -1;
+      if (c < kept) id = from[c];
+      else if (c >= held && c < held + need_r) id = free_at(top - c);
+      to[c] = id;
+    }
+    if (tid == 0) {
+      a.held_out[r] = kept + need_r;
+      a.kv_len[r] = fit(r) ? a.ctx_len[r] + a.new_len[r] : 0;
+      a.q_start[r] = s_row[r];
+    }
   }
   for (int i = at; i < a.n_free; i += step) a.free_out[i] = i < left ? free_at(i) : -1;
   for (int t = at; t < a.max_tokens; t += step) {
@@ -179,14 +232,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_kv4_plan(sl_kv4_plan_args a, i
     }
     a.slot[t] = slot; a.pos[t] = pos;
   }
-  for (int r = at; r < n; r += step) {
-    const bool f = fit(r);
-    const int held = min(max(a.held_in[r], 0), W);
-    a.held_out[r] = held - (s_give[r + 1] - s_give[r]) + (f ? s_need[r + 1] - s_need[r] : 0);
-    a.kv_len[r] = f ? a.ctx_len[r] + a.new_len[r] : 0;
-    a.q_start[r] = s_row[r];
-  }
-  if (at == 0) { a.q_start[n] = (int)all_rows; a.free_count_out[0] = min(left, a.n_free); a.unserved[0] = (int)all_unserved; }
+  if (at == 0) { a.q_start[n] = (int)all_rows; a.free_count_out[0] = min(left, a.n_free); a.unserved[0] = (int)s_unserved; }
 }
 
 // ---- norm, rotation, quantised store ----------------------------------------------------------------------------------------
@@ -211,51 +257,86 @@ SL_DEV double sum_lanes(double v) {
 }
 template <int LANES>
 SL_DEV float sum_lanes(float v) { return tree_sum<LANES>(v); }
-SL_DEV float inv_sqrt(float x) { return 1.0f / sqrtf(x); }
-SL_DEV double inv_sqrt(double x) { return 1.0 / sqrt(x); }
+SL_DEV float inv_sqrt(float x) { return __builtin_amdgcn_rsqf(x); }
+SL_DEV double inv_sqrt(double x) {                    // the instruction's estimate and two Newton steps: within 2^-51
+  double y = __builtin_amdgcn_rsq(x);
+  y = y * fma(-0.5 * x * y, y, 1.5);
+  return y * fma(-0.5 * x * y, y, 1.5);
+}
 
-// A head row over D/4 lanes, four consecutive dims each: norm and rotation in precision F.
-template <class F, int D, bool BF>
-SL_DEV void turn_row(F* x, const uint16_t* weight, const float* cos_t, const float* sin_t, int half, int pos, double eps, int l) {
-  if (weight) {
-    const F ss = sum_lanes<D / 4>((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]));
-    const F inv = inv_sqrt(ss / (F)D + (F)eps);
-    float w[4];
-    load4<BF>(weight + 4 * l, w);
+// What a lane needs of a token beside its row: four weights, four cosines and sines, and from which lane the other half comes.
+struct Turn {
+  float w[4], c[4], s[4];
+  int from;
+  bool norm, low, turns;
+};
+template <int D, bool BF>
+SL_DEV Turn turn_of(const uint16_t* weight, const float* cos_t, const float* sin_t, int half, int pos, int l) {
+  Turn u;
+  const int lane = threadIdx.x & 63, hl = half / 4;     // a half of the rotated dims, in lanes
+  u.norm = weight != nullptr; u.low = l < hl; u.turns = l < 2 * hl;
+  u.from = u.turns ? (u.low ? lane + hl : lane - hl) : lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * (F)w[i];
+  for (int i = 0; i < 4; ++i) { u.w[i] = 1.0f; u.c[i] = 1.0f; u.s[i] = 0.0f; }
+  if (weight) load4<BF>(weight + 4 * l, u.w);
+  if (u.turns) {
+    const size_t row = (size_t)pos * half + 4 * (u.low ? l : l - hl);
+    const float4 c = *reinterpret_cast<const float4*>(cos_t + row), s = *reinterpret_cast<const float4*>(sin_t + row);
+    u.c[0] = c.x; u.c[1] = c.y; u.c[2] = c.z; u.c[3] = c.w;
+    u.s[0] = s.x; u.s[1] = s.y; u.s[2] = s.z; u.s[3] = s.w;
+  }
+  return u;
+}
+// A head row over D/4 lanes, four consecutive dims each: norm and rotation in precision F.
+template <class F, int D>
+SL_DEV void turn_row(F* x, const Turn& u, int half, double eps) {
+  if (u.norm) {
+    const F inv = inv_sqrt(sum_lanes<D / 4>((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) * (F)(1.0 / D) + (F)eps);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * (F)u.w[i];
   }
   if (half) {
-    const int hl = half / 4;                          // a half of the rotated dims, in lanes
-    const bool low = l < hl, turns = l < 2 * hl;
-    const int lane = threadIdx.x & 63, from = turns ? (low ? lane + hl : lane - hl) : lane;
     F y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __shfl(x[i], from);
-    if (turns) {
-      const size_t row = (size_t)pos * half + 4 * (low ? l : l - hl);
-      const float4 c = *reinterpret_cast<const float4*>(cos_t + row), s = *reinterpret_cast<const float4*>(sin_t + row);
-      const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+    for (int i = 0; i < 4; ++i) y[i] = __shfl(x[i], u.from);
+    if (u.turns) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = low ? x[i] * (F)cv[i] - y[i] * (F)sv[i] : x[i] * (F)cv[i] + y[i] * (F)sv[i];
+      for (int i = 0; i < 4; ++i) x[i] = u.low ? x[i] * (F)u.c[i] - y[i] * (F)u.s[i] : x[i] * (F)u.c[i] + y[i] * (F)u.s[i];
     }
   }
 }
 
 // The four codes of this lane (16 lanes = one group of 64 dims), low nibble first, and the group's scale and bias.
-// Double precision throughout: a value next to the border of two codes takes the side that exact arithmetic takes.
-SL_DEV uint32_t quantise4(const double* v, uint32_t& sb) {
-  const double lim = 65504.0;
-  double x[4];
+// Double precision decides: a value next to the border of two codes takes the side that exact arithmetic takes.  Codes are
+// formed in fp32 with one reciprocal and only those formed again by a double division that lie so near a border that fp32 could
+// be wrong: with t = (x - b) / s its error stays below (|x| + |b|) / |s| * 2^-21 + 2^-18 (three roundings of x, b and the
+// difference, each within 2^-24 of their size, the reciprocal's and the product's on |t| < 16).
+SL_DEV float row16_f(float v, bool least) {
+  auto f = [&](float a, float b) { return least ? fminf(a, b) : fmaxf(a, b); };
+  v = f(v, dpp_f<DPP_XOR1>(v)); v = f(v, dpp_f<DPP_XOR2>(v));
+  v = f(v, dpp_f<DPP_HALF_MIRROR>(v)); return f(v, dpp_f<DPP_MIRROR>(v));
+}
+// Least and largest of a group: fp32 values (what comes in as halves is exact there) or doubles.
+SL_DEV void group_range(const float* x, double& mn, double& mx) {
+  mn = (double)row16_f(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), true);
+  mx = (double)row16_f(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), false);
+}
+SL_DEV void group_range(const double* x, double& mn, double& mx) {
+  mn = row16(fmin(fmin(x[0], x[1]), fmin(x[2], x[3])), [](double a, double b) { return fmin(a, b); });
+  mx = row16(fmax(fmax(x[0], x[1]), fmax(x[2], x[3])), [](double a, double b) { return fmax(a, b); });
+}
+template <class F>
+SL_DEV uint32_t quantise4(const F* v, uint32_t& sb) {
+  const F lim = (F)65504.0;
+  F x[4];
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    bad = bad || !(fabs(v[i]) <= 1.7976931348623157e308);
-    x[i] = fmin(fmax(v[i], -lim), lim);
+    bad = bad || !(fabs(v[i]) <= (F)1e300 && fabs(v[i]) < (F)__builtin_inf());
+    x[i] = v[i] < -lim ? -lim : (v[i] > lim ? lim : v[i]);
   }
-  double mn = fmin(fmin(x[0], x[1]), fmin(x[2], x[3])), mx = fmax(fmax(x[0], x[1]), fmax(x[2], x[3]));
-  mn = row16(mn, [](double a, double b) { return fmin(a, b); });
-  mx = row16(mx, [](double a, double b) { return fmax(a, b); });
+  double mn, mx;
+  group_range(x, mn, mx);
   const unsigned long long bads = __ballot(bad);
   if ((bads >> (threadIdx.x & 48)) & 0xffffull) { sb = 0x7e007e00u; return 0; }
   const bool low = fabs(mn) > fabs(mx);
@@ -265,84 +346,119 @@ SL_DEV uint32_t quantise4(const double* v, uint32_t& sb) {
   double bias = 0.0;
   if (steps != 0.0) { scale = edge / steps; bias = edge; }
   const uint16_t hs = f2h((float)scale), hb = f2h((float)bias);
-  const double s = (double)h2f(hs), b = (double)h2f(hb);
   sb = (uint32_t)hs | ((uint32_t)hb << 16);
+  const float s = h2f(hs), b = h2f(hb), inv = 1.0f / s;
   uint32_t codes = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) codes |= (uint32_t)fmin(fmax(rint((x[i] - b) / s), 0.0), 15.0) << (4 * i);
+  for (int i = 0; i < 4; ++i) {
+    const float f = (float)x[i], t = (f - b) * inv, near = fmaf((fabsf(f) + fabsf(b)) * fabsf(inv), 4.76837158203125e-7f, 3.814697265625e-6f);
+    float c = rintf(t);
+    if (!(fabsf(fabsf(t - c) - 0.5f) > near)) c = (float)rint(((double)x[i] - (double)b) / (double)s);
+    codes |= (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * i);
+  }
   return codes;
 }
 
-// A wave per (token, 256/D heads): D/4 lanes carry a head row.  Query heads first, then key heads, then value heads.
+// A wave per token and `per` times 256/D heads: D/4 lanes carry a head row.  blockIdx.y: runs of query heads, then of key heads, then
+// of value heads; the token's weights and angles are loaded once for a run.
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void k_kv4_append(Pool pool, sl_kv4_append_args a, int q_units, int units) {
+__global__ __launch_bounds__(256) void k_kv4_append(Pool pool, sl_kv4_append_args a, int q_units, int kv_units, int per) {
   constexpr int LANES = D / 4, HEADS = 64 / LANES;
   const int lane = threadIdx.x & 63, l = lane % LANES, sub = lane / LANES;
-  const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= (long)a.n_tokens * units) return;
-  const int t = (int)(item / units);
-  int u = (int)(item - (long)t * units);
+  const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t >= a.n_tokens) return;
+  const int q_runs = (q_units + per - 1) / per, kv_runs = (kv_units + per - 1) / per;
   const int pos = a.rot_dim ? a.pos[t] : 0, half = a.rot_dim / 2;
   const bool placed = !a.rot_dim || (pos >= 0 && pos < a.max_pos);
-  if (u < q_units) {
-    const int h = u * HEADS + sub;
-    const bool there = h < a.n_heads;                 // (lanes without a head still take part in the exchanges)
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (there) load4<BF>((const uint16_t*)a.q + t * a.q_token + h * a.q_head + 4 * l, x);
-    if (placed) turn_row<float, D, BF>(x, (const uint16_t*)a.q_weight, a.cos, a.sin, half, pos, a.eps, l);
-    else { x[0] = x[1] = x[2] = x[3] = 0.0f; }
-    if (there)
-      *reinterpret_cast<uint2*>((uint16_t*)a.q_out + t * a.out_token + h * a.out_head + 4 * l) =
-          make_uint2((uint32_t)f_elem<BF>(x[0]) | ((uint32_t)f_elem<BF>(x[1]) << 16), (uint32_t)f_elem<BF>(x[2]) | ((uint32_t)f_elem<BF>(x[3]) << 16));
+  int run = blockIdx.y;
+  if (run < q_runs) {
+    const int u1 = min(q_units, (run + 1) * per);
+    const uint16_t* src = (const uint16_t*)a.q + t * a.q_token + 4 * l;
+    uint16_t* dst = (uint16_t*)a.q_out + t * a.out_token + 4 * l;
+    const Turn turn = turn_of<D, BF>((const uint16_t*)a.q_weight, a.cos, a.sin, placed ? half : 0, pos, l);
+    for (int u = run * per; u < u1; ++u) {
+      const int h = u * HEADS + sub;
+      const bool there = h < a.n_heads;               // (lanes without a head still take part in the exchanges)
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (there && placed) load4<BF>(src + h * a.q_head, x);
+      if (placed) turn_row<float, D>(x, turn, half, a.eps);
+      if (there)
+        *reinterpret_cast<uint2*>(dst + h * a.out_head) =
+            make_uint2((uint32_t)f_elem<BF>(x[0]) | ((uint32_t)f_elem<BF>(x[1]) << 16), (uint32_t)f_elem<BF>(x[2]) | ((uint32_t)f_elem<BF>(x[3]) << 16));
+    }
     return;
   }
-  u -= q_units;
+  run -= q_runs;
   const int slot = a.slot[t];
   if (!placed || slot < 0 || (slot >> pool.page_shift) >= pool.n_pages) return;
-  const int kv_units = (units - q_units) / 2;
-  const bool key = u < kv_units;
-  const int h = (key ? u : u - kv_units) * HEADS + sub;
-  const bool there = h < pool.n_kv;
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (there) load4<BF>(key ? (const uint16_t*)a.k + t * a.k_token + h * a.k_head + 4 * l : (const uint16_t*)a.v + t * a.v_token + h * a.v_head + 4 * l, x);
-  double y[4] = {x[0], x[1], x[2], x[3]};
-  if (key) turn_row<double, D, BF>(y, (const uint16_t*)a.k_weight, a.cos, a.sin, half, pos, a.eps, l);
-  uint32_t sb;
-  const uint32_t codes = quantise4(y, sb);
-  if (!there) return;
+  const bool key = run < kv_runs;
+  if (!key) run -= kv_runs;
+  const int u1 = min(kv_units, (run + 1) * per);
   const int off = slot & ((1 << pool.page_shift) - 1), part = (D / 2) << pool.page_shift, sbs = (D / 16) << pool.page_shift;
-  unsigned char* at = head_at<D>(pool, slot >> pool.page_shift, h) + (key ? 0 : part + sbs);
-  *reinterpret_cast<uint16_t*>(at + (key ? key_codes_at<D>(off, 4 * l) : value_codes_at<D>(off, 4 * l))) = (uint16_t)codes;
-  if (l % 16 == 0) reinterpret_cast<uint32_t*>(at + part)[off * (D / 64) + l / 16] = sb;
+  unsigned char* page = head_at<D>(pool, slot >> pool.page_shift, 0) + (key ? 0 : part + sbs);
+  const int codes_at = key ? key_codes_at<D>(off, 4 * l) : value_codes_at<D>(off, 4 * l);
+  const uint16_t* src = key ? (const uint16_t*)a.k + t * a.k_token + 4 * l : (const uint16_t*)a.v + t * a.v_token + 4 * l;
+  const int64_t stride = key ? a.k_head : a.v_head;
+  Turn turn;
+  if (key) turn = turn_of<D, BF>((const uint16_t*)a.k_weight, a.cos, a.sin, half, pos, l);
+  for (int u = run * per; u < u1; ++u) {
+    const int h = u * HEADS + sub;
+    const bool there = h < pool.n_kv;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (there) load4<BF>(src + h * stride, x);
+    uint32_t sb, codes;
+    if (key) {
+      double y[4] = {x[0], x[1], x[2], x[3]};
+      turn_row<double, D>(y, turn, half, a.eps);
+      codes = quantise4(y, sb);
+    } else codes = quantise4(x, sb);
+    if (!there) continue;
+    unsigned char* at = page + h * head_bytes<D>(pool);
+    *reinterpret_cast<uint16_t*>(at + codes_at) = (uint16_t)codes;
+    if (l % 16 == 0) reinterpret_cast<uint32_t*>(at + part)[off * (D / 64) + l / 16] = sb;
+  }
 }
 
 // ---- rows as values -----------------------------------------------------------------------------------------------------
+// A lane takes four dims of a key row and of a value row; a workgroup 4096 / D rows of one head, four loads of each kind in flight.
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void k_kv4_read(Pool pool, const int32_t* slots, long items, void* k_out, void* v_out) {
-  constexpr int LANES = D / 4;
-  const int l = (threadIdx.x & 63) % LANES;
-  const long item = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;     // (row, head)
-  if (item >= items) return;
-  const int row = (int)(item / pool.n_kv), h = (int)(item - (long)row * pool.n_kv);
-  const int slot = slots[row];
-  const bool in = slot >= 0 && (slot >> pool.page_shift) < pool.n_pages;
-  const int off = slot & ((1 << pool.page_shift) - 1), part = (D / 2) << pool.page_shift, sbs = (D / 16) << pool.page_shift;
-  const unsigned char* base = head_at<D>(pool, in ? slot >> pool.page_shift : 0, h);
+__global__ __launch_bounds__(256) void k_kv4_read(Pool pool, const int32_t* slots, int n, void* k_out, void* v_out) {
+  constexpr int LANES = D / 4, ROWS = 256 / LANES, TURNS = 4;
+  const int l = threadIdx.x % LANES, h = blockIdx.y;
+  const int part = (D / 2) << pool.page_shift, sbs = (D / 16) << pool.page_shift, mask = (1 << pool.page_shift) - 1;
+  const int row0 = blockIdx.x * (ROWS * TURNS) + threadIdx.x / LANES;
+  int slot[TURNS];
+  uint32_t codes[TURNS][2], sb[TURNS][2];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    void* out = kv ? v_out : k_out;
-    if (!out) continue;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (in) {
-      const unsigned char* at = base + (kv ? part + sbs : 0);
-      const uint32_t codes = *reinterpret_cast<const uint16_t*>(at + (kv ? value_codes_at<D>(off, 4 * l) : key_codes_at<D>(off, 4 * l)));
-      const uint32_t sb = reinterpret_cast<const uint32_t*>(at + part)[off * (D / 64) + l / 16];
+  for (int i = 0; i < TURNS; ++i) slot[i] = row0 + i * ROWS < n ? slots[row0 + i * ROWS] : -1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = fmaf(lo_h(sb), (float)((codes >> (4 * i)) & 15u), hi_h(sb));
+  for (int i = 0; i < TURNS; ++i) {
+    const bool in = slot[i] >= 0 && (slot[i] >> pool.page_shift) < pool.n_pages;
+    if (!in) slot[i] = -1;
+    const int off = in ? slot[i] & mask : 0;
+    const unsigned char* at = head_at<D>(pool, in ? slot[i] >> pool.page_shift : 0, h);
+    codes[i][0] = *reinterpret_cast<const uint16_t*>(at + key_codes_at<D>(off, 4 * l));
+    codes[i][1] = *reinterpret_cast<const uint16_t*>(at + part + sbs + value_codes_at<D>(off, 4 * l));
+    sb[i][0] = reinterpret_cast<const uint32_t*>(at + part)[off * (D / 64) + l / 16];
+    sb[i][1] = reinterpret_cast<const uint32_t*>(at + 2 * part + sbs)[off * (D / 64) + l / 16];
+  }
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int row = row0 + i * ROWS;
+    if (row >= n) return;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      void* out = kv ? v_out : k_out;
+      if (!out) continue;
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (slot[i] >= 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(lo_h(sb[i][kv]), (float)((codes[i][kv] >> (4 * j)) & 15u), hi_h(sb[i][kv]));
+      }
+      const size_t to = ((size_t)row * pool.n_kv + h) * D + 4 * l;
+      if (F16) *reinterpret_cast<uint2*>((uint16_t*)out + to) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
+      else *reinterpret_cast<float4*>((float*)out + to) = make_float4(x[0], x[1], x[2], x[3]);
     }
-    const size_t to = (size_t)item * D + 4 * l;
-    if (F16) *reinterpret_cast<uint2*>((uint16_t*)out + to) = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3]));
-    else *reinterpret_cast<float4*>((float*)out + to) = make_float4(x[0], x[1], x[2], x[3]);
   }
 }
 
@@ -1392,15 +1508,15 @@ int sl_kv4_plan(const sl_kv4_plan_args* a, void* stream) {
   if (!a || a->n_req < 0 || a->table_width < 0 || a->n_free < 0 || a->max_tokens < 0) return SL_ERR_ARG;
   const int shift = page_shift_of(a->page_size);
   if (shift < 0) return SL_ERR_UNSUPPORTED;
-  if (a->n_req > PLAN_MAX_REQ || (int64_t)a->n_req * a->table_width > 0x7fffffffLL || a->max_tokens > (1 << 30)) return SL_ERR_TOO_LARGE;
+  if (a->n_req > PLAN_MAX_REQ || (int64_t)a->n_req * a->table_width + a->n_free > 0x7fffffffLL || a->max_tokens > (1 << 30)) return SL_ERR_TOO_LARGE;
   const bool table = a->n_req > 0 && a->table_width > 0;
   if ((a->n_req > 0 && (!a->ctx_len || !a->new_len || !a->held_in || !a->held_out || !a->kv_len)) || (table && (!a->table_in || !a->table_out)) ||
       (a->n_free > 0 && (!a->free_in || !a->free_out)) || !a->free_count_in || !a->free_count_out || !a->q_start || !a->unserved ||
       (a->max_tokens > 0 && (!a->slot || !a->pos))) return SL_ERR_ARG;
   if ((table && a->table_in == a->table_out) || (a->n_free > 0 && a->free_in == a->free_out) || a->free_count_in == a->free_count_out ||
       (a->n_req > 0 && a->held_in == a->held_out)) return SL_ERR_ARG;
-  const int64_t most = std::max<int64_t>((int64_t)a->n_req * a->table_width, std::max(a->n_free, a->max_tokens));
-  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(512, (most + PLAN_THREADS - 1) / PLAN_THREADS));
+  const int64_t most = std::max(a->n_free, a->max_tokens);
+  const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(512, std::max<int64_t>(a->n_req, (most + PLAN_THREADS - 1) / PLAN_THREADS)));
   (void)hipGetLastError();            // an error an unrelated earlier call of this thread left behind is not this call's
   hipLaunchKernelGGL(k_kv4_plan, dim3((unsigned)blocks), dim3(PLAN_THREADS), 0, (hipStream_t)stream, *a, shift);
   return launch_status();
@@ -1418,13 +1534,15 @@ int sl_kv4_append(const sl_kv4_pool* p, const sl_kv4_append_args* a, void* strea
   const int64_t strides[] = {a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->out_token, a->out_head};
   for (int i = a->q ? 0 : 2; i < (a->q ? 8 : 6); ++i) if (strides[i] % 4) return SL_ERR_ARG;
   if (a->rot_dim && (!aligned(a->cos, 16) || !aligned(a->sin, 16))) return SL_ERR_ARG;
-  if (a->n_heads > 65536) return SL_ERR_TOO_LARGE;
+  if (a->n_heads > 32768 || a->n_tokens > 0x7ffffff0) return SL_ERR_TOO_LARGE;
   const int heads = 256 / p->head_dim, q_units = a->q ? (a->n_heads + heads - 1) / heads : 0;
-  const int units = q_units + 2 * ((p->n_kv + heads - 1) / heads);
-  const int64_t blocks = ((int64_t)a->n_tokens * units + 3) / 4;
-  if (blocks > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
+  const int kv_units = (p->n_kv + heads - 1) / heads;
+  // enough waves to fill the chip come first, then longer runs of heads (8192 waves: eight per SIMD)
+  const int64_t waves = (int64_t)a->n_tokens * (q_units + 2 * kv_units);
+  const int per = (int)std::max<int64_t>(1, std::min<int64_t>(8, waves / 8192));
+  const int runs = (q_units + per - 1) / per + 2 * ((kv_units + per - 1) / per);
   (void)hipGetLastError();
-#define KV4_CALL(D, BF) hipLaunchKernelGGL((k_kv4_append<D, BF>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, pool, *a, q_units, units)
+#define KV4_CALL(D, BF) hipLaunchKernelGGL((k_kv4_append<D, BF>), dim3((a->n_tokens + 3) / 4, runs), dim3(256), 0, (hipStream_t)stream, pool, *a, q_units, kv_units, per)
   KV4_BY_LAYOUT(p->head_dim, a->dtype == SL_BF16, KV4_CALL);
 #undef KV4_CALL
   return launch_status();
@@ -1465,10 +1583,9 @@ int sl_kv4_read(const sl_kv4_pool* p, const int32_t* slots, int n, int dtype, vo
   if (n < 0 || (dtype != SL_F32 && dtype != SL_F16) || !aligned(k_out, 16) || !aligned(v_out, 16)) return SL_ERR_ARG;
   if (n == 0 || (!k_out && !v_out)) return SL_OK;
   if (!slots) return SL_ERR_ARG;
-  const int64_t items = (int64_t)n * p->n_kv, blocks = (items * (p->head_dim / 4) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
+  const unsigned blocks = (unsigned)(((int64_t)n + 4 * (1024 / p->head_dim) - 1) / (4 * (1024 / p->head_dim)));
   (void)hipGetLastError();
-#define KV4_CALL(D, F16) hipLaunchKernelGGL((k_kv4_read<D, F16>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, pool, slots, (long)items, k_out, v_out)
+#define KV4_CALL(D, F16) hipLaunchKernelGGL((k_kv4_read<D, F16>), dim3(blocks, p->n_kv), dim3(256), 0, (hipStream_t)stream, pool, slots, n, k_out, v_out)
   KV4_BY_LAYOUT(p->head_dim, dtype == SL_F16, KV4_CALL);
 #undef KV4_CALL
   return launch_status();

@@ -40,10 +40,17 @@ class Plan(NamedTuple):
     unserved: torch.Tensor     # [1] requests that did not get their pages
 
 
+_page_bytes = {}
+
+
 def page_bytes(page_size, n_kv, head_dim):
-    n = _lib.get().dll.sl_kv4_page_bytes(page_size, n_kv, head_dim)
-    if not n:
-        raise ValueError(f"no such layout: pages of {page_size} tokens, {n_kv} heads of {head_dim} dims")
+    layout = (page_size, n_kv, head_dim)
+    n = _page_bytes.get(layout)
+    if n is None:
+        n = _lib.get().dll.sl_kv4_page_bytes(*layout)
+        if not n:
+            raise ValueError(f"no such layout: pages of {page_size} tokens, {n_kv} heads of {head_dim} dims")
+        _page_bytes[layout] = n
     return n
 
 
@@ -60,24 +67,26 @@ def rope_tables(max_pos, rot_dim, theta=1e7, device="cuda"):
 
 
 def _flat(t, shape, dtype, device, what):
-    if t.dtype is not dtype or t.device != device or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: {dtype} {list(shape)} side by side on {device} is wanted, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _rows(t, shape, dtype, device, what):
     """Address and strides of [tokens, heads, dims] with the dims side by side."""
-    if t.dtype is not dtype or t.device != device or t.shape != shape or t.stride(2) != 1:
+    token, head, dim = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.dtype is not dtype or t.shape != shape or t.device != device or dim != 1:
         raise ValueError(f"{what}: {dtype} {list(shape)} with dims side by side on {device} is wanted, got {t.dtype} {list(t.shape)} "
                          f"with strides {t.stride()} on {t.device}")
-    return t.data_ptr(), t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
+    return t.data_ptr(), token if shape[0] > 1 else 0, head if shape[1] > 1 else 0
 
 
 def _pool(pool):
-    p = pool.pages
-    if p.dtype is not torch.uint8 or not p.is_cuda or p.dim() != 2 or not p.is_contiguous() or p.shape[1] != page_bytes(*pool[1:]):
-        raise ValueError(f"pages: uint8 [n_pages, {page_bytes(*pool[1:])}] side by side on a GPU is wanted, got {p.dtype} {list(p.shape)} on {p.device}")
-    return abi.Kv4Pool(p.data_ptr(), p.shape[0], *pool[1:])
+    p, page_size, n_kv, head_dim = pool
+    n = page_bytes(page_size, n_kv, head_dim)
+    if p.dtype is not torch.uint8 or not p.is_cuda or p.dim() != 2 or p.shape[1] != n or not p.is_contiguous():
+        raise ValueError(f"pages: uint8 [n_pages, {n}] side by side on a GPU is wanted, got {p.dtype} {list(p.shape)} on {p.device}")
+    return abi.Kv4Pool(p.data_ptr(), p.shape[0], page_size, n_kv, head_dim)
 
 
 def _call(name, device, *args):
@@ -88,22 +97,31 @@ def _call(name, device, *args):
     else:
         with torch.cuda.device(device):
             status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.Library.check(status, name)
+    if status:
+        _lib.Library.check(status, name)
 
 
 def plan(ctx_len, new_len, table, held, free, free_count, page_size, max_tokens, out=None):
     """sl_kv4_plan: page tables, slots and row offsets of one step from the requests' lengths (int32 tensors).  `out`: a
-    Plan whose tensors are written, none of which may be an input."""
+    Plan whose tensors are written, none of which may be an input; without it they come as parts of one new tensor."""
     dev, i32 = ctx_len.device, torch.int32
-    if not ctx_len.is_cuda or ctx_len.dim() != 1 or table.dim() != 2 or free.dim() != 1:
+    if not ctx_len.is_cuda or ctx_len.dim() != 1 or table.dim() != 2 or free.dim() != 1 or max_tokens < 0:
         raise ValueError("lengths [n_req], table [n_req, width] and free [n_free] on a GPU are wanted")
     n, width, n_free = ctx_len.shape[0], table.shape[1], free.shape[0]
-    shapes = ((n, width), (n,), (n_free,), (1,), (n + 1,), (n,), (max_tokens,), (max_tokens,), (1,))
+    lengths = (n,)
+    ins = (_flat(ctx_len, lengths, i32, dev, "ctx_len"), _flat(new_len, lengths, i32, dev, "new_len"), _flat(table, (n, width), i32, dev, "table"),
+           _flat(held, lengths, i32, dev, "held"), _flat(free, (n_free,), i32, dev, "free"), _flat(free_count, (1,), i32, dev, "free_count"))
+    sizes = (n * width, n, n_free, 1, n + 1, n, max_tokens, max_tokens, 1)
     if out is None:
-        out = Plan(*(torch.empty(s, dtype=i32, device=dev) for s in shapes))
-    ins = [_flat(t, s, i32, dev, w) for t, s, w in ((ctx_len, (n,), "ctx_len"), (new_len, (n,), "new_len"), (table, (n, width), "table"),
-                                                    (held, (n,), "held"), (free, (n_free,), "free"), (free_count, (1,), "free_count"))]
-    outs = [_flat(t, s, i32, dev, "out." + w) for t, s, w in zip(out, shapes, Plan._fields)]
+        whole = torch.empty(sum(sizes), dtype=i32, device=dev)
+        parts = whole.split_with_sizes(sizes)
+        out = Plan(parts[0].view(n, width), *parts[1:])
+        at, outs = whole.data_ptr(), []
+        for size in sizes:
+            outs.append(at)
+            at += 4 * size
+    else:
+        outs = [_flat(t, (n, width) if i == 0 else (sizes[i],), i32, dev, "out." + Plan._fields[i]) for i, t in enumerate(out)]
     _call("sl_kv4_plan", dev, abi.Kv4PlanArgs(n, width, n_free, page_size, max_tokens, *ins, *outs))
     return out
 
@@ -115,25 +133,25 @@ def append(pool, q, k, v, slot, pos, cos, sin, q_weight, k_weight, eps=1e-6, out
     if k.dtype not in _DTYPES or k.dim() != 3:
         raise ValueError(f"keys [tokens, heads, dims] in float16 or bfloat16 are wanted, got {k.dtype} {list(k.shape)}")
     dt, n, dim = k.dtype, k.shape[0], pool.head_dim
-    a = abi.Kv4AppendArgs(n_tokens=n, dtype=_DTYPES[dt], eps=eps, slot=_flat(slot, (n,), torch.int32, dev, "slot"))
-    a.k, a.k_token, a.k_head = _rows(k, (n, pool.n_kv, dim), dt, dev, "k")
-    a.v, a.v_token, a.v_head = _rows(v, (n, pool.n_kv, dim), dt, dev, "v")
+    kv, i32 = (n, pool.n_kv, dim), torch.int32
+    k_at, v_at, q_at, out_at = _rows(k, kv, dt, dev, "k"), _rows(v, kv, dt, dev, "v"), (None, 0, 0), (None, 0, 0)
+    heads = max_pos = rot = 0
+    cos_at = sin_at = pos_at = qw_at = kw_at = None
     if q is not None:
-        shape = (n, q.shape[1], dim)
+        heads = q.shape[1] if q.dim() == 3 else 0
+        shape = (n, heads, dim)
         if out is None:
             out = torch.empty(shape, dtype=dt, device=dev)
-        a.n_heads = q.shape[1]
-        a.q, a.q_token, a.q_head = _rows(q, shape, dt, dev, "q")
-        a.q_out, a.out_token, a.out_head = _rows(out, shape, dt, dev, "out")
+        q_at, out_at = _rows(q, shape, dt, dev, "q"), _rows(out, shape, dt, dev, "out")
         if q_weight is not None:
-            a.q_weight = _flat(q_weight, (dim,), dt, dev, "q_weight")
+            qw_at = _flat(q_weight, (dim,), dt, dev, "q_weight")
     if k_weight is not None:
-        a.k_weight = _flat(k_weight, (dim,), dt, dev, "k_weight")
+        kw_at = _flat(k_weight, (dim,), dt, dev, "k_weight")
     if cos is not None:
-        a.max_pos, a.rot_dim = cos.shape[0], 2 * cos.shape[1]
-        a.cos, a.sin = _flat(cos, cos.shape, torch.float32, dev, "cos"), _flat(sin, cos.shape, torch.float32, dev, "sin")
-        a.pos = _flat(pos, (n,), torch.int32, dev, "pos")
-    _call("sl_kv4_append", dev, p, a)
+        max_pos, rot = cos.shape[0], 2 * cos.shape[1]
+        cos_at, sin_at, pos_at = _flat(cos, cos.shape, torch.float32, dev, "cos"), _flat(sin, cos.shape, torch.float32, dev, "sin"), _flat(pos, (n,), i32, dev, "pos")
+    _call("sl_kv4_append", dev, p, abi.Kv4AppendArgs(n, heads, rot, max_pos, _DTYPES[dt], 0, eps, q_at[0], k_at[0], v_at[0], qw_at, kw_at, cos_at, sin_at,
+                                                     _flat(slot, (n,), i32, dev, "slot"), pos_at, out_at[0], *q_at[1:], *k_at[1:], *v_at[1:], *out_at[1:]))
     return out
 
 
@@ -147,14 +165,13 @@ def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, g
     shape, dt = (n, heads, dim), q.dtype
     if out is None:
         out = torch.empty(shape, dtype=dt, device=dev)
-    a = abi.Kv4AttnArgs(n_req, n, heads, _DTYPES[dt], table.shape[1], max_rows, max_keys, dim ** -0.5 if scale is None else scale)
-    a.q, a.q_token, a.q_head = _rows(q, shape, dt, dev, "q")
-    a.out, a.out_token, a.out_head = _rows(out, shape, dt, dev, "out")
+    i32 = torch.int32
+    q_at, out_at, gate_at = _rows(q, shape, dt, dev, "q"), _rows(out, shape, dt, dev, "out"), (None, 0, 0)
     if gate is not None:
-        a.gate, a.gate_token, a.gate_head = _rows(gate, shape, dt, dev, "gate")
-    a.table = _flat(table, table.shape, torch.int32, dev, "table")
-    a.q_start = _flat(q_start, (n_req + 1,), torch.int32, dev, "q_start")
-    a.kv_len = _flat(kv_len, (n_req,), torch.int32, dev, "kv_len")
+        gate_at = _rows(gate, shape, dt, dev, "gate")
+    a = abi.Kv4AttnArgs(n_req, n, heads, _DTYPES[dt], table.shape[1], max_rows, max_keys, dim ** -0.5 if scale is None else scale, q_at[0], gate_at[0], out_at[0],
+                        *q_at[1:], *gate_at[1:], *out_at[1:], _flat(table, table.shape, i32, dev, "table"), _flat(q_start, (n_req + 1,), i32, dev, "q_start"),
+                        _flat(kv_len, (n_req,), i32, dev, "kv_len"))
     need = _lib.get().dll.sl_kv4_attention_workspace(p, a)
     if need > 0:
         if workspace is None:
@@ -166,9 +183,10 @@ def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, g
     return out
 
 
-def attention_workspace(pool, n_tokens, n_heads, n_req, max_rows, max_keys):
-    """Bytes of workspace that attention() takes for such a call."""
-    return _lib.get().dll.sl_kv4_attention_workspace(_pool(pool), abi.Kv4AttnArgs(n_req=n_req, n_tokens=n_tokens, n_heads=n_heads, max_rows=max_rows, max_keys=max_keys))
+def attention_workspace(pool, n_tokens, n_heads, n_req, table_width, max_rows, max_keys):
+    """Bytes of workspace that attention() takes for such a call (0: a call that has nothing to do, or is refused)."""
+    a = abi.Kv4AttnArgs(n_req=n_req, n_tokens=n_tokens, n_heads=n_heads, table_width=table_width, max_rows=max_rows, max_keys=max_keys)
+    return _lib.get().dll.sl_kv4_attention_workspace(_pool(pool), a)
 
 
 def read(pool, slots, dtype=torch.float32):
