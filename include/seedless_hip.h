@@ -379,6 +379,23 @@ int sl_set_persistent(sl_engine* e, int enable);
  * and attention stay on the exact kernels.  Decode steps and steps of fewer than 16 rows are unaffected. */
 int sl_set_hybrid(sl_engine* e, int enable);
 
+/* No counterpart in the reference.  The attention layers of this engine, and of the lanes created from it afterwards, keep their
+ * keys and values in 4 bits, in n_pages pages of page_size tokens (16, 32, 64, 128, 256) per layer that all
+ * sequences share (0: enough for max_seq_len tokens): 576 instead of 2048 bytes per token and layer.  The fp16 caches of the
+ * engine are freed.  To be called once, on a new engine (not a lane) before its first token and its first lane; at most 63 lanes, with
+ * max_seq_len and max_m up to the engine's max_seq_len (or its max_m, if that is larger).
+ * A call for which the pages do not suffice returns SL_ERR_TOO_LARGE and changes nothing; pages return when a sequence
+ * is rolled back, reset or destroyed, with the next call of any of them.
+ * Steps then run kernel by kernel (sl_set_persistent has no effect), with the operators below in the attention layers
+ * and the same arithmetic everywhere else.  Results are no longer bit-identical to the oracle; they are deterministic, and a
+ * sequence of up to 128 tokens gets the same bits whichever lanes it is stepped with (longer axes are cut by the lengths of a
+ * whole step).  sl_lane_step_argmax steps all lanes as one group.  sl_full_restore
+ * refuses a snapshot behind what the sequence's pages still hold; sl_read_layer_cache returns the values that the codes stand for, rounded to
+ * fp16; sl_load_layer_cache quantises and takes keys and values together; the persisted-state calls answer
+ * SL_ERR_UNSUPPORTED (sl_persist_size 0).  SL_ERR_UNSUPPORTED: an engine without attention layers, another page size.
+ * SL_ERR_TOO_LARGE: no memory for the pages (the engine stays as it was). */
+int sl_set_kv4(sl_engine* e, int page_size, int n_pages);
+
 /* Diagnostic in the manner of forwardRowsProfiled (SFV:4352), at the grain of one stage of the single-launch step:
  * while enabled, batch-1 steps run a variant of that kernel in which every workgroup records 100 MHz clock stamps of
  * the last step of a launch (kept on chip until the launch ends, so they do not disturb what they time).  The call

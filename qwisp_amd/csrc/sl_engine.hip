@@ -11,7 +11,9 @@
 #include <cstdlib>
 #include <atomic>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <system_error>
 #include <thread>
@@ -44,6 +46,7 @@ struct LayerDev {
   // attention
   DevQ4 qkv, o_proj;
   uint16_t *q_norm = nullptr, *k_norm = nullptr, *kcache = nullptr, *vcache = nullptr;
+  void* kv4 = nullptr;             // pages of the 4-bit cache (sl_set_kv4), shared by the engine and its lanes; kcache and vcache are null then
   // MoE
   uint16_t *router_w = nullptr, *sgate_w = nullptr;
   uint16_t* router_pad = nullptr;   // fp16 gates as one matrix [288, 2048] for the matrix-core router of hybrid chunks: rows 0..E-1, row 256 = shared gate
@@ -109,6 +112,28 @@ struct sl_full_snap {
   std::vector<float*> state;
 };
 
+// ---- 4-bit caches of an engine and its lanes (sl_set_kv4) -------------------------------------------------------
+// One set of pages per attention layer, one page table for all layers.  The sequences (the engine itself, its lanes) are the
+// requests of sl_kv4_plan: before the layers of a call run, it is told every sequence's length and how many rows
+// come to it, so pages that a rollback, a reset or a destroyed lane no longer needs go back by themselves.  The host knows all
+// lengths, so it knows beforehand whether the pages suffice.
+constexpr int KV4_SEQS = 64;              // (sl_kv4_plan takes up to 64 requests in one wave)
+struct Kv4Lens { int32_t ctx[KV4_SEQS], nw[KV4_SEQS]; };
+__global__ __launch_bounds__(64) void k_kv4_lens(Kv4Lens lens, int32_t* ctx, int32_t* nw) {
+  ctx[threadIdx.x] = lens.ctx[threadIdx.x];
+  nw[threadIdx.x] = lens.nw[threadIdx.x];
+}
+struct Kv4Store {
+  int page_size = 0, n_pages = 0, width = 0, max_rows = 0, max_seq = 0;
+  sl_engine* seq[KV4_SEQS] = {};
+  int32_t *table[2] = {}, *held[2] = {}, *free_list[2] = {}, *free_count[2] = {};      // now and after the next plan
+  int32_t *ctx = nullptr, *nw = nullptr, *q_start = nullptr, *kv_len = nullptr, *slot = nullptr, *pos = nullptr, *unserved = nullptr;
+  int now = 0;
+  int rows = 0, most_rows = 0, most_keys = 0;      // of the call at work
+  void* workspace = nullptr;
+  int64_t workspace_bytes = 0;
+};
+
 struct sl_engine {
   uint64_t uid = g_engine_uid.fetch_add(1);   // never reused: identifies an engine in another engine's lane table
   // lanes keep their base alive: a base destroyed while lanes exist is only marked, and goes with its last lane
@@ -171,6 +196,9 @@ struct sl_engine {
   int32_t* hy_counts = nullptr;
   unsigned char* gc_scratch = nullptr;   // chunked gated-delta scan of hybrid chunks: [max_m / 64][32][GC_UNIT_BYTES]
   bool inject_failure = false;
+  Kv4Store* kv4 = nullptr;         // the base's, which owns it (kv4_seq 0)
+  int kv4_seq = -1;
+  int kv4_rows = 0;                // leading rows of this sequence that its pages still hold
   // lane batch driven from this engine's scratch: device table [n_layers][max_m] of the lanes last stepped together
   LaneRef* lane_tab = nullptr;
   std::vector<uint64_t> lane_set;              // uids of the lanes the table was built for
@@ -280,15 +308,33 @@ int guard(sl_engine* e) {
   if (!e->fault.empty()) return SL_ERR_POISONED;
   return SL_OK;
 }
+// Whether the pages of the 4-bit caches suffice with sequence i at ctx[i] tokens and nw[i] more.
+bool kv4_fits(const Kv4Store& k, const Kv4Lens& lens) {
+  int64_t pages = 0;
+  for (int i = 0; i < KV4_SEQS; ++i) pages += ((int64_t)lens.ctx[i] + lens.nw[i] + k.page_size - 1) / k.page_size;
+  return pages <= k.n_pages;
+}
+Kv4Lens kv4_lens(const Kv4Store& k) {
+  Kv4Lens lens;
+  for (int i = 0; i < KV4_SEQS; ++i) { lens.ctx[i] = k.seq[i] ? k.seq[i]->pos : 0; lens.nw[i] = 0; }
+  return lens;
+}
+bool kv4_room(const sl_engine* e, int m) {
+  if (!e->kv4) return true;
+  Kv4Lens lens = kv4_lens(*e->kv4);
+  lens.nw[e->kv4_seq] = m;
+  return kv4_fits(*e->kv4, lens);
+}
 int check_rows(sl_engine* e, int m) {
   if (m < 1 || m > e->max_m) return SL_ERR_ARG;
   if (e->has_attn && e->pos + m > e->max_seq) return SL_ERR_ARG;
-  return SL_OK;
+  return kv4_room(e, m) ? SL_OK : SL_ERR_TOO_LARGE;
 }
 // Waits for the stream; the injected failure stands in for a failed submission.
 int finish(sl_engine* e, const char* what) {
   hipError_t r = hipStreamSynchronize(e->stream);
   if (r == hipSuccess) r = hipGetLastError();
+  if (!e->fault.empty()) return SL_ERR_DEVICE;          // a launch on the way here was refused
   if (e->inject_failure) {
     e->inject_failure = false;
     e->fault = std::string(what) + ": injected device failure";
@@ -471,18 +517,58 @@ void launch_gdn_mixer(sl_engine* e, LayerDev& L, int li, int M, const HiddenArgs
                        L.out_proj.w, L.out_proj.sb, H, e->mix);
   }
 }
-void launch_attn_mixer(sl_engine* e, LayerDev& L, int M, const HiddenArgs& ha, const LaneRef* lanes, int lane_tiles) {
-  const bool mm = use_matrix_cores(e, M, lanes);
-  if (mm) {
-    HiddenArgs hn = ha; hn.xn_out = e->xn;
-    hipLaunchKernelGGL(k_final_rows, dim3(M), dim3(64), 0, e->stream, hn);
-    launch_qmm4_mfma(QmmArgs{e->xn, H, L.qkv.w, L.qkv.sb, M, SL_ATT_QKV_N, H, e->proj, PROJ_STRIDE}, e->stream);
-  } else if (M >= 2) {
-    launch_hidden_tile(e, ha, L.qkv.w, L.qkv.sb, SL_ATT_QKV_N, M);
-  } else {
-    hipLaunchKernelGGL(k_qmv_hidden<4>, dim3(SL_ATT_QKV_N / 16, M), dim3(256), 0, e->stream, ha, L.qkv.w, L.qkv.sb,
-                       SL_ATT_QKV_N, e->proj, PROJ_STRIDE);
+void kv4_failed(sl_engine* e, const char* what, int status) {
+  if (e->fault.empty()) e->fault = std::string(what) + " failed with status " + std::to_string(status);
+}
+// Pages and row offsets of a call: lens.nw[i] rows come to sequence i (rows in the sequences' order), on e's stream.
+void kv4_begin(sl_engine* e, const Kv4Lens& lens) {
+  Kv4Store& k = *e->kv4;
+  k.rows = k.most_rows = k.most_keys = 0;
+  for (int i = 0; i < KV4_SEQS; ++i) {
+    k.rows += lens.nw[i];
+    k.most_rows = std::max(k.most_rows, lens.nw[i]);
+    if (lens.nw[i]) k.most_keys = std::max(k.most_keys, lens.ctx[i] + lens.nw[i]);
+    if (k.seq[i]) k.seq[i]->kv4_rows = lens.ctx[i] + lens.nw[i];
   }
+  hipLaunchKernelGGL(k_kv4_lens, dim3(1), dim3(KV4_SEQS), 0, e->stream, lens, k.ctx, k.nw);
+  const int a = k.now, b = 1 - a;
+  const sl_kv4_plan_args p{KV4_SEQS, k.width, k.n_pages, k.page_size, k.rows, k.ctx, k.nw, k.table[a], k.held[a], k.free_list[a], k.free_count[a],
+                           k.table[b], k.held[b], k.free_list[b], k.free_count[b], k.q_start, k.kv_len, k.slot, k.pos, k.unserved};
+  const int r = sl_kv4_plan(&p, e->stream);
+  if (r) { kv4_failed(e, "sl_kv4_plan", r); return; }
+  k.now = b;
+}
+void kv4_begin(sl_engine* e, int M) {
+  Kv4Lens lens = kv4_lens(*e->kv4);
+  lens.nw[e->kv4_seq] = M;
+  kv4_begin(e, lens);
+}
+sl_kv4_pool kv4_pool(const Kv4Store& k, const LayerDev& L) { return sl_kv4_pool{L.kv4, k.n_pages, k.page_size, SL_ATT_KV, SL_ATT_D}; }
+// Attention of one layer over the 4-bit caches: projection rows in e->proj, gated output rows to e->ycore.
+void launch_attn_kv4(sl_engine* e, const LayerDev& L, int M) {
+  if (!e->fault.empty()) return;
+  Kv4Store& k = *e->kv4;
+  const sl_kv4_pool pool = kv4_pool(k, L);
+  const uint16_t *q = e->proj, *kk = e->proj + 8192, *vv = kk + SL_ATT_KV * SL_ATT_D;
+  const sl_kv4_append_args a{M, SL_ATT_HEADS, SL_ROPE_DIM, e->max_seq, SL_F16, 0, EPS, q, kk, vv, L.q_norm, L.k_norm, e->rope_cos, e->rope_sin, k.slot, k.pos, e->qrot,
+                             PROJ_STRIDE, 2 * SL_ATT_D, PROJ_STRIDE, SL_ATT_D, PROJ_STRIDE, SL_ATT_D, SL_ATT_HEADS * SL_ATT_D, SL_ATT_D};
+  int r = sl_kv4_append(&pool, &a, e->stream);
+  if (r) { kv4_failed(e, "sl_kv4_append", r); return; }
+  sl_kv4_attn_args t{KV4_SEQS, M, SL_ATT_HEADS, SL_F16, k.width, k.most_rows, k.most_keys, 0.0625f, e->qrot, e->proj + SL_ATT_D, e->ycore,
+                     SL_ATT_HEADS * SL_ATT_D, SL_ATT_D, PROJ_STRIDE, 2 * SL_ATT_D, SL_ATT_HEADS * SL_ATT_D, SL_ATT_D, k.table[k.now], k.q_start, k.kv_len, nullptr, 0};
+  const int64_t need = sl_kv4_attention_workspace(&pool, &t);
+  if (need > k.workspace_bytes) {              // grows with the rows of a call; calls are serialised, hipFree waits for what still runs
+    if (k.workspace) (void)hipFree(k.workspace);
+    k.workspace = nullptr; k.workspace_bytes = 0;
+    if (!ok(e, hipMalloc(&k.workspace, (size_t)need), "hipMalloc")) return;
+    k.workspace_bytes = need;
+  }
+  t.workspace = k.workspace; t.workspace_bytes = k.workspace_bytes;
+  r = sl_kv4_attention(&pool, &t, e->stream);
+  if (r) kv4_failed(e, "sl_kv4_attention", r);
+}
+// Attention of one layer over the fp16 caches: projection rows in e->proj, gated output rows to e->ycore.
+void launch_attn_tiles(sl_engine* e, LayerDev& L, int M, const LaneRef* lanes, int lane_tiles, bool mm) {
   AttnPrepArgs p{};
   p.proj = e->proj; p.q_norm = L.q_norm; p.k_norm = L.k_norm; p.rope_cos = e->rope_cos; p.rope_sin = e->rope_sin;
   p.st = e->st; p.qrot = e->qrot; p.kcache = L.kcache; p.vcache = L.vcache; p.maxSeq = e->max_seq; p.lanes = lanes;
@@ -514,9 +600,24 @@ void launch_attn_mixer(sl_engine* e, LayerDev& L, int M, const HiddenArgs& ha, c
   else if (M <= MERGE_BLOCKS_ROWS) hipLaunchKernelGGL(k_sdpa_merge_blocks, dim3(SL_ATT_HEADS, M, 4), dim3(64 * MERGE_BLOCKS_WAVES), 0, e->stream, g);
   else if (M <= MERGE_LONG_ROWS) hipLaunchKernelGGL(k_sdpa_merge_long, dim3(SL_ATT_HEADS, M), dim3(1024), MERGE_DYN_LDS, e->stream, g);
   else hipLaunchKernelGGL(k_sdpa_merge, dim3(SL_ATT_HEADS, M), dim3(64), 0, e->stream, g);
+}
+void launch_attn_mixer(sl_engine* e, LayerDev& L, int M, const HiddenArgs& ha, const LaneRef* lanes, int lane_tiles) {
+  const bool mm = use_matrix_cores(e, M, lanes);
+  if (mm) {
+    HiddenArgs hn = ha; hn.xn_out = e->xn;
+    hipLaunchKernelGGL(k_final_rows, dim3(M), dim3(64), 0, e->stream, hn);
+    launch_qmm4_mfma(QmmArgs{e->xn, H, L.qkv.w, L.qkv.sb, M, SL_ATT_QKV_N, H, e->proj, PROJ_STRIDE}, e->stream);
+  } else if (M >= 2) {
+    launch_hidden_tile(e, ha, L.qkv.w, L.qkv.sb, SL_ATT_QKV_N, M);
+  } else {
+    hipLaunchKernelGGL(k_qmv_hidden<4>, dim3(SL_ATT_QKV_N / 16, M), dim3(256), 0, e->stream, ha, L.qkv.w, L.qkv.sb,
+                       SL_ATT_QKV_N, e->proj, PROJ_STRIDE);
+  }
+  if (L.kv4) launch_attn_kv4(e, L, M);
+  else launch_attn_tiles(e, L, M, lanes, lane_tiles, mm);
   if (mm && !(lanes && M < MM_OUT_ROWS)) launch_qmm4_mfma(QmmArgs{e->ycore, 4096, L.o_proj.w, L.o_proj.sb, M, H, 4096, e->mix, H}, e->stream);
   else if (M >= 2) hipLaunchKernelGGL((k_qmv_tile<2, 2, 4, false>), dim3(H / 8, (M + 3) / 4), dim3(256), 0, e->stream, HiddenArgs{}, e->ycore, 4096,
-                                      L.o_proj.w, L.o_proj.sb, H, e->mix, H, M, (float*)nullptr, (int32_t*)nullptr, mm ? (float*)nullptr : e->ysum);
+                                      L.o_proj.w, L.o_proj.sb, H, e->mix, H, M, (float*)nullptr, (int32_t*)nullptr, mm || L.kv4 ? (float*)nullptr : e->ysum);
   else hipLaunchKernelGGL((k_qmv_plain<2, 2>), dim3(H / 8, M), dim3(256), 0, e->stream, e->ycore, 4096, L.o_proj.w, L.o_proj.sb,
                           H, e->mix, H);
 }
@@ -538,6 +639,7 @@ void launch_layer(sl_engine* e, int li, int M, const LaneRef* lane_tab = nullptr
   else launch_moe(e, L, M, hb);
 }
 void launch_layers(sl_engine* e, int M, const LaneRef* lane_tab = nullptr, int lane_tiles = 0) {
+  if (e->kv4 && !lane_tab) kv4_begin(e, M);          // (a batch of lanes has had its own)
   for (int li = 0; li < e->n_layers; ++li) launch_layer(e, li, M, lane_tab, lane_tiles);
 }
 void advance(sl_engine* e, int M) {
@@ -647,9 +749,11 @@ int alloc_layer_state(sl_engine* e, LayerDev& L) {
     if (!L.hist[1] || !L.state[1]) return SL_ERR_DEVICE;
   } else {
     e->has_attn = true;
-    L.kcache = dalloc<uint16_t>(e, (size_t)SL_ATT_KV * e->max_seq * SL_ATT_D, true);
-    L.vcache = dalloc<uint16_t>(e, (size_t)SL_ATT_KV * e->max_seq * SL_ATT_D, true);
-    if (!L.kcache || !L.vcache) return SL_ERR_DEVICE;
+    if (!L.kv4) {
+      L.kcache = dalloc<uint16_t>(e, (size_t)SL_ATT_KV * e->max_seq * SL_ATT_D, true);
+      L.vcache = dalloc<uint16_t>(e, (size_t)SL_ATT_KV * e->max_seq * SL_ATT_D, true);
+      if (!L.kcache || !L.vcache) return SL_ERR_DEVICE;
+    }
   }
   L.route_inds = dalloc<int32_t>(e, (size_t)e->max_m * 8, true);
   L.route_scores = dalloc<uint16_t>(e, (size_t)e->max_m * 8, true);
@@ -913,6 +1017,13 @@ int sl_lane_create(const sl_engine* base, int max_m, int max_seq_len, sl_engine*
     if (root->destroy_pending || !root->fault.empty()) return SL_ERR_POISONED;
   }
   std::lock_guard<std::recursive_mutex> gpu_lock_(g_gpu_mutex);
+  Kv4Store* kv4 = base->kv4;
+  int seq = -1;
+  if (kv4) {                                      // a sequence of the base's 4-bit caches
+    if (max_seq_len > kv4->max_seq || max_m > kv4->max_rows) return SL_ERR_ARG;
+    for (int i = 0; i < KV4_SEQS && seq < 0; ++i) if (!kv4->seq[i]) seq = i;
+    if (seq < 0) return SL_ERR_TOO_LARGE;
+  }
   sl_engine* e = new sl_engine();
   *out = e;
   e->n_layers = base->n_layers; e->n_experts = base->n_experts; e->vocab = base->vocab;
@@ -933,7 +1044,10 @@ int sl_lane_create(const sl_engine* base, int max_m, int max_seq_len, sl_engine*
   sl_engine* root = const_cast<sl_engine*>(base->base_of ? base->base_of : base);   // a lane of a lane shares the root's weights
   e->base_of = root;
   root->lane_refs += 1;
-  return alloc_runtime(e);
+  const int r = alloc_runtime(e);
+  if (r) return r;
+  if (kv4) { e->kv4 = kv4; e->kv4_seq = seq; e->dec_grid = 0; kv4->seq[seq] = e; }
+  return SL_OK;
 }
 
 namespace {
@@ -945,7 +1059,7 @@ bool lanes_batchable(sl_engine** lanes, int b) {
   for (int i = 0; i < b; ++i) {
     const sl_engine* l = lanes[i];
     if (l->n_layers != d->n_layers || l->max_seq != d->max_seq || l->lm_head.w != d->lm_head.w ||
-        l->layers[0].router_w != d->layers[0].router_w || l->layers[0].gate8_w != d->layers[0].gate8_w) return false;
+        l->layers[0].router_w != d->layers[0].router_w || l->layers[0].gate8_w != d->layers[0].gate8_w || l->kv4 != d->kv4) return false;
   }
   return true;
 }
@@ -956,7 +1070,7 @@ bool lanes_batchable(sl_engine** lanes, int b) {
 // 8 rows are too small to share the device, and there are 2000 of them.)
 constexpr int LANE_GROUPS_MAX = 2, LANE_GROUP_ROWS = 16;
 int lane_groups(sl_engine** lanes, int b) {
-  if (b < 2 * LANE_GROUP_ROWS) return 1;
+  if (b < 2 * LANE_GROUP_ROWS || lanes[0]->kv4) return 1;      // (4-bit caches: one page plan and one attention for all lanes of a step)
   // the second group's first lane (lanes[1]) must be able to drive its half
   const sl_engine* d1 = lanes[1];
   if (b / 2 > d1->max_m || !d1->has_head || d1->max_seq != lanes[0]->max_seq) return 1;
@@ -1000,6 +1114,13 @@ int sl_lane_step_argmax(sl_engine** lanes, int b, const int32_t* tokens, int32_t
     for (int j = 0; j < i; ++j) if (lanes[j] == lanes[i]) return SL_ERR_ARG;
   }
   for (int i = 0; i < b; ++i) lanes[i]->normed_rows = 0;
+  Kv4Lens lens{};                                // of lanes[0]'s 4-bit caches
+  for (int i = b - 1; i >= 0; --i) {             // pages for all of them, or for none
+    if (!lanes[i]->kv4) continue;
+    lens = kv4_lens(*lanes[i]->kv4);
+    for (int j = 0; j < b; ++j) if (lanes[j]->kv4 == lanes[i]->kv4) lens.nw[lanes[j]->kv4_seq] = 1;
+    if (!kv4_fits(*lanes[i]->kv4, lens)) return SL_ERR_TOO_LARGE;
+  }
   if (!lanes_batchable(lanes, b)) {
     for (int i = 0; i < b; ++i) { const int r = sl_step_argmax(lanes[i], tokens + i, 1, out + i); if (r) return r; }
     return SL_OK;
@@ -1018,12 +1139,22 @@ int sl_lane_step_argmax(sl_engine** lanes, int b, const int32_t* tokens, int32_t
   // (Lane i goes to group i % 2: whatever order the caller keeps its lanes in, neighbours are dealt to both groups,
   // so a batch sorted by context length does not end up as a short group and a long one.)
   const int ng = lane_groups(lanes, b);
+  // (4-bit caches: rows come in the order of the sequences there)
+  std::vector<int> order(b), place(b);
+  for (int i = 0; i < b; ++i) order[i] = i;
+  if (d->kv4) std::sort(order.begin(), order.end(), [&](int x, int y) { return lanes[x]->kv4_seq < lanes[y]->kv4_seq; });
+  sl_engine* drv[LANE_GROUPS_MAX];               // lends scratch rows and stream to its group
   std::vector<sl_engine*> grp[LANE_GROUPS_MAX];
   std::vector<int32_t> gtok[LANE_GROUPS_MAX];
-  for (int i = 0; i < b; ++i) { grp[i % ng].push_back(lanes[i]); gtok[i % ng].push_back(tokens[i]); }
+  for (int g = 0; g < ng; ++g) drv[g] = lanes[g];
+  for (int j = 0; j < b; ++j) {
+    const int i = order[j];
+    place[i] = (int)grp[j % ng].size();
+    grp[j % ng].push_back(lanes[i]); gtok[j % ng].push_back(tokens[i]);
+  }
   int tiles[LANE_GROUPS_MAX];
   for (int g = 0; g < ng; ++g) {
-    sl_engine* dg = grp[g][0];
+    sl_engine* dg = drv[g];
     if (g > 0 && d->hybrid != dg->hybrid) { const int r = sl_set_hybrid(dg, d->hybrid ? 1 : 0); if (r) return r; }
     int max_pos = 0;
     for (const sl_engine* l : grp[g]) if (l->pos > max_pos) max_pos = l->pos;
@@ -1034,7 +1165,7 @@ int sl_lane_step_argmax(sl_engine** lanes, int b, const int32_t* tokens, int32_t
   for (int i = 1; i < b; ++i) SL_TRY(lanes[i], hipStreamSynchronize(lanes[i]->stream));
   SL_TRY(d, hipEventRecord(d->ev0, d->stream));
   for (int g = 0; g < ng; ++g) {
-    sl_engine* dg = grp[g][0];
+    sl_engine* dg = drv[g];
     const int n = (int)grp[g].size();
     const int r = to_device(dg, dg->tok_in, gtok[g].data(), (size_t)n * 4); if (r) return r;
     if (g > 0) SL_TRY(dg, hipStreamWaitEvent(dg->stream, d->ev0, 0));      // (the step's time is measured on the first group's stream)
@@ -1044,9 +1175,10 @@ int sl_lane_step_argmax(sl_engine** lanes, int b, const int32_t* tokens, int32_t
   // are on the device early in the step)
   hipError_t queued[LANE_GROUPS_MAX];
   auto queue_group = [&](int g) {
-    sl_engine* dg = grp[g][0];
+    sl_engine* dg = drv[g];
     const int n = (int)grp[g].size();
     if (g > 0) { (void)hipSetDevice(dg->device); (void)hipGetLastError(); }
+    if (dg->kv4) kv4_begin(dg, lens);
     launch_layers(dg, n, dg->lane_tab, tiles[g]);
     HiddenArgs ha{dg->hA, dg->moe_out, dg->final_norm, dg->hB, dg->normed};
     launch_head(dg, n, ha, 0, false);
@@ -1067,32 +1199,32 @@ int sl_lane_step_argmax(sl_engine** lanes, int b, const int32_t* tokens, int32_t
   }
   for (int g = 1; g < ng; ++g)
     if (!ok(d, queued[g], "stepArgmaxBatch (second group)")) {
-      for (int h = 0; h < ng; ++h) (void)hipStreamSynchronize(grp[h][0]->stream);
+      for (int h = 0; h < ng; ++h) (void)hipStreamSynchronize(drv[h]->stream);
       for (int i = 1; i < b; ++i) if (lanes[i]->fault.empty()) lanes[i]->fault = d->fault;
       return SL_ERR_DEVICE;
     }
   for (int g = 1; g < ng; ++g) {                         // the first group's stream ends the step: it waits for the others
-    sl_engine* dg = grp[g][0];
+    sl_engine* dg = drv[g];
     SL_TRY(dg, hipEventRecord(dg->ev1, dg->stream));
     SL_TRY(d, hipStreamWaitEvent(d->stream, dg->ev1, 0));
   }
   SL_TRY(d, hipEventRecord(d->ev1, d->stream));
   int r = SL_OK;
   for (int g = 0; g < ng && !r; ++g) {
-    sl_engine* dg = grp[g][0];
+    sl_engine* dg = drv[g];
     r = read_back(dg, gtok[g].data(), dg->tok_out, grp[g].size() * 4, "stepArgmaxBatch");
     if (r && d->fault.empty()) d->fault = dg->fault;
   }
   if (r) {   // the lanes' caches were written by the failed step: all of them are unusable
-    for (int g = 1; g < ng; ++g) (void)hipStreamSynchronize(grp[g][0]->stream);
+    for (int g = 1; g < ng; ++g) (void)hipStreamSynchronize(drv[g]->stream);
     for (int i = 1; i < b; ++i) if (lanes[i]->fault.empty()) lanes[i]->fault = d->fault;
     return r;
   }
   time_end(d);
   for (int i = 0; i < b; ++i) {
     sl_engine* l = lanes[i];
-    sl_engine* dg = grp[i % ng][0];
-    const int row = i / ng;
+    sl_engine* dg = drv[i % ng];
+    const int row = place[i];
     out[i] = gtok[i % ng][row];
     l->pos += 1;
     for (int j = 0; j < l->n_layers; ++j) if (l->layers[j].is_linear) l->parity[j] ^= 1;
@@ -1121,6 +1253,11 @@ void sl_destroy(sl_engine* e) {
   }
   sl_engine* root = e->base_of;
   if (e->stream) (void)hipStreamSynchronize(e->stream);
+  if (e->kv4) e->kv4->seq[e->kv4_seq] = nullptr;      // (its pages go back with the next plan)
+  if (e->kv4 && !root) {
+    if (e->kv4->workspace) (void)hipFree(e->kv4->workspace);
+    delete e->kv4;
+  }
   for (void* p : e->allocs) (void)hipFree(p);
   if (e->pinned) (void)hipHostFree(e->pinned);
   for (hipEvent_t ev : e->head_ev) (void)hipEventDestroy(ev);
@@ -1299,6 +1436,7 @@ int sl_chained_step_argmax(sl_engine* e, int32_t first, int k, int32_t* out) {
   e->logits_view = e->normed_view = nullptr;
   if (!out || !e->has_head || k < 1 || k > MAX_CHAIN || first < 0 || first >= e->vocab) return SL_ERR_ARG;
   if (e->has_attn && e->pos + k > e->max_seq) return SL_ERR_ARG;
+  if (!kv4_room(e, k)) return SL_ERR_TOO_LARGE;
   r = to_device(e, e->tok_in, &first, 4); if (r) return r;
   const bool persistent = (e->dec_grid > 0 && e->use_persistent);
   SL_TRY(e, hipEventRecord(e->ev0, e->stream));
@@ -1462,6 +1600,7 @@ int sl_full_snapshot(sl_engine* e, sl_full_snap** out) {
 int sl_full_restore(sl_engine* e, const sl_full_snap* s) {
   SL_ENTER(e);
   if (!s || (int)s->hist.size() != e->n_layers) return SL_ERR_ARG;
+  if (e->kv4 && s->pos > e->kv4_rows) return SL_ERR_ARG;       // the pages behind a rewind have gone back
   for (int i = 0; i < e->n_layers; ++i) {
     LayerDev& L = e->layers[i];
     if (!L.is_linear) continue;
@@ -1484,7 +1623,7 @@ void sl_full_snap_free(sl_full_snap* s) {
 // (per head the used rows), V bytes; GDN: u32 convCount, stateCount, history bytes, state bytes.
 static const uint32_t PERSIST_MAGIC = 0x31535751u, PERSIST_FORMAT = 1u;
 size_t sl_persist_size(sl_engine* e) {
-  if (!e) return 0;
+  if (!e || e->kv4) return 0;
   size_t n = 12;
   for (auto& L : e->layers) {
     n += 4;
@@ -1495,6 +1634,7 @@ size_t sl_persist_size(sl_engine* e) {
 }
 int sl_persist_write(sl_engine* e, void* dst, size_t cap) {
   SL_ENTER(e);
+  if (e->kv4) return SL_ERR_UNSUPPORTED;
   if (!dst || cap < sl_persist_size(e)) return SL_ERR_ARG;
   uint8_t* p = (uint8_t*)dst;
   auto u32 = [&](uint32_t v) { std::memcpy(p, &v, 4); p += 4; };
@@ -1522,6 +1662,7 @@ int sl_persist_write(sl_engine* e, void* dst, size_t cap) {
 }
 int sl_persist_restore(sl_engine* e, const void* src, size_t len) {
   SL_ENTER(e);
+  if (e->kv4) return SL_ERR_UNSUPPORTED;
   if (!src) return SL_ERR_ARG;
   const uint8_t* p = (const uint8_t*)src;
   const uint8_t* end = p + len;
@@ -1559,6 +1700,118 @@ int sl_persist_restore(sl_engine* e, const void* src, size_t len) {
   return push_state(e);
 }
 
+namespace {
+// Slots of rows 0 .. n - 1 of this sequence (and pages for them), as if they came now.
+int kv4_whole(sl_engine* e, int n) {
+  Kv4Lens lens = kv4_lens(*e->kv4);
+  lens.ctx[e->kv4_seq] = 0; lens.nw[e->kv4_seq] = n;
+  if (!kv4_fits(*e->kv4, lens)) return SL_ERR_TOO_LARGE;
+  kv4_begin(e, lens);
+  return e->fault.empty() ? SL_OK : SL_ERR_DEVICE;
+}
+// Device memory for the span of a call.
+struct Temp {
+  void* p = nullptr;
+  ~Temp() { if (p) (void)hipFree(p); }
+};
+int kv4_read_rows(sl_engine* e, const LayerDev& L, uint16_t* k, uint16_t* v) {
+  const int n = e->pos;
+  if (n == 0 || (!k && !v)) return SL_OK;
+  int r = kv4_whole(e, n); if (r) return r;
+  const size_t row = (size_t)SL_ATT_KV * SL_ATT_D * 2, head = SL_ATT_D * 2;
+  Temp t;
+  SL_TRY(e, hipMalloc(&t.p, 2 * n * row));
+  uint8_t* dev[2] = {(uint8_t*)t.p, (uint8_t*)t.p + n * row};
+  const sl_kv4_pool pool = kv4_pool(*e->kv4, L);
+  r = sl_kv4_read(&pool, e->kv4->slot, n, SL_F16, dev[0], dev[1], e->stream);
+  if (r) { kv4_failed(e, "sl_kv4_read", r); return SL_ERR_DEVICE; }
+  uint16_t* host[2] = {k, v};
+  for (int i = 0; i < 2; ++i)
+    for (int h = 0; h < SL_ATT_KV && host[i]; ++h)
+      SL_TRY(e, hipMemcpy2DAsync(host[i] + (size_t)h * n * SL_ATT_D, head, dev[i] + h * head, row, head, n, hipMemcpyDeviceToHost, e->stream));
+  SL_TRY(e, hipStreamSynchronize(e->stream));
+  return SL_OK;
+}
+int kv4_load_rows(sl_engine* e, const LayerDev& L, const uint16_t* k, const uint16_t* v, int n) {
+  if (n > 0 && (!k || !v)) return SL_ERR_ARG;           // (both are quantised together)
+  int r = kv4_whole(e, n); if (r) return r;
+  if (n == 0) return SL_OK;
+  const size_t bytes = (size_t)SL_ATT_KV * n * SL_ATT_D * 2;
+  Temp t;
+  SL_TRY(e, hipMalloc(&t.p, 2 * bytes));
+  uint16_t* dev[2] = {(uint16_t*)t.p, (uint16_t*)((uint8_t*)t.p + bytes)};
+  SL_TRY(e, hipMemcpyAsync(dev[0], k, bytes, hipMemcpyHostToDevice, e->stream));
+  SL_TRY(e, hipMemcpyAsync(dev[1], v, bytes, hipMemcpyHostToDevice, e->stream));
+  const sl_kv4_pool pool = kv4_pool(*e->kv4, L);
+  sl_kv4_append_args a{};
+  a.n_tokens = n; a.dtype = SL_F16; a.k = dev[0]; a.v = dev[1]; a.slot = e->kv4->slot;
+  a.k_token = a.v_token = SL_ATT_D; a.k_head = a.v_head = (int64_t)n * SL_ATT_D;
+  r = sl_kv4_append(&pool, &a, e->stream);
+  if (r) { kv4_failed(e, "sl_kv4_append", r); return SL_ERR_DEVICE; }
+  SL_TRY(e, hipStreamSynchronize(e->stream));
+  return SL_OK;
+}
+}  // namespace
+int sl_set_kv4(sl_engine* e, int page_size, int n_pages) {
+  SL_ENTER(e);
+  if (!e->has_attn) return SL_ERR_UNSUPPORTED;
+  if (e->kv4 || e->base_of || e->lane_refs > 0 || e->pos != 0 || n_pages < 0) return SL_ERR_ARG;
+  const int64_t page_bytes = sl_kv4_page_bytes(page_size, SL_ATT_KV, SL_ATT_D);
+  if (page_bytes == 0) return SL_ERR_UNSUPPORTED;
+  const int width = (e->max_seq + page_size - 1) / page_size;
+  if (n_pages == 0) n_pages = width;
+  if ((int64_t)n_pages * page_size > 0x7fffffffLL || (int64_t)KV4_SEQS * width + n_pages > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
+  const int rows = std::max(e->max_seq, e->max_m);
+  // everything is allocated before anything of the engine changes: a device without the memory leaves the fp16 caches
+  std::vector<void*> mem;
+  auto get = [&](size_t bytes) -> void* {
+    void* p = nullptr;
+    if (hipMalloc(&p, bytes) != hipSuccess) { (void)hipGetLastError(); return nullptr; }
+    mem.push_back(p);
+    return p;
+  };
+  auto ints = [&](size_t n) { return (int32_t*)get(n * 4); };
+  std::unique_ptr<Kv4Store> k(new (std::nothrow) Kv4Store());
+  if (!k) return SL_ERR_DEVICE;
+  k->page_size = page_size; k->n_pages = n_pages; k->width = width; k->max_rows = rows; k->max_seq = e->max_seq;
+  bool got = true;
+  for (int i = 0; i < 2; ++i) {
+    k->table[i] = ints((size_t)KV4_SEQS * width); k->held[i] = ints(KV4_SEQS); k->free_list[i] = ints(n_pages); k->free_count[i] = ints(1);
+    got = got && k->table[i] && k->held[i] && k->free_list[i] && k->free_count[i];
+  }
+  k->ctx = ints(KV4_SEQS); k->nw = ints(KV4_SEQS); k->q_start = ints(KV4_SEQS + 1); k->kv_len = ints(KV4_SEQS); k->slot = ints(rows); k->pos = ints(rows); k->unserved = ints(1);
+  got = got && k->ctx && k->nw && k->q_start && k->kv_len && k->slot && k->pos && k->unserved;
+  std::vector<void*> pages(e->n_layers, nullptr);
+  for (int i = 0; i < e->n_layers && got; ++i)
+    if (!e->layers[i].is_linear) got = (pages[i] = get((size_t)n_pages * page_bytes)) != nullptr;
+  if (!got) {
+    for (void* p : mem) (void)hipFree(p);
+    return SL_ERR_TOO_LARGE;
+  }
+  std::vector<int32_t> order(n_pages);
+  for (int i = 0; i < n_pages; ++i) order[i] = n_pages - 1 - i;            // (pages come off the end)
+  const int32_t count = n_pages;
+  e->allocs.insert(e->allocs.end(), mem.begin(), mem.end());
+  SL_TRY(e, hipMemsetAsync(k->held[0], 0, KV4_SEQS * 4, e->stream));
+  SL_TRY(e, hipMemsetAsync(k->table[0], 0xff, (size_t)KV4_SEQS * width * 4, e->stream));
+  SL_TRY(e, hipMemcpyAsync(k->free_list[0], order.data(), (size_t)n_pages * 4, hipMemcpyHostToDevice, e->stream));
+  SL_TRY(e, hipMemcpyAsync(k->free_count[0], &count, 4, hipMemcpyHostToDevice, e->stream));
+  SL_TRY(e, hipStreamSynchronize(e->stream));
+  for (int i = 0; i < e->n_layers; ++i) {
+    LayerDev& L = e->layers[i];
+    if (L.is_linear) continue;
+    for (uint16_t** p : {&L.kcache, &L.vcache}) {
+      e->allocs.erase(std::remove(e->allocs.begin(), e->allocs.end(), (void*)*p), e->allocs.end());
+      (void)hipFree(*p);
+      *p = nullptr;
+    }
+    L.kv4 = pages[i];
+  }
+  k->seq[0] = e;
+  e->kv4 = k.release(); e->kv4_seq = 0; e->dec_grid = 0;
+  return SL_OK;
+}
+
 int sl_read_layer_cache(sl_engine* e, int layer, void* a, void* b) {
   SL_ENTER(e);
   if (layer < 0 || layer >= e->n_layers) return SL_ERR_ARG;
@@ -1566,6 +1819,8 @@ int sl_read_layer_cache(sl_engine* e, int layer, void* a, void* b) {
   if (L.is_linear) {
     if (a) { r = copy_sync(e, a, L.hist[e->parity[layer]], HIST_ELEMS * 2, hipMemcpyDeviceToHost); if (r) return r; }
     if (b) { r = copy_sync(e, b, L.state[e->parity[layer]], STATE_ELEMS * 4, hipMemcpyDeviceToHost); if (r) return r; }
+  } else if (L.kv4) {
+    return kv4_read_rows(e, L, (uint16_t*)a, (uint16_t*)b);
   } else {
     const size_t rb = (size_t)e->pos * SL_ATT_D * 2;
     for (int h = 0; h < SL_ATT_KV && rb; ++h) {
@@ -1585,6 +1840,11 @@ int sl_load_layer_cache(sl_engine* e, int layer, const void* a, const void* b, i
     return SL_OK;
   }
   if (len < 0 || len > e->max_seq) return SL_ERR_ARG;
+  if (L.kv4) {
+    r = kv4_load_rows(e, L, (const uint16_t*)a, (const uint16_t*)b, len); if (r) return r;
+    e->pos = len;
+    return push_state(e);
+  }
   const size_t rb = (size_t)len * SL_ATT_D * 2;
   for (int h = 0; h < SL_ATT_KV && rb; ++h) {
     if (a) { r = copy_sync(e, L.kcache + (size_t)h * e->max_seq * SL_ATT_D, (const uint8_t*)a + h * rb, rb, hipMemcpyHostToDevice); if (r) return r; }
@@ -1659,6 +1919,7 @@ int sl_attn_layer_rows(sl_engine* e, int layer, const uint16_t* x, int m, uint16
   } else {
     HiddenArgs ha{e->xn, nullptr, nullptr, nullptr, nullptr};
     e->last_block_flow = false;
+    if (e->kv4) kv4_begin(e, m);
     launch_attn_mixer(e, e->layers[layer], m, ha, nullptr, 0);
     SL_TRY(e, hipEventRecord(e->ev1, e->stream));
     r = read_back(e, out, e->mix, (size_t)m * H * 2, "attnLayerRows"); if (r) return r;

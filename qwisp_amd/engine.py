@@ -107,6 +107,11 @@ class SeedlessFusedForward:
         """forwardRowsHybrid (SeedlessFusedVerify.swift:4247): prefill chunks of >= 16 rows on the matrix cores."""
         self.lib.check(self.lib.dll.sl_set_hybrid(self.h, 1 if enable else 0), "sl_set_hybrid", self.gpu_fault)
 
+    def set_kv4(self, page_size=64, n_pages=0):
+        """Keys and values of this engine and its later lanes in 4 bits, in n_pages shared pages (0: enough for
+        max_seq_len tokens); once, before the first token and the first lane."""
+        self.lib.check(self.lib.dll.sl_set_kv4(self.h, page_size, n_pages), "sl_set_kv4", self.gpu_fault)
+
     def set_persistent(self, enable=True):
         return self.lib.dll.sl_set_persistent(self.h, int(enable)) == abi.SL_OK
 
