@@ -251,6 +251,41 @@ def test_any_guess_of_the_longest_is_right(max_keys):
     check(128, "f16", 8, 2, 64, [1500, 3, 800], [1, 2, 1], max_keys=max_keys, seed=7)
 
 
+@pytest.mark.parametrize("dim, dtype, page", [(256, "f16", 64), (128, "bf16", 16)])
+def test_more_requests_than_a_wave(dim, dtype, page):
+    rng = np.random.default_rng(30)
+    lens = rng.integers(0, 300, 90).tolist()
+    check(dim, dtype, 4, 2, page, lens, rng.integers(0, 3, 90).tolist(), gate=True, seed=30)
+
+
+@pytest.mark.parametrize("dim, dtype, heads, kv, page, lens, rows", [
+    (256, "f16", 4, 1, 32, [2600, 40, 900], [30, 25, 17]),          # 64 rows a workgroup, the long axis in parts
+    (256, "bf16", 8, 1, 64, [1500, 1500], [5, 1]),                   # 40 and 8 rows: tiles of 16
+    (128, "f16", 4, 2, 16, [2500, 77], [40, 20]),                    # tiles of 32
+    (64, "bf16", 3, 3, 64, [3000, 1000], [33, 50])])
+def test_many_rows_against_long_axes(dim, dtype, heads, kv, page, lens, rows):
+    check(dim, dtype, heads, kv, page, lens, rows, gate=True, seed=31)
+
+
+def test_more_than_64_requests_with_many_rows():
+    rng = np.random.default_rng(32)
+    check(256, "f16", 4, 1, 16, rng.integers(20, 200, 70).tolist(), [0, 20, 1] * 23 + [3], seed=32)
+
+
+def test_values_at_the_edge_of_fp16():
+    """Scales up to 8734: weights times scales stay within fp16 while the running maximum lags."""
+    m, rng = kv4(), np.random.default_rng(33)
+    n, dim, page = 700, 128, 32
+    k = ref.quantise(np.sort(rng.normal(size=(n + 4, 1, dim)), axis=0))       # scores that keep growing
+    v = ref.quantise(rng.choice([-65504.0, 65504.0, 1.0], size=(n + 4, 1, dim)))
+    pool = m.Pool(gpu(ref.pack(k, v, page, 1, dim)), page, 1, dim)
+    table = np.arange(22, dtype=np.int32)[None]
+    q = gpu(np.abs(rng.normal(size=(2, 4, dim))), torch.bfloat16)
+    out = m.attention(pool, q, gpu(table), gpu(np.array([0, 2], np.int32)), gpu(np.array([n], np.int32)), max_rows=2, max_keys=n)
+    want, tol = ref.attention(f64(q), dict(k=k, v=v), table, [0, 2], [n], page, 22, dim ** -0.5, eps_out=HALF_STEP["bf16"])
+    assert (np.abs(f64(out) - want) <= tol).all()
+
+
 def test_long_context():
     check(256, "f16", 16, 2, 64, [20011, 513], [1, 1], gate=True, seed=8)
 
