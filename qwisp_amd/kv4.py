@@ -89,14 +89,22 @@ def _pool(pool):
     return abi.Kv4Pool(p.data_ptr(), p.shape[0], page_size, n_kv, head_dim)
 
 
+# The current stream's handle without a Stream object around it (2 us of a call's 15), where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_functions = {}
+
+
 def _call(name, device, *args):
     """The library's call on torch's current stream of `device`, with that device current."""
-    fn = getattr(_lib.get().dll, name)
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.get().dll, name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            status = fn(*args, _raw_stream(index))
     if status:
         _lib.Library.check(status, name)
 
