@@ -1331,17 +1331,17 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
   }
 }
 
-// Partial sums joined.  TILE 16 or 32: a workgroup per row (there are many parts); its waves read 256 / D partial rows at once, 16
-// bytes a lane, four such loads in flight, and meet in LDS.  TILE 64: a wave per row (few parts), 16 rows a workgroup.
-template <int D, bool BF, int TILE>
+// Partial sums joined.  WIDE: a workgroup per row; its waves read 256 / D partial rows at once, 16 bytes a lane, four such loads
+// in flight, and meet in LDS.  Otherwise a wave per row, 16 rows a workgroup.
+template <int D, bool BF, int TILE, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
-  constexpr int LANES = D / 4, PER_WAVE = 64 / LANES, WAVES = TILE == 64 ? 1 : 4, PER = WAVES * PER_WAVE;
+  constexpr int LANES = D / 4, PER_WAVE = 64 / LANES, WAVES = WIDE ? 4 : 1, PER = WAVES * PER_WAVE;
   __shared__ float s_red[4];
   __shared__ float4 s_y[4 * PER_WAVE][LANES];
   __shared__ float s_sum[4 * PER_WAVE];
   const int h = blockIdx.y, r = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, group = a.n_heads / pool.n_kv;
   int start, n;
-  const int rows = rows_of(a, r, start, n), row_first = TILE == 64 ? blockIdx.x * 16 : blockIdx.x;
+  const int rows = rows_of(a, r, start, n), row_first = WIDE ? blockIdx.x : blockIdx.x * 16;
   if (row_first >= rows * group) return;
   const int tile = row_first / TILE, tiles = (rows * group + TILE - 1) / TILE, share = cut.first[a.n_req + 1];
   const long keys = seen_keys(a, pool, r);
@@ -1355,14 +1355,14 @@ __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_a
   const long first = cut.first[r] + (item < full ? (long)(item & ~7) * most + (item & 7) : (long)full * most + (item - full));
   if (cut.first[r] + (long)items * most > cut.slots) return;      // (row offsets that overlap: more parts than rows allow)
   const float* stat = cut.part + cut.slots * cut.rows * D;
-  const int d = 4 * (lane % LANES), mine = (TILE == 64 ? 0 : wave * PER_WAVE) + lane / LANES;
-  for (int j = 0; j < (TILE == 64 ? 4 : 1); ++j) {
-    const int row = TILE == 64 ? row_first + wave * 4 + j : row_first, in = row % TILE;
+  const int d = 4 * (lane % LANES), mine = (WIDE ? wave * PER_WAVE : 0) + lane / LANES;
+  for (int j = 0; j < (WIDE ? 1 : 4); ++j) {
+    const int row = WIDE ? row_first : row_first + wave * 4 + j, in = row % TILE;
     if (row >= rows * group) return;
     float best = -__builtin_inff();
-    for (int i = TILE == 64 ? lane : tid; i < count; i += 64 * WAVES) best = fmaxf(best, stat[(first + (long)i * side) * cut.rows + in]);
+    for (int i = WIDE ? tid : lane; i < count; i += 64 * WAVES) best = fmaxf(best, stat[(first + (long)i * side) * cut.rows + in]);
     best = tree_max<64>(best);
-    if constexpr (TILE != 64) {
+    if constexpr (WIDE) {
       if (lane == 0) s_red[wave] = best;
       __syncthreads();
       best = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
@@ -1388,23 +1388,23 @@ __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_a
         y.x = fmaf(f, p[u].x, y.x); y.y = fmaf(f, p[u].y, y.y); y.z = fmaf(f, p[u].z, y.z); y.w = fmaf(f, p[u].w, y.w);
       }
     }
-    const int slot_y = TILE == 64 ? wave * PER_WAVE + lane / LANES : mine;
+    const int slot_y = WIDE ? mine : wave * PER_WAVE + lane / LANES;
     s_y[slot_y][lane % LANES] = y;
     if (lane % LANES == 0) s_sum[slot_y] = sum;
-    if constexpr (TILE != 64) __syncthreads(); else wave_lds_order();
-    const int lead = TILE == 64 ? lane : tid;
+    if constexpr (WIDE) __syncthreads(); else wave_lds_order();
+    const int lead = WIDE ? tid : lane;
     if (lead < LANES) {
       sum = 0.0f; y = make_float4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int from = (TILE == 64 ? wave * PER_WAVE : 0) + i;
+        const int from = (WIDE ? 0 : wave * PER_WAVE) + i;
         const float4 x = s_y[from][lead];
         sum += s_sum[from]; y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
       }
       const int tok = row / group;
       finish_row<BF>(a, start + tok, h * group + (row - tok * group), 4 * lead, y, sum);
     }
-    if constexpr (TILE == 64) wave_lds_order();
+    if constexpr (!WIDE) wave_lds_order();
   }
 }
 
@@ -1430,8 +1430,10 @@ struct AttnShape {
   AttnCut cut{};
   int tile = 16;              // rows of a workgroup
   int grid = 0;
+  bool wide = true;           // many parts to a row: a workgroup joins one
   int64_t part_bytes = 0, bytes = 0;
 };
+constexpr int64_t MAX_GROUPS = 0xffffffffLL / 256;      // workgroups of 256 along one axis: a launch has fewer than 2^32 threads there
 int compute_units() {         // of the current device
   static std::atomic<int> known[64];
   int dev = 0;
@@ -1447,7 +1449,7 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   if (!p || !a || a->n_heads < 1 || p->n_kv < 1 || a->n_heads % p->n_kv || a->n_req < 1 || a->max_rows < 1 || !layout_ok(p->page_size, p->n_kv, p->head_dim)) return SL_ERR_ARG;
   const int64_t group = a->n_heads / p->n_kv, rows = (int64_t)std::min(a->max_rows, std::max(a->n_tokens, 1)) * group;
   const int64_t widest = (int64_t)a->table_width * p->page_size;
-  if (a->n_req > AT_MAX_REQ || a->n_heads > 65535 || rows > (1ll << 30) || widest > 0x7fffffffLL - 4096) return SL_ERR_TOO_LARGE;
+  if (a->n_req > AT_MAX_REQ || a->n_heads > 65535 || rows > MAX_GROUPS || widest > 0x7fffffffLL - 4096) return SL_ERR_TOO_LARGE;
   // 256 dims: 16 rows a workgroup, from 49 rows on 64 (32 lanes of 32 rows 66 against 98 us, of 64 rows 140 against 103); fewer dims: a
   // second row tile as soon as there are rows for it (128 dims, six requests of 32 rows at 20-32K: 71 against 83 us).
   sh.tile = p->head_dim == 256 ? (rows <= 48 ? 16 : 64) : (rows <= 16 ? 16 : 32);
@@ -1456,13 +1458,16 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   const int64_t items = p->n_kv * std::min(a->n_req * ((rows + tile - 1) / tile), a->n_tokens * group / tile + a->n_req);
   const int64_t resident = (int64_t)compute_units() * (tile == 64 ? 2 : attn_places(p->head_dim, tile / 16));
   const int64_t rounds = items * (std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1);
-  if (p->n_kv * a->n_req * ((rows + tile - 1) / tile) + 2 * resident > 0x7fffffffLL) return SL_ERR_TOO_LARGE;
+  if (p->n_kv * a->n_req * ((rows + tile - 1) / tile) + 4 * resident > MAX_GROUPS) return SL_ERR_TOO_LARGE;
   // 16 and 32 rows: parts are equally long, so with few items they and the parts together fill the chip once; with more, parts of half
   // a turn.  64 rows: row tiles see different numbers of keys, the longest first, and the chip takes parts as it gets free; tiles that
   // fill it by themselves are cut where they are twice the mean (2048 rows of a prompt 147 us, cut at the mean 168).
   sh.cut.want = (int)std::min(tile == 64 ? (items >= resident ? resident / 2 : resident) : (items <= resident / 2 ? resident - items : 2 * resident), std::max<int64_t>(rounds, 1));
   // a request's items are numbered with the parts of its longest row tile: at most twice the mean of longest and shortest
   sh.grid = (int)(2 * sh.cut.want + items);
+  // Joining: a workgroup per row while there are few rows or many parts to each, else a wave per row (2333 rows of 64 dims on 16K keys
+  // 213 us with the first, 183 with the second; 128 lanes of 8 rows 102 and 105, 64 rows on 32K keys 97 and 113).
+  sh.wide = rows * p->n_kv * a->n_req <= 4096 || sh.cut.want > 8 * items;
   sh.cut.slots = sh.grid; sh.cut.rows = (int)std::min<int64_t>(rows, tile);
   sh.part_bytes = sh.cut.slots * sh.cut.rows * (p->head_dim + 2) * 4;
   sh.part_bytes = (sh.part_bytes + 15) & ~15ll;
@@ -1481,7 +1486,8 @@ void launch_attn(const Pool& pool, const sl_kv4_attn_args& a, const AttnCut& cut
 #define KV4_ATTN(TILE, KERNEL, LDS)                                                                            \
   do {                                                                                                         \
     launch_attn_kernel(KERNEL, LDS, pool, a, cut, sh.grid, st);                                                \
-    hipLaunchKernelGGL((k_kv4_attn_merge<D, BF, TILE>), dim3(TILE == 64 ? (rows + 15) / 16 : rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut); \
+    if (sh.wide) hipLaunchKernelGGL((k_kv4_attn_merge<D, BF, TILE, true>), dim3(rows, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut);               \
+    else hipLaunchKernelGGL((k_kv4_attn_merge<D, BF, TILE, false>), dim3((rows + 15) / 16, pool.n_kv, a.n_req), dim3(256), 0, st, pool, a, cut);          \
   } while (0)
   if (sh.tile == 16) KV4_ATTN(16, (k_kv4_attn<D, BF, 1>), (AttnLds<D, 1>::BYTES));
   else if constexpr (D == 256) KV4_ATTN(64, (k_kv4_attn_tile<D, BF>), TileLds<D>::BYTES);
@@ -1513,8 +1519,12 @@ int sl_kv4_plan(const sl_kv4_plan_args* a, void* stream) {
   if ((a->n_req > 0 && (!a->ctx_len || !a->new_len || !a->held_in || !a->held_out || !a->kv_len)) || (table && (!a->table_in || !a->table_out)) ||
       (a->n_free > 0 && (!a->free_in || !a->free_out)) || !a->free_count_in || !a->free_count_out || !a->q_start || !a->unserved ||
       (a->max_tokens > 0 && (!a->slot || !a->pos))) return SL_ERR_ARG;
-  if ((table && a->table_in == a->table_out) || (a->n_free > 0 && a->free_in == a->free_out) || a->free_count_in == a->free_count_out ||
-      (a->n_req > 0 && a->held_in == a->held_out)) return SL_ERR_ARG;
+  // (a step planned into the tensors that it is planned from: workgroups would read what others have written)
+  const int32_t* ins[] = {a->n_req ? a->ctx_len : nullptr, a->n_req ? a->new_len : nullptr, a->n_req ? a->held_in : nullptr, table ? a->table_in : nullptr,
+                          a->n_free ? a->free_in : nullptr, a->free_count_in};
+  const int32_t* outs[] = {a->n_req ? a->held_out : nullptr, a->n_req ? a->kv_len : nullptr, table ? a->table_out : nullptr, a->n_free ? a->free_out : nullptr,
+                           a->free_count_out, a->q_start, a->max_tokens ? a->slot : nullptr, a->max_tokens ? a->pos : nullptr, a->unserved};
+  for (const int32_t* in : ins) for (const int32_t* out : outs) if (in && in == out) return SL_ERR_ARG;
   const int64_t most = std::max(a->n_free, a->max_tokens);
   const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(512, std::max<int64_t>(a->n_req, (most + PLAN_THREADS - 1) / PLAN_THREADS)));
   (void)hipGetLastError();            // an error an unrelated earlier call of this thread left behind is not this call's
@@ -1534,7 +1544,7 @@ int sl_kv4_append(const sl_kv4_pool* p, const sl_kv4_append_args* a, void* strea
   const int64_t strides[] = {a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->out_token, a->out_head};
   for (int i = a->q ? 0 : 2; i < (a->q ? 8 : 6); ++i) if (strides[i] % 4) return SL_ERR_ARG;
   if (a->rot_dim && (!aligned(a->cos, 16) || !aligned(a->sin, 16))) return SL_ERR_ARG;
-  if (a->n_heads > 32768 || a->n_tokens > 0x7ffffff0) return SL_ERR_TOO_LARGE;
+  if (a->n_heads > 32768 || a->n_tokens > 4 * MAX_GROUPS) return SL_ERR_TOO_LARGE;
   const int heads = 256 / p->head_dim, q_units = a->q ? (a->n_heads + heads - 1) / heads : 0;
   const int kv_units = (p->n_kv + heads - 1) / heads;
   // enough waves to fill the chip come first, then longer runs of heads (8192 waves: eight per SIMD)
@@ -1583,9 +1593,10 @@ int sl_kv4_read(const sl_kv4_pool* p, const int32_t* slots, int n, int dtype, vo
   if (n < 0 || (dtype != SL_F32 && dtype != SL_F16) || !aligned(k_out, 16) || !aligned(v_out, 16)) return SL_ERR_ARG;
   if (n == 0 || (!k_out && !v_out)) return SL_OK;
   if (!slots) return SL_ERR_ARG;
-  const unsigned blocks = (unsigned)(((int64_t)n + 4 * (1024 / p->head_dim) - 1) / (4 * (1024 / p->head_dim)));
+  const int64_t blocks = ((int64_t)n + 4 * (1024 / p->head_dim) - 1) / (4 * (1024 / p->head_dim));
+  if (blocks > MAX_GROUPS) return SL_ERR_TOO_LARGE;
   (void)hipGetLastError();
-#define KV4_CALL(D, F16) hipLaunchKernelGGL((k_kv4_read<D, F16>), dim3(blocks, p->n_kv), dim3(256), 0, (hipStream_t)stream, pool, slots, n, k_out, v_out)
+#define KV4_CALL(D, F16) hipLaunchKernelGGL((k_kv4_read<D, F16>), dim3((unsigned)blocks, p->n_kv), dim3(256), 0, (hipStream_t)stream, pool, slots, n, k_out, v_out)
   KV4_BY_LAYOUT(p->head_dim, dtype == SL_F16, KV4_CALL);
 #undef KV4_CALL
   return launch_status();

@@ -67,6 +67,8 @@ def rope_tables(max_pos, rot_dim, theta=1e7, device="cuda"):
 
 
 def _flat(t, shape, dtype, device, what):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: a tensor is wanted")
     if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: {dtype} {list(shape)} side by side on {device} is wanted, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -74,6 +76,8 @@ def _flat(t, shape, dtype, device, what):
 
 def _rows(t, shape, dtype, device, what):
     """Address and strides of [tokens, heads, dims] with the dims side by side."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: a tensor is wanted")
     token, head, dim = t.stride() if t.dim() == 3 else (0, 0, 0)
     if t.dtype is not dtype or t.shape != shape or t.device != device or dim != 1:
         raise ValueError(f"{what}: {dtype} {list(shape)} with dims side by side on {device} is wanted, got {t.dtype} {list(t.shape)} "
@@ -155,6 +159,8 @@ def append(pool, q, k, v, slot, pos, cos, sin, q_weight, k_weight, eps=1e-6, out
             qw_at = _flat(q_weight, (dim,), dt, dev, "q_weight")
     if k_weight is not None:
         kw_at = _flat(k_weight, (dim,), dt, dev, "k_weight")
+    if (cos is None) != (sin is None) or (cos is not None and cos.dim() != 2):
+        raise ValueError("cos and sin [positions, rotated dims / 2] are wanted, or neither")
     if cos is not None:
         max_pos, rot = cos.shape[0], 2 * cos.shape[1]
         cos_at, sin_at, pos_at = _flat(cos, cos.shape, torch.float32, dev, "cos"), _flat(sin, cos.shape, torch.float32, dev, "sin"), _flat(pos, (n,), i32, dev, "pos")
@@ -163,9 +169,19 @@ def append(pool, q, k, v, slot, pos, cos, sin, q_weight, k_weight, eps=1e-6, out
     return out
 
 
+def _workspace(device, p, a):
+    """(The library cuts a call by the current device's compute units.)"""
+    size = _lib.get().dll.sl_kv4_attention_workspace
+    if torch.cuda.current_device() == device.index:
+        return size(p, a)
+    with torch.cuda.device(device):
+        return size(p, a)
+
+
 def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, gate=None, out=None, workspace=None):
     """sl_kv4_attention: q [tokens, heads, dims] against the pages of each request; `workspace` (uint8, of at least
-    attention_workspace() bytes) is taken from torch if it is not given."""
+    attention_workspace() bytes) is taken from torch if it is not given.  Rows that no request has are not written: in
+    a new `out` they hold whatever the memory held."""
     p, dev = _pool(pool), pool.pages.device
     if q.dtype not in _DTYPES or q.dim() != 3 or table.dim() != 2:
         raise ValueError(f"queries [tokens, heads, dims] in float16 or bfloat16 and a table [n_req, width] are wanted, got {q.dtype} {list(q.shape)}, {list(table.shape)}")
@@ -177,10 +193,11 @@ def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, g
     q_at, out_at, gate_at = _rows(q, shape, dt, dev, "q"), _rows(out, shape, dt, dev, "out"), (None, 0, 0)
     if gate is not None:
         gate_at = _rows(gate, shape, dt, dev, "gate")
+    max_rows, max_keys = min(max_rows, n), min(max_keys, 0x7fffffff)      # (the struct's are 32 bits)
     a = abi.Kv4AttnArgs(n_req, n, heads, _DTYPES[dt], table.shape[1], max_rows, max_keys, dim ** -0.5 if scale is None else scale, q_at[0], gate_at[0], out_at[0],
                         *q_at[1:], *gate_at[1:], *out_at[1:], _flat(table, table.shape, i32, dev, "table"), _flat(q_start, (n_req + 1,), i32, dev, "q_start"),
                         _flat(kv_len, (n_req,), i32, dev, "kv_len"))
-    need = _lib.get().dll.sl_kv4_attention_workspace(p, a)
+    need = _workspace(dev, p, a)
     if need > 0:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -193,8 +210,8 @@ def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, g
 
 def attention_workspace(pool, n_tokens, n_heads, n_req, table_width, max_rows, max_keys):
     """Bytes of workspace that attention() takes for such a call (0: a call that has nothing to do, or is refused)."""
-    a = abi.Kv4AttnArgs(n_req=n_req, n_tokens=n_tokens, n_heads=n_heads, table_width=table_width, max_rows=max_rows, max_keys=max_keys)
-    return _lib.get().dll.sl_kv4_attention_workspace(_pool(pool), a)
+    a = abi.Kv4AttnArgs(n_req=n_req, n_tokens=n_tokens, n_heads=n_heads, table_width=table_width, max_rows=min(max_rows, n_tokens), max_keys=min(max_keys, 0x7fffffff))
+    return _workspace(pool.pages.device, _pool(pool), a)
 
 
 def read(pool, slots, dtype=torch.float32):

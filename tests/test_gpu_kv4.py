@@ -272,6 +272,14 @@ def test_more_than_64_requests_with_many_rows():
     check(256, "f16", 4, 1, 16, rng.integers(20, 200, 70).tolist(), [0, 20, 1] * 23 + [3], seed=32)
 
 
+@pytest.mark.parametrize("dim, dtype, most, n", [(256, "bf16", 15, 70), (256, "f16", 12, 70), (128, "f16", 15, 70), (128, "bf16", 4, 130), (64, "f16", 17, 64), (64, "bf16", 4, 130)])
+def test_many_rows_with_few_parts_each(dim, dtype, most, n):
+    rng = np.random.default_rng(34)
+    lens, rows = rng.integers(0, 90, n), rng.integers(0, 3, n)
+    lens[::23], rows[::23] = 1000 + np.arange(len(lens[::23])), most
+    check(dim, dtype, 8, 2, 64, lens.tolist(), rows.tolist(), gate=True, seed=34)
+
+
 def test_values_at_the_edge_of_fp16():
     """Scales up to 8734: weights times scales stay within fp16 while the running maximum lags."""
     m, rng = kv4(), np.random.default_rng(33)
@@ -410,3 +418,26 @@ def test_tensors_of_the_wrong_kind_are_refused():
         m.new_pool(2, 24, 1, 64)
     with pytest.raises(ValueError):
         m.append(pool, q, q, q, torch.zeros(3, **i32), None, None, None, None, None)
+
+
+def test_what_is_left_out_is_refused():
+    m = kv4()
+    from qwisp_amd.lib import SeedlessError
+    pool = m.new_pool(2, 16, 1, 64)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q, one, few = torch.zeros(2, 1, 64, dtype=torch.float16, device="cuda"), torch.zeros(1, **i32), torch.zeros(2, **i32)
+    cos, sin = m.rope_tables(4, 16)
+    for bad in (dict(pos=None), dict(sin=None), dict(cos=None), dict(slot=None), dict(v=None), dict(cos=cos[0], sin=sin[0])):
+        with pytest.raises(ValueError):
+            m.append(pool, **{**dict(q=q, k=q, v=q, slot=few, pos=few, cos=cos, sin=sin, q_weight=None, k_weight=None), **bad})
+    with pytest.raises(ValueError):
+        m.attention(pool, q, torch.zeros(1, 1, **i32), few, None, max_rows=1, max_keys=1)
+    # a step planned into its own inputs
+    free, table, count = torch.arange(2, **i32), torch.full((1, 2), -1, **i32), torch.full((1,), 2, **i32)
+    step = m.plan(one, one + 1, table, one.clone(), free, count, 16, 2)
+    with pytest.raises(SeedlessError):
+        m.plan(step.kv_len, one + 1, table, step.held.clone(), free, count, 16, 2, out=step)
+    # numbers beyond the library's 32 bits mean what they say
+    got = m.attention(pool, q, step.table, step.q_start, step.kv_len, max_rows=1 << 33, max_keys=1 << 33)
+    want = m.attention(pool, q, step.table, step.q_start, step.kv_len, max_rows=2, max_keys=2)
+    assert torch.equal(got[:1], want[:1])

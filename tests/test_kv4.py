@@ -113,6 +113,12 @@ def test_plan_refuses(bad, status):
     assert lib.get().dll.sl_kv4_plan(plan(**bad), None) == status
 
 
+@pytest.mark.parametrize("out", ["table_out", "held_out", "free_out", "free_count_out", "q_start", "kv_len", "slot", "pos", "unserved"])
+@pytest.mark.parametrize("inp", ["ctx_len", "new_len", "table_in", "held_in", "free_in", "free_count_in"])
+def test_plan_refuses_an_output_that_is_an_input(out, inp):
+    assert lib.get().dll.sl_kv4_plan(plan(**{inp: 5 * P, out: 5 * P}), None) == abi.SL_ERR_ARG
+
+
 def test_empty_calls_do_nothing():
     dll = lib.get().dll
     assert dll.sl_kv4_append(pool(), append(n_tokens=0), None) == abi.SL_OK
@@ -135,3 +141,12 @@ def test_struct_sizes_match_the_header(tmp_path):
     subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), "-o", str(tmp_path / "s"), str(src)])
     got = [int(x) for x in subprocess.check_output([str(tmp_path / "s")]).split()]
     assert got == [C.sizeof(t) for t in (abi.Kv4Pool, abi.Kv4PlanArgs, abi.Kv4AppendArgs, abi.Kv4AttnArgs)]
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    dll = lib.get().dll
+    assert dll.sl_kv4_append(pool(), append(n_tokens=0x7ffffff0), None) == abi.SL_ERR_TOO_LARGE
+    assert dll.sl_kv4_read(pool(head_dim=256), P, 0x7fffffff, abi.SL_F32, P, P, None) == abi.SL_ERR_TOO_LARGE
+    assert dll.sl_kv4_attention(pool(), attn(n_tokens=1 << 24, max_rows=1 << 24), None) == abi.SL_ERR_TOO_LARGE
+    assert dll.sl_kv4_attention(pool(n_kv=2), attn(n_tokens=1 << 22, max_rows=1 << 22, n_heads=16, n_req=4096), None) == abi.SL_ERR_TOO_LARGE
+    assert dll.sl_kv4_attention(pool(), attn(n_req=4097), None) == abi.SL_ERR_TOO_LARGE
