@@ -344,7 +344,11 @@ int sl_sched_round(sl_sched* s);
 /* LaneBatchSlots (LaneServe.swift:26): n_slots lanes on the weights of `base`; prefill in chunks of chunk_rows
  * rows, resumable at chunk boundaries (a budget grants whole chunks, rounded up, at least one); decode through
  * sl_lane_step_argmax; can_admit holds the sum of the admitted requests' seq_budget within kv_budget_tokens
- * (<= 0: n_slots * max_seq_len).  Fills `table` for sl_sched_create; destroy after the scheduler, before `base`. */
+ * (<= 0: n_slots * max_seq_len).  Fills `table` for sl_sched_create; destroy after the scheduler, before `base`.
+ * On a base with 4-bit caches (sl_set_kv4) a request's pages go back when it ends, and can_admit also waits until the pages
+ * hold what all admitted requests may grow to; without a budget (kv_budget_tokens <= 0) the pages have to hold every slot
+ * at max_seq_len, else SL_ERR_TOO_LARGE.  (A scheduler without a token budget does not ask can_admit: there a request
+ * that finds no pages ends, as any whose prompt fails.) */
 typedef struct sl_lane_slots sl_lane_slots;
 int sl_lane_slots_create(const sl_engine* base, int n_slots, int chunk_rows, int max_seq_len, long kv_budget_tokens,
                          sl_lane_slots** out, sl_batch_slots* table);
@@ -393,8 +397,12 @@ int sl_set_hybrid(sl_engine* e, int enable);
  * refuses a snapshot behind what the sequence's pages still hold; sl_read_layer_cache returns the values that the codes stand for, rounded to
  * fp16; sl_load_layer_cache quantises and takes keys and values together; the persisted-state calls answer
  * SL_ERR_UNSUPPORTED (sl_persist_size 0).  SL_ERR_UNSUPPORTED: an engine without attention layers, another page size.
- * SL_ERR_TOO_LARGE: no memory for the pages (the engine stays as it was). */
+ * SL_ERR_TOO_LARGE: no memory for the pages (the engine stays as it was).  Rows of one call share tiles, so tokens that are
+ * verified together (sl_spec_generate) may differ in their last bits from the same tokens stepped one by one. */
 int sl_set_kv4(sl_engine* e, int page_size, int n_pages);
+/* Pages that none of the sequences of this engine's 4-bit caches needs at its length now, and (where not NULL) their size
+ * and number; SL_ERR_UNSUPPORTED without such caches. */
+int sl_kv4_free_pages(const sl_engine* e, int32_t* page_size, int32_t* n_pages);
 
 /* Diagnostic in the manner of forwardRowsProfiled (SFV:4352), at the grain of one stage of the single-launch step:
  * while enabled, batch-1 steps run a variant of that kernel in which every workgroup records 100 MHz clock stamps of

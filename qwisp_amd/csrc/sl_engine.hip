@@ -1249,6 +1249,7 @@ void sl_destroy(sl_engine* e) {
     if (e->stream) (void)hipStreamSynchronize(e->stream);
     e->destroy_pending = true;
     if (e->fault.empty()) e->fault = "engine destroyed (kept alive by its lanes)";
+    if (e->kv4) e->kv4->seq[e->kv4_seq] = nullptr;    // (its own sequence's pages are the lanes')
     return;
   }
   sl_engine* root = e->base_of;
@@ -1717,10 +1718,10 @@ struct Temp {
 int kv4_read_rows(sl_engine* e, const LayerDev& L, uint16_t* k, uint16_t* v) {
   const int n = e->pos;
   if (n == 0 || (!k && !v)) return SL_OK;
-  int r = kv4_whole(e, n); if (r) return r;
   const size_t row = (size_t)SL_ATT_KV * SL_ATT_D * 2, head = SL_ATT_D * 2;
-  Temp t;
+  Temp t;                                               // (before the plan: no work stays behind a call that fails)
   SL_TRY(e, hipMalloc(&t.p, 2 * n * row));
+  int r = kv4_whole(e, n); if (r) return r;
   uint8_t* dev[2] = {(uint8_t*)t.p, (uint8_t*)t.p + n * row};
   const sl_kv4_pool pool = kv4_pool(*e->kv4, L);
   r = sl_kv4_read(&pool, e->kv4->slot, n, SL_F16, dev[0], dev[1], e->stream);
@@ -1734,11 +1735,11 @@ int kv4_read_rows(sl_engine* e, const LayerDev& L, uint16_t* k, uint16_t* v) {
 }
 int kv4_load_rows(sl_engine* e, const LayerDev& L, const uint16_t* k, const uint16_t* v, int n) {
   if (n > 0 && (!k || !v)) return SL_ERR_ARG;           // (both are quantised together)
-  int r = kv4_whole(e, n); if (r) return r;
-  if (n == 0) return SL_OK;
   const size_t bytes = (size_t)SL_ATT_KV * n * SL_ATT_D * 2;
   Temp t;
-  SL_TRY(e, hipMalloc(&t.p, 2 * bytes));
+  if (n > 0) SL_TRY(e, hipMalloc(&t.p, 2 * bytes));
+  int r = kv4_whole(e, n); if (r) return r;
+  if (n == 0) return SL_OK;
   uint16_t* dev[2] = {(uint16_t*)t.p, (uint16_t*)((uint8_t*)t.p + bytes)};
   SL_TRY(e, hipMemcpyAsync(dev[0], k, bytes, hipMemcpyHostToDevice, e->stream));
   SL_TRY(e, hipMemcpyAsync(dev[1], v, bytes, hipMemcpyHostToDevice, e->stream));
@@ -1810,6 +1811,19 @@ int sl_set_kv4(sl_engine* e, int page_size, int n_pages) {
   k->seq[0] = e;
   e->kv4 = k.release(); e->kv4_seq = 0; e->dec_grid = 0;
   return SL_OK;
+}
+
+int sl_kv4_free_pages(const sl_engine* e, int32_t* page_size, int32_t* n_pages) {
+  if (!e) return SL_ERR_ARG;
+  std::lock_guard<std::recursive_mutex> gpu_lock_(g_gpu_mutex);
+  if (!e->kv4) return SL_ERR_UNSUPPORTED;
+  const Kv4Store& k = *e->kv4;
+  const Kv4Lens lens = kv4_lens(k);
+  int left = k.n_pages;
+  for (int i = 0; i < KV4_SEQS; ++i) left -= (lens.ctx[i] + k.page_size - 1) / k.page_size;
+  if (page_size) *page_size = k.page_size;
+  if (n_pages) *n_pages = k.n_pages;
+  return left;
 }
 
 int sl_read_layer_cache(sl_engine* e, int layer, void* a, void* b) {

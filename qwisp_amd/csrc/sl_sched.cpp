@@ -180,6 +180,15 @@ struct sl_lane_slots {
   std::vector<int32_t> toks, outs;
   int chunk = 1, max_seq = 0;
   long kv_budget_tokens = 0;
+  // lanes with 4-bit caches share pages (page_size > 0): requests let in wait for the pages of their whole length
+  int32_t page_size = 0, n_pages = 0;
+  long promised = 0;                // pages of requests let in that have not begun
+  long pages(long tokens) const { return (tokens + page_size - 1) / page_size; }
+  long others() const {             // pages of sequences that are not slots
+    long held = n_pages - sl_kv4_free_pages(lanes[0], nullptr, nullptr);
+    for (sl_engine* e : lanes) held -= pages(sl_position(e));
+    return held;
+  }
 };
 
 namespace {
@@ -191,6 +200,10 @@ int lane_admit_step(void* ctx, const int32_t* prompt, int n_prompt, int slot, in
   if (slot < 0 || slot >= (int)L->lanes.size() || n_prompt < 1) return -1;
   if (seq_budget > L->max_seq || n_prompt + 1 > L->max_seq) return -1;      // would overflow the lane's KV arena
   sl_engine* e = L->lanes[slot];
+  if (L->pos[slot] == 0 && L->page_size && seq_budget > 0) {
+    L->promised -= L->promised < L->pages(seq_budget) ? L->promised : L->pages(seq_budget);
+    if (L->pages(seq_budget) > L->n_pages) return -1;                       // more than all pages
+  }
   if (L->pos[slot] == 0) {
     if (sl_reset(e) != SL_OK) return -1;
     L->reserved[slot] = seq_budget > 0 ? seq_budget : L->max_seq;
@@ -224,13 +237,20 @@ void lane_release(void* ctx, int slot) {
   sl_lane_slots* L = (sl_lane_slots*)ctx;
   if (slot < 0 || slot >= (int)L->lanes.size()) return;
   L->pos[slot] = 0; L->reserved[slot] = 0;
+  if (L->page_size) (void)sl_reset(L->lanes[slot]);        // its pages go to the others now, not when the slot is used again
 }
 int lane_can_admit(void* ctx, int prompt_len, int seq_budget) {
   sl_lane_slots* L = (sl_lane_slots*)ctx;
-  (void)prompt_len;
   long held = 0;
   for (int r : L->reserved) held += r;
-  return held + seq_budget <= L->kv_budget_tokens ? 1 : 0;
+  if (held + seq_budget > L->kv_budget_tokens) return 0;
+  // (what no pages could ever hold is let in, for admit_step to refuse; a request of no tokens never comes there)
+  if (!L->page_size || seq_budget > L->max_seq || L->pages(seq_budget) > L->n_pages || seq_budget <= prompt_len + 1) return 1;
+  long used = L->promised + L->others();
+  for (int r : L->reserved) used += L->pages(r);
+  if (used + L->pages(seq_budget) > L->n_pages) return 0;
+  L->promised += L->pages(seq_budget);
+  return 1;
 }
 
 }  // namespace
@@ -242,6 +262,9 @@ int sl_lane_slots_create(const sl_engine* base, int n_slots, int chunk_rows, int
   if (!base || !out || !table || n_slots < 1 || chunk_rows < 1 || max_seq_len < 2) return SL_ERR_ARG;
   sl_lane_slots* L = new sl_lane_slots();
   *out = L;
+  const int left = sl_kv4_free_pages(base, &L->page_size, &L->n_pages);
+  // without a budget there is no gate: the pages have to hold all slots at their longest
+  if (left >= 0 && kv_budget_tokens <= 0 && n_slots * L->pages(max_seq_len) > left) return SL_ERR_TOO_LARGE;
   const int rows = chunk_rows > n_slots ? chunk_rows : n_slots;   // lanes[0] lends its scratch rows to the batched step
   for (int i = 0; i < n_slots; ++i) {
     sl_engine* e = nullptr;

@@ -112,6 +112,13 @@ class SeedlessFusedForward:
         max_seq_len tokens); once, before the first token and the first lane."""
         self.lib.check(self.lib.dll.sl_set_kv4(self.h, page_size, n_pages), "sl_set_kv4", self.gpu_fault)
 
+    def kv4_free_pages(self):
+        """Pages of the 4-bit caches that no sequence needs at its length now."""
+        n = self.lib.dll.sl_kv4_free_pages(self.h, None, None)
+        if n < 0:
+            self.lib.check(n, "sl_kv4_free_pages", self.gpu_fault)
+        return n
+
     def set_persistent(self, enable=True):
         return self.lib.dll.sl_set_persistent(self.h, int(enable)) == abi.SL_OK
 

@@ -67,6 +67,7 @@ SIGNATURES = {
     "sl_set_persistent": (_i32, [_vp, _i32]),
     "sl_set_hybrid": (_i32, [_vp, _i32]),
     "sl_set_kv4": (_i32, [_vp, _i32, _i32]),
+    "sl_kv4_free_pages": (_i32, [_vp, C.POINTER(_i32), C.POINTER(_i32)]),
     "sl_debug_stage_clock": (_i32, [_vp, _i32, _vp, _i32]),
     "sl_stage_clock_words": (_i32, []),
     "sl_debug_set_spin_limit": (_i32, [_vp, C.c_uint32]),

@@ -169,3 +169,56 @@ def test_attention_layer_against_64_bits(attn_model, hybrid):
                 assert (np.abs(got[i, h] - want) <= tol).all(), (m, i, h)
         done += m
     e.close()
+
+
+@pytest.mark.parametrize("budget", [0, 16])
+def test_a_scheduler_with_fewer_pages_than_its_slots_could_use(hybrid_model, budget):
+    """Ten requests of different lengths on four slots and pages for about two of them: with the gate every request gets its
+    tokens; without a budget such a table is refused."""
+    from qwisp_amd.engine import LaneScheduler
+    from qwisp_amd.lib import SeedlessError
+    cfg, dev = hybrid_model
+    rng = np.random.default_rng(5)
+    jobs = [(rng.integers(0, 4096, int(n)).tolist(), int(g)) for n, g in zip(rng.integers(1, 60, 10), rng.integers(1, 40, 10))]
+    alone = make(cfg, dev, max_m=8, max_seq_len=128)
+    want = []
+    for p, n in jobs:
+        want.append(alone.greedy_generate(p, n, chain_k=4).tolist())
+        assert alone.lib.dll.sl_reset(alone.h) == 0
+    alone.close()
+    base = make(cfg, dev, page_size=16, n_pages=13, max_m=8, max_seq_len=128)
+    base.step_argmax([1, 2, 3])                          # the base's own sequence holds a page
+    assert base.kv4_free_pages() == 12
+    if budget == 0:
+        with pytest.raises(SeedlessError):
+            LaneScheduler(base, slots=4, chunk_rows=8, max_seq_len=128)
+        few = LaneScheduler(base, slots=1, chunk_rows=8, max_seq_len=128)
+        few.submit(*jobs[0])
+        assert few.run() == want[:1] and base.kv4_free_pages() == 12
+        few.close()
+    else:
+        sched = LaneScheduler(base, slots=4, chunk_rows=8, max_seq_len=128, token_budget=budget, kv_budget_tokens=512)
+        for p, n in jobs:
+            sched.submit(p, n)
+        sched.submit([1, 2], 0)
+        sched.submit([3] * 100, 100)                     # longer than a slot
+        sched.submit(*jobs[3])
+        assert sched.run() == want + [[], [], want[3]]
+        assert base.kv4_free_pages() == 12
+        sched.close()
+    base.close()
+
+
+def test_pages_of_a_base_that_is_gone_are_its_lanes(hybrid_model):
+    cfg, dev = hybrid_model
+    base = make(cfg, dev, page_size=16, n_pages=2, max_m=8, max_seq_len=32)
+    for _ in range(2):
+        assert base.step_argmax(list(range(8))) is not None
+    lane = base.new_lane(max_m=8, max_seq_len=32)
+    assert lane.step_argmax([1]) is not None and base.kv4_free_pages() == 0
+    for _ in range(2):
+        assert lane.step_argmax([1] * 7) is not None
+    assert lane.step_argmax([1] * 2) is None             # 15 tokens: the second page would be needed
+    base.close()
+    assert lane.step_argmax([1] * 2) is not None and lane.kv4_free_pages() == 0
+    lane.close()
