@@ -441,3 +441,42 @@ def test_what_is_left_out_is_refused():
     got = m.attention(pool, q, step.table, step.q_start, step.kv_len, max_rows=1 << 33, max_keys=1 << 33)
     want = m.attention(pool, q, step.table, step.q_start, step.kv_len, max_rows=2, max_keys=2)
     assert torch.equal(got[:1], want[:1])
+
+
+def test_two_graphs_share_a_workspace_and_two_streams_run_side_by_side():
+    m, rng = kv4(), np.random.default_rng(13)
+    calls = []
+    for dim, heads, kv, page, lens, rows in ((256, 8, 2, 32, [1700, 300], [40, 30]), (128, 8, 2, 64, rng.integers(1, 900, 90).tolist(), [1] * 90)):
+        pool, _, table, _ = filled(rng, lens, page, kv, dim)
+        start = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        q = gpu(rng.normal(size=(int(start[-1]), heads, dim)), torch.float16)
+        calls.append((pool, q, gpu(table), gpu(start), gpu(np.array(lens, np.int32)), max(rows), max(lens)))
+    want = [m.attention(*c) for c in calls]
+    need = [m.attention_workspace(c[0], c[1].shape[0], c[1].shape[1], c[2].shape[0], c[2].shape[1], c[5], c[6]) for c in calls]
+    shared = torch.zeros(max(need), dtype=torch.uint8, device="cuda")
+    graphs, outs = [], [torch.empty_like(w) for w in want]
+    torch.cuda.synchronize()
+    for c, o in zip(calls, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            m.attention(*c, out=o, workspace=shared)
+        graphs.append(g)
+    for i in range(4):
+        for o in outs:
+            o.zero_()
+        shared.fill_(255)
+        for g in graphs[::1 if i % 2 else -1]:
+            g.replay()
+        got = m.attention(*calls[i % 2], workspace=shared)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)) and torch.equal(got, want[i % 2])
+    with pytest.raises(Exception, match="sl_kv4_attention"):
+        m.attention(*calls[0], workspace=shared[:need[0] - 16])
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(5):
+        for s, c, o in zip(streams, calls, got):
+            with torch.cuda.stream(s):
+                o.append(m.attention(*c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for o, w in zip(got, want) for x in o)
