@@ -32,21 +32,18 @@ SL_DEV int value_codes_at(int off, int d) { return (((off >> 3) * 16 + d / (D / 
 
 // ---- element types ------------------------------------------------------------------------------------------------------
 SL_DEV float bf2f(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-SL_DEV uint16_t f2bf(float x) {                       // to nearest, ties to even
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0x7fc0;
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+SL_DEV uint16_t f2bf(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }      // to nearest, ties to even: one instruction here
 template <bool BF>
 SL_DEV float elem_f(uint16_t u) { return BF ? bf2f(u) : h2f(u); }
 template <bool BF>
 SL_DEV uint16_t f_elem(float x) { return BF ? f2bf(x) : f2h(x); }
 template <bool BF>
-SL_DEV void load4(const uint16_t* p, float* x) {
-  const uint2 r = *reinterpret_cast<const uint2*>(p);
+SL_DEV void elems4(uint2 r, float* x) {
   x[0] = elem_f<BF>((uint16_t)r.x); x[1] = elem_f<BF>((uint16_t)(r.x >> 16));
   x[2] = elem_f<BF>((uint16_t)r.y); x[3] = elem_f<BF>((uint16_t)(r.y >> 16));
 }
+template <bool BF>
+SL_DEV void load4(const uint16_t* p, float* x) { elems4<BF>(*reinterpret_cast<const uint2*>(p), x); }
 
 // ---- page tables, slots and row offsets -----------------------------------------------------------------------------------
 constexpr int PLAN_MAX_REQ = 4096;
@@ -363,9 +360,10 @@ SL_DEV uint32_t quantise4(const F* v, uint32_t& sb) {
 // of value heads; the token's weights and angles are loaded once for a run.
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void k_kv4_append(Pool pool, sl_kv4_append_args a, int q_units, int kv_units, int per) {
-  constexpr int LANES = D / 4, HEADS = 64 / LANES;
+  constexpr int LANES = D / 4, HEADS = 64 / LANES, AHEAD = 4;
   const int lane = threadIdx.x & 63, l = lane % LANES, sub = lane / LANES;
-  const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // neighbouring tokens on one XCD (workgroups go round the eight): their value codes lie in one line, in turns of D / 32 bytes
+  const int block = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), t = block * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= a.n_tokens) return;
   const int q_runs = (q_units + per - 1) / per, kv_runs = (kv_units + per - 1) / per;
   const int pos = a.rot_dim ? a.pos[t] : 0, half = a.rot_dim / 2;
@@ -376,15 +374,25 @@ __global__ __launch_bounds__(256) void k_kv4_append(Pool pool, sl_kv4_append_arg
     const uint16_t* src = (const uint16_t*)a.q + t * a.q_token + 4 * l;
     uint16_t* dst = (uint16_t*)a.q_out + t * a.out_token + 4 * l;
     const Turn turn = turn_of<D, BF>((const uint16_t*)a.q_weight, a.cos, a.sin, placed ? half : 0, pos, l);
-    for (int u = run * per; u < u1; ++u) {
-      const int h = u * HEADS + sub;
-      const bool there = h < a.n_heads;               // (lanes without a head still take part in the exchanges)
-      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (there && placed) load4<BF>(src + h * a.q_head, x);
-      if (placed) turn_row<float, D>(x, turn, half, a.eps);
-      if (there)
-        *reinterpret_cast<uint2*>(dst + h * a.out_head) =
-            make_uint2((uint32_t)f_elem<BF>(x[0]) | ((uint32_t)f_elem<BF>(x[1]) << 16), (uint32_t)f_elem<BF>(x[2]) | ((uint32_t)f_elem<BF>(x[3]) << 16));
+    for (int u0 = run * per; u0 < u1; u0 += AHEAD) {
+      uint2 raw[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int h = (u0 + j) * HEADS + sub;
+        raw[j] = make_uint2(0, 0);
+        if (u0 + j < u1 && h < a.n_heads && placed) raw[j] = *reinterpret_cast<const uint2*>(src + h * a.q_head);
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (u0 + j >= u1) break;
+        const int h = (u0 + j) * HEADS + sub;           // (lanes without a head still take part in the exchanges)
+        float x[4];
+        elems4<BF>(raw[j], x);
+        if (placed) turn_row<float, D>(x, turn, half, a.eps);
+        if (h < a.n_heads)
+          *reinterpret_cast<uint2*>(dst + h * a.out_head) =
+              make_uint2((uint32_t)f_elem<BF>(x[0]) | ((uint32_t)f_elem<BF>(x[1]) << 16), (uint32_t)f_elem<BF>(x[2]) | ((uint32_t)f_elem<BF>(x[3]) << 16));
+      }
     }
     return;
   }
@@ -401,21 +409,31 @@ __global__ __launch_bounds__(256) void k_kv4_append(Pool pool, sl_kv4_append_arg
   const int64_t stride = key ? a.k_head : a.v_head;
   Turn turn;
   if (key) turn = turn_of<D, BF>((const uint16_t*)a.k_weight, a.cos, a.sin, half, pos, l);
-  for (int u = run * per; u < u1; ++u) {
-    const int h = u * HEADS + sub;
-    const bool there = h < pool.n_kv;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (there) load4<BF>(src + h * stride, x);
-    uint32_t sb, codes;
-    if (key) {
-      double y[4] = {x[0], x[1], x[2], x[3]};
-      turn_row<double, D>(y, turn, half, a.eps);
-      codes = quantise4(y, sb);
-    } else codes = quantise4(x, sb);
-    if (!there) continue;
-    unsigned char* at = page + h * head_bytes<D>(pool);
-    *reinterpret_cast<uint16_t*>(at + codes_at) = (uint16_t)codes;
-    if (l % 16 == 0) reinterpret_cast<uint32_t*>(at + part)[off * (D / 64) + l / 16] = sb;
+  for (int u0 = run * per; u0 < u1; u0 += AHEAD) {
+    uint2 raw[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int h = (u0 + j) * HEADS + sub;
+      raw[j] = make_uint2(0, 0);
+      if (u0 + j < u1 && h < pool.n_kv) raw[j] = *reinterpret_cast<const uint2*>(src + h * stride);
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (u0 + j >= u1) break;
+      const int h = (u0 + j) * HEADS + sub;
+      float x[4];
+      elems4<BF>(raw[j], x);
+      uint32_t sb, codes;
+      if (key) {
+        double y[4] = {x[0], x[1], x[2], x[3]};
+        turn_row<double, D>(y, turn, half, a.eps);
+        codes = quantise4(y, sb);
+      } else codes = quantise4(x, sb);
+      if (h >= pool.n_kv) continue;
+      unsigned char* at = page + h * head_bytes<D>(pool);
+      *reinterpret_cast<uint16_t*>(at + codes_at) = (uint16_t)codes;
+      if (l % 16 == 0) reinterpret_cast<uint32_t*>(at + part)[off * (D / 64) + l / 16] = sb;
+    }
   }
 }
 
@@ -1544,15 +1562,16 @@ int sl_kv4_append(const sl_kv4_pool* p, const sl_kv4_append_args* a, void* strea
   const int64_t strides[] = {a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->out_token, a->out_head};
   for (int i = a->q ? 0 : 2; i < (a->q ? 8 : 6); ++i) if (strides[i] % 4) return SL_ERR_ARG;
   if (a->rot_dim && (!aligned(a->cos, 16) || !aligned(a->sin, 16))) return SL_ERR_ARG;
-  if (a->n_heads > 32768 || a->n_tokens > 4 * MAX_GROUPS) return SL_ERR_TOO_LARGE;
+  if (a->n_heads > 32768 || a->n_tokens > 4 * (MAX_GROUPS - 8)) return SL_ERR_TOO_LARGE;
   const int heads = 256 / p->head_dim, q_units = a->q ? (a->n_heads + heads - 1) / heads : 0;
   const int kv_units = (p->n_kv + heads - 1) / heads;
-  // enough waves to fill the chip come first, then longer runs of heads (8192 waves: eight per SIMD)
+  // enough waves to fill the chip come first, then longer runs of heads (2048 tokens of 16 + 2 heads with their read-back: 22.3 us
+  // with runs from 16384 waves on, 20.8 from 4096 on; 7.6K tokens of 32 + 8 heads: runs of 1, 2, 4, 8, 16 units 110, 86, 77, 73, 73)
   const int64_t waves = (int64_t)a->n_tokens * (q_units + 2 * kv_units);
-  const int per = (int)std::max<int64_t>(1, std::min<int64_t>(8, waves / 8192));
+  const int per = (int)std::max<int64_t>(1, std::min<int64_t>(8, waves / 2048));
   const int runs = (q_units + per - 1) / per + 2 * ((kv_units + per - 1) / per);
   (void)hipGetLastError();
-#define KV4_CALL(D, BF) hipLaunchKernelGGL((k_kv4_append<D, BF>), dim3((a->n_tokens + 3) / 4, runs), dim3(256), 0, (hipStream_t)stream, pool, *a, q_units, kv_units, per)
+#define KV4_CALL(D, BF) hipLaunchKernelGGL((k_kv4_append<D, BF>), dim3((a->n_tokens + 31) / 32 * 8, runs), dim3(256), 0, (hipStream_t)stream, pool, *a, q_units, kv_units, per)
   KV4_BY_LAYOUT(p->head_dim, a->dtype == SL_BF16, KV4_CALL);
 #undef KV4_CALL
   return launch_status();
