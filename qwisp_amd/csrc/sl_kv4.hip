@@ -508,6 +508,7 @@ constexpr int AT_MAX_REQ = 4096;
 // behind the last part leave at once, as do those whose rows see fewer keys than the request has.
 struct AttnCut {
   int want;           // workgroups to share the cost out to
+  int turns;          // how often the share may grow until there are no more than that
   int rows;           // rows of a partial sum
   int32_t* first;     // [n_req + 1] parts before each request, then share (written by the first workgroup, for the merge)
   float* part;        // partial sums by workgroup: [grid][rows][D], then maxima [grid][rows], sums [grid][rows]
@@ -531,19 +532,19 @@ SL_DEV int parts_of(int rounds, int cost, int share) { return (int)(((unsigned)r
 // cost of a part: total / want, rounded up (a quotient of doubles is exact where it is whole)
 SL_DEV int share_of(long total, int want) { return max(1, (int)fmin(ceil((double)total / (double)want), 2147483647.0)); }
 struct AttnPart { int r, tile, h, part, share; };
-// What a request asks for: its items, its most rounds, their cost, and the sum of its items' costs (row tiles further up see
+// What a request asks for: its items, its most and least rounds, their cost, and the sum of its items' costs (row tiles further up see
 // fewer keys: their rounds lie evenly between the first tile's and the last's).
 template <int TILE>
-SL_DEV void request_work(const sl_kv4_attn_args& a, const Pool& pool, int r, int& items, int& rounds, int& cost, long& all) {
+SL_DEV void request_work(const sl_kv4_attn_args& a, const Pool& pool, int r, int& items, int& rounds, int& least, int& cost, long& all) {
   int start, n;
   const int rows = rows_of(a, r, start, n), group = a.n_heads / pool.n_kv;
-  items = rounds = 0; cost = 1; all = 0;
+  items = rounds = least = 0; cost = 1; all = 0;
   if (rows <= 0) return;
   const int tiles = (rows * group + TILE - 1) / TILE;
   const long keys = seen_keys(a, pool, r);
   items = tiles * pool.n_kv; rounds = rounds_for(min(keys, keys - n + rows)); cost = round_cost(TILE, rows * group);
-  const int least = rounds_for(keys - n + min(rows, TILE / group + 1));
-  all = (long)items * (rounds + (tiles > 1 ? least : rounds)) * cost / 2;
+  least = tiles > 1 ? rounds_for(keys - n + min(rows, TILE / group + 1)) : rounds;
+  all = (long)items * (rounds + least) * cost / 2;
 }
 // Rounds of a row tile and how they are cut: `parts` of `per` rounds (at most parts_of() of the request's most rounds).
 template <int TILE>
@@ -559,18 +560,29 @@ SL_DEV void tile_cut(long keys, int n, int rows_total, int tile, int group, int 
 template <int TILE>
 SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut& cut, int idx, int* s_first, int* s_tmp, AttnPart& out) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.n_req;
-  int before, items, rounds, cost, share;
+  int before, items, rounds, least, cost, share;
   long all;
+  // Rounding up makes more parts than were asked for, and a few more than the chip has places cost another turn: while the items
+  // alone are fewer, the share grows until their parts are too (row tiles further up have parts for fewer keys).
+  auto used = [&] { return items * (parts_of(rounds, cost, share) + parts_of(least, cost, share)); };       // twice the parts
+  auto too_many = [&](int twice, int items_now, int it) { return it < cut.turns && twice / 2 > cut.want && items_now < cut.want; };
+  auto grown = [&](int twice) { return (int)fmin(ceil((double)share * (double)twice / (2.0 * (double)cut.want)), 2147483647.0); };
   if (n <= 64) {
-    items = rounds = 0; cost = 1; all = 0;
-    if (lane < n) request_work<TILE>(a, pool, lane, items, rounds, cost, all);
+    items = rounds = least = 0; cost = 1; all = 0;
+    if (lane < n) request_work<TILE>(a, pool, lane, items, rounds, least, cost, all);
+    int all_items = items;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+    for (int d = 1; d < 64; d <<= 1) { all += __shfl_xor(all, d); all_items += __shfl_xor(all_items, d); }
     share = share_of(all, cut.want);
-    const int parts = parts_of(rounds, cost, share), own = items * parts;
-    int upto = own;
+    int parts, own, upto;
+    for (int it = 0;; ++it) {
+      parts = parts_of(rounds, cost, share); own = upto = items * parts;
+      int twice = used();
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; }
+      for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; twice += __shfl_xor(twice, d); }
+      if (!too_many(twice, all_items, it)) break;
+      share = grown(twice);
+    }
     if (idx == 0 && wave == 0) {
       if (lane < n) cut.first[lane] = upto - own;
       if (lane == 63) { cut.first[n] = upto; cut.first[n + 1] = share; }
@@ -579,36 +591,45 @@ SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut
     if (r >= n) return false;                      // (lanes behind n hold the total as well)
     out.r = r;
     before = __builtin_amdgcn_readlane(upto - own, r); rounds = __builtin_amdgcn_readlane(parts, r); items = __builtin_amdgcn_readlane(items, r);
+    share = __builtin_amdgcn_readfirstlane(share);
   } else {
     const int per = (n + 255) / 256;
     long total = 0;
+    int all_items = 0;
     for (int j = 0; j < per; ++j) {
       const int r = tid * per + j;
-      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, cost, all); total += all; }
+      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, least, cost, all); total += all; all_items += items; }
     }
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d);
+    for (int d = 1; d < 64; d <<= 1) { total += __shfl_xor(total, d); all_items += __shfl_xor(all_items, d); }
     long* s_total = reinterpret_cast<long*>(s_tmp);
-    if (lane == 0) s_total[wave] = total;
+    if (lane == 0) { s_total[wave] = total; s_tmp[8 + wave] = all_items; }
     __syncthreads();
     total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
+    all_items = (s_tmp[8] + s_tmp[9]) + (s_tmp[10] + s_tmp[11]);
     share = share_of(total, cut.want);
-    int own = 0;
-    for (int j = 0; j < per; ++j) {
-      const int r = tid * per + j;
-      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, cost, all); own += items * parts_of(rounds, cost, share); }
+    int at, sum;
+    for (int it = 0;; ++it) {
+      int own = 0, twice = 0;
+      for (int j = 0; j < per; ++j) {
+        const int r = tid * per + j;
+        if (r < n) { request_work<TILE>(a, pool, r, items, rounds, least, cost, all); own += items * parts_of(rounds, cost, share); twice += used(); }
+      }
+      int upto = own;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; twice += __shfl_xor(twice, d); }
+      __syncthreads();
+      if (lane == 63) { s_tmp[wave] = twice; s_tmp[8 + wave] = upto; }
+      __syncthreads();
+      at = upto - own; sum = 0; twice = 0;
+#pragma unroll
+      for (int w = 0; w < AT_WAVES; ++w) { if (w < wave) at += s_tmp[8 + w]; sum += s_tmp[8 + w]; twice += s_tmp[w]; }
+      if (!too_many(twice, all_items, it)) break;
+      share = grown(twice);
     }
-    int upto = own;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; }
-    if (lane == 63) s_tmp[8 + wave] = upto;
-    __syncthreads();
-    int at = upto - own, sum = 0;
-#pragma unroll
-    for (int w = 0; w < AT_WAVES; ++w) { if (w < wave) at += s_tmp[8 + w]; sum += s_tmp[8 + w]; }
     for (int j = 0; j < per; ++j) {
       const int r = tid * per + j;
-      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, cost, all); s_first[r] = at; at += items * parts_of(rounds, cost, share); }
+      if (r < n) { request_work<TILE>(a, pool, r, items, rounds, least, cost, all); s_first[r] = at; at += items * parts_of(rounds, cost, share); }
     }
     if (tid == 0) s_first[n] = sum;
     __syncthreads();
@@ -616,7 +637,7 @@ SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut
     if (idx >= sum) return false;
     out.r = __builtin_amdgcn_readfirstlane(owner_of(s_first, n, idx));
     before = s_first[out.r];
-    request_work<TILE>(a, pool, out.r, items, rounds, cost, all);
+    request_work<TILE>(a, pool, out.r, items, rounds, least, cost, all);
     rounds = parts_of(rounds, cost, share);
   }
   // (rounds: from here on the most parts of an item.)  Workgroups go round the eight XCDs in turn: eight items side by side, part
@@ -1008,11 +1029,11 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
   {
     const int r = at.r, h = at.h;
     int start, n;
-    const int rows = rows_of(a, r, start, n), row0 = at.tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);
+    const int rows = rows_of(a, r, start, n), tile = NT > 1 ? (rows * group + 16 * NT - 1) / (16 * NT) - 1 - at.tile : at.tile, row0 = tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);
     const long keys = seen_keys(a, pool, r);
     long last;
     int parts, per;
-    tile_cut<16 * NT>(keys, n, rows * group, at.tile, group, at.share, last, parts, per);
+    tile_cut<16 * NT>(keys, n, rows * group, tile, group, at.share, last, parts, per);
     if (at.part >= parts) return;
     const long slot = parts > 1 ? (long)blockIdx.x : -1;
     const int key0 = at.part * per * AT_UNIT, key1 = (int)min((long)(at.part + 1) * per * AT_UNIT, last);
@@ -1369,7 +1390,7 @@ __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_a
   if (count == 1) return;                               // one workgroup had all of it and wrote the rows
   const int most = parts_of(rounds_for(min(keys, keys - n + rows)), round_cost(TILE, rows * group), share);      // parts that each item is numbered with
   // as find_part numbers them: part i of the item stands at first + i * side
-  const int items = tiles * pool.n_kv, item = (TILE == 64 ? tiles - 1 - tile : tile) * pool.n_kv + h, full = items & ~7, side = item < full ? 8 : items - full;
+  const int items = tiles * pool.n_kv, item = (TILE > 16 ? tiles - 1 - tile : tile) * pool.n_kv + h, full = items & ~7, side = item < full ? 8 : items - full;
   const long first = cut.first[r] + (item < full ? (long)(item & ~7) * most + (item & 7) : (long)full * most + (item - full));
   if (cut.first[r] + (long)items * most > cut.slots) return;      // (row offsets that overlap: more parts than rows allow)
   const float* stat = cut.part + cut.slots * cut.rows * D;
@@ -1477,10 +1498,22 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   const int64_t resident = (int64_t)compute_units() * (tile == 64 ? 2 : attn_places(p->head_dim, tile / 16));
   const int64_t rounds = items * (std::min<int64_t>(widest, a->max_keys) / AT_UNIT + 1);
   if (p->n_kv * a->n_req * ((rows + tile - 1) / tile) + 4 * resident > MAX_GROUPS) return SL_ERR_TOO_LARGE;
-  // 16 and 32 rows: parts are equally long, so with few items they and the parts together fill the chip once; with more, parts of half
-  // a turn.  64 rows: row tiles see different numbers of keys, the longest first, and the chip takes parts as it gets free; tiles that
-  // fill it by themselves are cut where they are twice the mean (2048 rows of a prompt 147 us, cut at the mean 168).
-  sh.cut.want = (int)std::min(tile == 64 ? (items >= resident ? resident / 2 : resident) : (items <= resident / 2 ? resident - items : 2 * resident), std::max<int64_t>(rounds, 1));
+  // How many parts.  Up to three quarters of the chip's places in items: as many parts as places, no more (128 lanes of 256 dims 83 us,
+  // two turns of parts 91, unchecked 102; 40 verify requests 63, 69, 72).  More items: single tokens are cut for two
+  // turns, from one and a half turns of items on for one (200 lanes 121 and 133, 500 lanes 224 and 210).  Row tiles of a prompt that
+  // begins here see from nothing to all of it: the longest first and uncut, the chip takes them as it gets free (2048 rows of
+  // 256 dims 140 us, parts of the mean 160; of 64 dims 34 and 46), unless there are fewer than two thirds of the places (1024 rows
+  // 84 and 67).  Chunks behind a long context are alike: uncut where whole turns of items fill the chip to 85 % (2048 rows behind
+  // 4096 390 us, cut for three turns 434), else cut (2333 rows in three requests 1520 and 975; of 64 dims 243, for two turns 184,
+  // for three 193).
+  const int64_t whole = (items + resident - 1) / resident;
+  const bool alike = a->max_keys > 2ll * a->max_rows;
+  int64_t want = resident;
+  if (tile != 16 && !alike && 3 * items >= 2 * resident) want = items / 2;
+  else if (4 * items <= 3 * resident) sh.cut.turns = 4;
+  else if (tile == 16) { want = 2 * items <= 3 * resident ? 2 * resident : resident; sh.cut.turns = 4; }
+  else want = items * 20 >= whole * resident * 17 ? items / 2 : (tile == 64 ? 3 : 2) * resident;
+  sh.cut.want = (int)std::min(want, std::max<int64_t>(rounds, 1));
   // a request's items are numbered with the parts of its longest row tile: at most twice the mean of longest and shortest
   sh.grid = (int)(2 * sh.cut.want + items);
   // Joining: a workgroup per row while there are few rows or many parts to each, else a wave per row (2333 rows of 64 dims on 16K keys
