@@ -85,7 +85,9 @@ SL_DEV int owner_of(const int* first, int n, int x) {
 
 // Every workgroup forms the running sums over the requests (rows; pages missing and pages given back) for itself, in LDS, and then
 // fills its share of the outputs: one launch, no exchange between workgroups.  The requests' numbers are 12 bytes each and
-// come from L2; up to 64 requests are one wave's work, without a barrier.
+// come from L2; up to 64 requests are one wave's work, without a barrier.  A few KB: bound by the launch and three dependent trips to
+// memory (32 requests 4.5 us), with many requests by the sums that every workgroup repeats (1024 requests of up to 32K
+// tokens 13 us, of which the table's rows take 4).
 __global__ __launch_bounds__(PLAN_THREADS) void k_kv4_plan(sl_kv4_plan_args a, int page_shift) {
   __shared__ int s_row[PLAN_MAX_REQ + 1], s_need[PLAN_MAX_REQ + 1], s_give[PLAN_MAX_REQ + 1];
   __shared__ unsigned s_wave[PLAN_THREADS / 64];
@@ -357,7 +359,9 @@ SL_DEV uint32_t quantise4(const F* v, uint32_t& sb) {
 }
 
 // A wave per token and `per` times 256/D heads: D/4 lanes carry a head row.  blockIdx.y: runs of query heads, then of key heads, then
-// of value heads; the token's weights and angles are loaded once for a run.
+// of value heads; the token's weights and angles are loaded once for a run, the rows of four units ahead of their use.  Bound by the
+// issue of vector instructions: 7.6K tokens of 32 + 8 heads of 128 dims 51 us (3400 instructions a token, half of them for the
+// 16 rows that are quantised; 187 MB in and out at 3.6 TB/s), 2048 tokens of 16 + 2 heads of 256 dims 13 us, one token 3.6.
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void k_kv4_append(Pool pool, sl_kv4_append_args a, int q_units, int kv_units, int per) {
   constexpr int LANES = D / 4, HEADS = 64 / LANES, AHEAD = 4;
@@ -439,6 +443,7 @@ __global__ __launch_bounds__(256) void k_kv4_append(Pool pool, sl_kv4_append_arg
 
 // ---- rows as values -----------------------------------------------------------------------------------------------------
 // A lane takes four dims of a key row and of a value row; a workgroup 4096 / D rows of one head, four loads of each kind in flight.
+// Bound by memory: 39K rows of 8 heads of 128 dims to fp32 78 us, 4.75 TB/s (one load in flight: 110); 500 rows of 2 heads 3.5 us.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void k_kv4_read(Pool pool, const int32_t* slots, int n, void* k_out, void* v_out) {
   constexpr int LANES = D / 4, ROWS = 256 / LANES, TURNS = 4;
@@ -1004,6 +1009,10 @@ SL_DEV void put_row(const sl_kv4_attn_args& a, const AttnCut& cut, long slot, in
   }
 }
 
+// Up to 16 (NT = 1) or 32 rows a workgroup.  What bounds it: one token at 4K 9.5 us, start and end (lengths, table, page, queries, the
+// join in LDS) with one round of keys between; 32 lanes at 1K-16K 33 us, the same 9 us and 107 MB at 4.5 TB/s; six requests
+// of 3-5 rows at 20-32K, 128 dims, 49 us, 187 MB, vector instructions in 67 % of the slots; 2333 rows behind 4-16K, 64 dims,
+// 189 us, 92 % of the slots (unpacking 1/2, softmax and weights 1/2; the matrix cores are busy 21 %).
 // Workgroups on a compute unit: by the registers, of which the running sums alone take NT * D / 4.
 constexpr int attn_places(int dim, int nt) { return dim == 64 ? (nt == 1 ? 4 : 3) : (dim == 128 && nt == 1 ? 3 : 2); }
 template <int D, bool BF, int NT>
@@ -1196,6 +1205,8 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
 // waves a SIMD).  The waves lay a step's bytes out in LDS together, a step ahead of its use, so the registers hold no bytes but
 // those on their way.  (With fewer dims a wave has room for 32 rows, and waves that unpack their own keys are faster than
 // ones that meet at a barrier every step: 64 rows of 128 dims against 32K keys 121 us, with this kernel's scheme 190.)
+// A prompt of 2048 rows and 16 heads 141 us, 245 TFLOP/s: 512 workgroups, two to a unit, and the last row tile's 64 steps of 2.2 us
+// are its length; 512 rows behind 8K 176 us, 400 TFLOP/s.
 template <int D>
 struct TileLds {
   static constexpr int KEYS = 16 * D;                                  // key words in the order of the lanes
@@ -1371,7 +1382,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
 }
 
 // Partial sums joined.  WIDE: a workgroup per row; its waves read 256 / D partial rows at once, 16 bytes a lane, four such loads
-// in flight, and meet in LDS.  Otherwise a wave per row, 16 rows a workgroup.
+// in flight, and meet in LDS.  Otherwise a wave per row, 16 rows a workgroup.  A launch and three dependent trips: 4-5.5 us.
 template <int D, bool BF, int TILE, bool WIDE>
 __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_args a, AttnCut cut) {
   constexpr int LANES = D / 4, PER_WAVE = 64 / LANES, WAVES = WIDE ? 4 : 1, PER = WAVES * PER_WAVE;
