@@ -570,24 +570,25 @@ SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut
   // Rounding up makes more parts than were asked for, and a few more than the chip has places cost another turn: while the items
   // alone are fewer, the share grows until their parts are too (row tiles further up have parts for fewer keys).
   auto used = [&] { return items * (parts_of(rounds, cost, share) + parts_of(least, cost, share)); };       // twice the parts
-  auto too_many = [&](int twice, int items_now, int it) { return it < cut.turns && twice / 2 > cut.want && items_now < cut.want; };
+  auto too_many = [&](int twice, int items_now) { return twice / 2 > cut.want && items_now < cut.want; };
   auto grown = [&](int twice) { return (int)fmin(ceil((double)share * (double)twice / (2.0 * (double)cut.want)), 2147483647.0); };
   if (n <= 64) {
     items = rounds = least = 0; cost = 1; all = 0;
     if (lane < n) request_work<TILE>(a, pool, lane, items, rounds, least, cost, all);
-    int all_items = items;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { all += __shfl_xor(all, d); all_items += __shfl_xor(all_items, d); }
+    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
     share = share_of(all, cut.want);
-    int parts, own, upto;
-    for (int it = 0;; ++it) {
-      parts = parts_of(rounds, cost, share); own = upto = items * parts;
-      int twice = used();
+    for (int it = 0; it < cut.turns; ++it) {
+      int twice = used(), all_items = items;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; twice += __shfl_xor(twice, d); }
-      if (!too_many(twice, all_items, it)) break;
+      for (int d = 1; d < 64; d <<= 1) { twice += __shfl_xor(twice, d); all_items += __shfl_xor(all_items, d); }
+      if (!too_many(twice, all_items)) break;
       share = grown(twice);
     }
+    const int parts = parts_of(rounds, cost, share), own = items * parts;
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const int y = __shfl_up(upto, d); if (lane >= d) upto += y; }
     if (idx == 0 && wave == 0) {
       if (lane < n) cut.first[lane] = upto - own;
       if (lane == 63) { cut.first[n] = upto; cut.first[n + 1] = share; }
@@ -629,7 +630,7 @@ SL_DEV bool find_part(const sl_kv4_attn_args& a, const Pool& pool, const AttnCut
       at = upto - own; sum = 0; twice = 0;
 #pragma unroll
       for (int w = 0; w < AT_WAVES; ++w) { if (w < wave) at += s_tmp[8 + w]; sum += s_tmp[8 + w]; twice += s_tmp[w]; }
-      if (!too_many(twice, all_items, it)) break;
+      if (it >= cut.turns || !too_many(twice, all_items)) break;
       share = grown(twice);
     }
     for (int j = 0; j < per; ++j) {
@@ -1038,7 +1039,7 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
   {
     const int r = at.r, h = at.h;
     int start, n;
-    const int rows = rows_of(a, r, start, n), tile = NT > 1 ? (rows * group + 16 * NT - 1) / (16 * NT) - 1 - at.tile : at.tile, row0 = tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);
+    const int rows = rows_of(a, r, start, n), tile = NT > 1 ? (rows * group + 16 * NT - 1) / (16 * NT) - 1 - at.tile : at.tile, row0 = tile * 16 * NT, rows_here = min(16 * NT, rows * group - row0);      // (the tiles that see most keys first)
     const long keys = seen_keys(a, pool, r);
     long last;
     int parts, per;
@@ -1515,7 +1516,7 @@ int attn_shape(const sl_kv4_pool* p, const sl_kv4_attn_args* a, AttnShape& sh) {
   // begins here see from nothing to all of it: the longest first and uncut, the chip takes them as it gets free (2048 rows of
   // 256 dims 140 us, parts of the mean 160; of 64 dims 34 and 46), unless there are fewer than two thirds of the places (1024 rows
   // 84 and 67).  Chunks behind a long context are alike: uncut where whole turns of items fill the chip to 85 % (2048 rows behind
-  // 4096 390 us, cut for three turns 434), else cut (2333 rows in three requests 1520 and 975; of 64 dims 243, for two turns 184,
+  // 4096 390 us, cut for three turns 434), else cut (2333 rows in three requests 1520 and 975; of 64 dims 243, for two turns 189,
   // for three 193).
   const int64_t whole = (items + resident - 1) / resident;
   const bool alike = a->max_keys > 2ll * a->max_rows;
