@@ -1429,11 +1429,11 @@ __global__ __launch_bounds__(256) void k_kv4_attn_merge(Pool pool, sl_kv4_attn_a
         const long slot = first + (long)(in_range ? i + u * PER : i) * side;
         p[u] = *reinterpret_cast<const float4*>(cut.part + (slot * cut.rows + in) * D + d);
         m[u] = in_range ? stat[slot * cut.rows + in] : -__builtin_inff();
-        l[u] = stat[(cut.slots + slot) * cut.rows + in];
+        l[u] = in_range ? stat[(cut.slots + slot) * cut.rows + in] : 0.0f;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        if (m[u] == -__builtin_inff()) continue;         // (a part in which the row sees no key)
+        if (m[u] == -__builtin_inff() && l[u] == 0.0f) continue;         // a part in which the row sees no key; one whose scores are all NaN has that sum
         const float f = __builtin_amdgcn_exp2f(m[u] - best);
         sum = fmaf(f, l[u], sum);
         y.x = fmaf(f, p[u].x, y.x); y.y = fmaf(f, p[u].y, y.y); y.z = fmaf(f, p[u].z, y.z); y.w = fmaf(f, p[u].w, y.w);

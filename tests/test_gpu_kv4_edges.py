@@ -1,0 +1,102 @@
+"""The 4-bit cache's attention where numbers are not finite: against the plain 64-bit form, with tolerances that follow the values'
+own size."""
+import numpy as np
+import pytest
+
+from . import kv4_ref as ref
+from .test_gpu_kv4 import DTYPES, HALF_STEP, f64, filled, gpu, kv4
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def call(pool, q, table, start, lens, scale=None):
+    """Attention into an output that holds 5."""
+    out = torch.full(tuple(q.shape), 5.0, dtype=q.dtype, device="cuda")
+    rows = np.diff(start)
+    return kv4().attention(pool, q, gpu(table), gpu(start), gpu(np.array(lens, np.int32)), max_rows=int(rows.max()), max_keys=max(lens), scale=scale, out=out)
+
+
+def offsets(rows):
+    return np.concatenate(([0], np.cumsum(rows))).astype(np.int32)
+
+
+# ---- numbers that are not finite, the axis in parts ------------------------------------------------------------------------
+# (dim, dtype, heads, kv, page, lengths, rows): a few rows (parts joined by a workgroup each), 32-row tiles, 64-row tiles, and parts of
+# many requests (joined by a wave each)
+SPLIT = [(64, "f16", 4, 2, 32, [3000, 200], [1, 1]), (128, "bf16", 6, 2, 16, [2900, 70], [3, 2]), (256, "f16", 4, 2, 64, [4000], [1]),
+         (128, "f16", 4, 2, 16, [2500, 77], [40, 20]), (256, "bf16", 4, 1, 32, [2600, 40, 900], [30, 25, 17]),
+         (256, "f16", 8, 2, 64, [1000, 60, 1003] + [7] * 67, [12, 1, 12] + [1] * 67), (128, "bf16", 8, 2, 64, [1000, 60, 1003] + [7] * 67, [15, 1, 12] + [1] * 67)]
+
+
+@pytest.mark.parametrize("dim, dtype, heads, kv, page, lens, rows", SPLIT)
+@pytest.mark.parametrize("what", ["query", "keys"])
+def test_what_is_not_finite_shows_however_the_axis_is_cut(dim, dtype, heads, kv, page, lens, rows, what):
+    rng = np.random.default_rng(40)
+    pool, parts, table, n_pages = filled(rng, lens, page, kv, dim)
+    start = offsets(rows)
+    q = gpu(rng.normal(size=(int(start[-1]), heads, dim)), DTYPES[dtype])
+    if what == "query":                                      # NaN in one row, Inf in others, of different heads
+        q[0, 0, 5], q[-1, heads - 1, dim - 1], q[rows[0] - 1, heads // 2, 0] = float("nan"), float("-inf"), float("inf")
+    else:                                                    # whole parts of the first request, up to the last key that all its rows see
+        first, name = lens[0] * 3 // 5 // 128 * 128, what[0]
+        j = np.arange(first, lens[0] - rows[0] + 1)
+        at = table[0, j // page] * page + j % page
+        parts[name]["scale"][at, 0], parts[name]["bias"][at, 0] = np.nan, np.nan
+        if len(lens) > 1:                                    # and the second's very last key, in its last group and head: seen by one row
+            last = lens[1] - 1
+            parts[name]["scale"][table[1, last // page] * page + last % page, kv - 1, -1] = np.nan
+        pool = kv4().Pool(gpu(ref.pack(parts["k"], parts["v"], page, kv, dim)), page, kv, dim)
+    have = f64(call(pool, q, table, start, lens))
+    with np.errstate(invalid="ignore"):
+        want, var, size = expected(f64(q), parts, table, start, lens, page, dim ** -0.5, HALF_STEP[dtype])
+    bad = np.isnan(want)
+    assert bad.any() and not bad.all() and np.array_equal(np.isnan(have), bad)
+    compare(have[~bad], want[~bad], var[~bad], size[~bad])
+
+
+# ---- small values, and keys that stand out ------------------------------------------------------------------------------------
+H = 2.0 ** -11          # half a step of fp16, in which weights meet the matrix instructions
+
+
+def expected(q, parts, table, start, lens, page, scale, eps_out):
+    """Rows in 64 bits; per number the variance that the roundings on the way leave; and the sum of its terms' sizes.
+    A weight p meets the values in two parts, (p s) (code - 8) and p (b + 8 s), and the normaliser: p s, p and b + 8 s are each
+    rounded to fp16 (an error of at most H of itself, spread evenly: variance H^2 / 3 at most), independently of each other."""
+    t, heads, dim = q.shape
+    wide = lambda x: np.repeat(x, 64, -1)  # noqa: E731
+    kv = parts["k"]["codes"].shape[1]
+    kk, vv = ref.values(parts["k"]), ref.values(parts["v"])
+    out, var, size = (np.zeros((t, heads, dim)) for _ in range(3))
+    for r, length in enumerate(lens):
+        rows = start[r + 1] - start[r]
+        j = np.arange(length)
+        at = table[r, j // page] * page + j % page
+        for g in range(kv):
+            k, v, s = kk[at, g], vv[at, g], wide(parts["v"]["scale"][at, g])
+            mid = wide(parts["v"]["bias"][at, g]) + 8 * s
+            hs = slice(g * (heads // kv), (g + 1) * (heads // kv))
+            for i in range(rows):
+                n = length - rows + i + 1
+                x = scale * (q[start[r] + i, hs] @ k[:n].T)
+                w = np.exp(x - x.max(-1, keepdims=True))
+                w /= w.sum(-1, keepdims=True)
+                o = w @ v[:n]
+                w2 = w * w
+                spread = w2 @ ((v[:n] - mid[:n]) ** 2 + 2 * mid[:n] ** 2) - 2 * o * (w2 @ mid[:n]) + o * o * w2.sum(-1, keepdims=True)
+                out[start[r] + i, hs] = o
+                var[start[r] + i, hs] = H * H / 3 * spread + (eps_out * o) ** 2 / 3
+                size[start[r] + i, hs] = w @ (np.abs(v[:n]) + 8 * np.abs(s[:n]))
+    return out, var, size
+
+
+def compare(have, want, var, size, fp32=2.0 ** -15, least=2.0 ** -25):
+    """The error as a whole within twice what the roundings leave at most (half a step is 0.7 of that for the average number, and the dims
+    of a row share the errors of p), each number within seven times, ten times its likely size.
+    fp32: a score is the difference of two sums over codes of up to 100 in units of log2, each of some rounded steps: within
+    2^-24 * 100 * 4, which is 2^-15, of the weight; below fp16's normal numbers an output is within 2^-25."""
+    err = np.abs(have - want)
+    rms = lambda x: np.sqrt((x * x).mean())  # noqa: E731
+    assert rms(err) <= 2 * np.sqrt(var.mean()) + fp32 * rms(size) + least, (rms(err), np.sqrt(var.mean()), rms(size))
+    worst = err / (7 * np.sqrt(var) + 4 * fp32 * size + 2 * least)
+    assert worst.max() <= 1, worst.max()
