@@ -709,11 +709,17 @@ struct StepLds {
   template <int D>
   static constexpr int bytes() { return (D / 64) * (V_STRIDE + 4 * AT_STEP * 2); }
 };
-// Scales and biases (lanes 0..31: key `lane`, lanes 32..63: value of key lane - 32) into LDS; a key that is not there gets
-// zeros.  Value lanes turn b into b + 8 s; one that is not finite is left to the scale as NaN, which the weights carry only
-// where the key is seen.
+// The keys of a step whose values in a group are not finite.  They stay away from the matrix instructions, where a NaN would reach all
+// dims of a row (it meets the zeros of the operands beside its own) and rows that do not see the key.
 template <int D>
-SL_DEV void put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& st) {
+struct BadValues {
+  unsigned any = 0;
+  uint32_t keys[D / 64];                      // by group, where there are any
+};
+// Scales and biases (lanes 0..31: key `lane`, lanes 32..63: value of key lane - 32) into LDS; a key that is not there gets
+// zeros.  Value lanes turn b into b + 8 s; a group in which that is not finite gets zeros and is named in what comes back.
+template <int D>
+SL_DEV BadValues<D> put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& st) {
   constexpr int G = D / 64, W = (G + 1) / 2;
   const int lane = threadIdx.x & 63;
   uint32_t sc[W], bi[W];
@@ -731,12 +737,16 @@ SL_DEV void put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& 
     bi[g] = lane < 32 ? bi[g] : __builtin_bit_cast(uint32_t, b);
   }
   const _Float16 none = odd.x + odd.y;
-  if (__any(none != none && lane >= 32)) {
+  BadValues<D> out;
+  out.any = __any(none != none && lane >= 32);
+  if (out.any) {
 #pragma unroll
-    for (int g = 0; g < W; ++g)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (lane >= 32 && ((bi[g] >> (16 * u)) & 0x7c00u) == 0x7c00u) { bi[g] &= u ? 0x0000ffffu : 0xffff0000u; sc[g] = (sc[g] & (u ? 0x0000ffffu : 0xffff0000u)) | (0x7e00u << (16 * u)); }
+    for (int g = 0; g < G; ++g) {
+      const uint32_t half = 0xffffu << (16 * (g & 1)), top = 0x7c00u << (16 * (g & 1));
+      const bool bad = lane >= 32 && (bi[g / 2] & top) == top;
+      out.keys[g] = (uint32_t)(__ballot(bad) >> 32);
+      if (bad) { bi[g / 2] &= ~half; sc[g / 2] &= ~half; }
+    }
   }
   if constexpr (G == 4) {
     *reinterpret_cast<uint2*>(st.ks + lane * G) = make_uint2(sc[0], sc[1]);
@@ -752,6 +762,7 @@ SL_DEV void put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& 
 #pragma unroll
     for (int g = 0; g < G; ++g) st.vb[g * AT_STEP + (lane & 31)] = (uint16_t)(bi[g / 2] >> (16 * (g & 1)));
   }
+  return out;
 }
 // s[row tile][8]: this lane's keys 8 kg .. 8 kg + 7 against row n16.  All products of the step first, so that no scale waits for
 // the product before it.  `query(nt, i)`: the operand of dims word i; k: the two key operands' words.
@@ -813,11 +824,10 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
   for (int nt = 0; nt < LIVE; ++nt) {
     // only the step at the end of a row's keys, and one with a page that is not there, has keys to hide
     const bool hides = there != 0xffffffffu || __any(limit[nt] < k0 + AT_STEP);
-    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
     if (hides) {
 #pragma unroll
       for (int t = 0; t < 8; ++t)
-        if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) { s[nt][t] = -__builtin_inff(); keep[t / 2] &= t & 1 ? 0x0000ffffu : 0xffff0000u; }
+        if (!((there >> (8 * kg + t)) & 1u) || k0 + 8 * kg + t >= limit[nt]) s[nt][t] = -__builtin_inff();
     }
     float top = s[nt][0];
 #pragma unroll
@@ -844,12 +854,19 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int t = 0; t < 4; ++t) pw[nt][g][t] = pair_of(fmaf(p[2 * t], nth_half(vs, 2 * t * G + g), 0.0f), fmaf(p[2 * t + 1], nth_half(vs, (2 * t + 1) * G + g), 0.0f));   // (fma: takes the half as it is)
-    if (hides) {                 // a hidden key's scale may be NaN
+  }
+}
+// Rows that see a key whose values in a group are not finite: their sum over b + 8 s of that group becomes NaN, and all its dims with it.
+template <int D, int LIVE, int NT>
+SL_DEV void mark_bad(const BadValues<D>& bad, int k0, const int (&limit)[NT], f4 (&ob)[NT]) {
+  const int kg = (threadIdx.x & 63) >> 4;
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+  for (int nt = 0; nt < LIVE; ++nt) {
+    const int seen = min(max(limit[nt] - k0, 0), AT_STEP);
+    const uint32_t sees = seen == AT_STEP ? ~0u : (1u << seen) - 1u;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) pw[nt][g][t] &= keep[t];
-    }
+    for (int g = 0; g < D / 64; ++g)
+      if (kg == 0 && (bad.keys[g] & sees)) ob[nt][g] = __builtin_nanf("");       // (lanes of the first 16 hold rows 0..3 of ob)
   }
 }
 // Values: o[group][i] gathers (p s_g) c of the dims 4 m' + i, in units of 2^-24 (odd i: 2^-20, the nibble standing four bits up).
@@ -1132,7 +1149,7 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
         const bool more = k0 + AT_UNIT < key1;
         const unsigned there = (unsigned)__ballot(cur.there);
         wave_lds_order();
-        put_scales<D>(cur.sb, cur.there, st);
+        const BadValues<D> bad = put_scales<D>(cur.sb, cur.there, st);
         // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
 #pragma unroll
         for (int c = 0; c < G; ++c) {
@@ -1156,6 +1173,7 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
         uint32_t pw[LIVE][G + 1][4];
         step_weights<D, LIVE, NT>(s, there, k0, limit, mul, st, m, o, ob, pw);
         step_values<D, LIVE, NT>(pw, st, ones, o, ob);
+        if (bad.any) mark_bad<D, LIVE, NT>(bad, k0, limit, ob);
       }
     };
     if (NT == 1 || rows_here <= 16) keys_loop(std::integral_constant<int, 1>{});
@@ -1284,7 +1302,8 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
     }
   };
   auto step_lds = [&](int buf) { return lds + buf * L::STEP; };
-  unsigned* s_there = reinterpret_cast<unsigned*>(s_m);                // by buffer; free until the end
+  struct Note { unsigned there; BadValues<D> bad; };
+  Note* s_note = reinterpret_cast<Note*>(s_m);                         // by buffer: the keys that are there; free until the end
   // keys: [operand][half of the row's quarter][quarter][row of the operand]; values: pieces of 4 dims, two keys a word
   const int k_to = ((((key_token >> 2) & 1) * HALVES + key_part % HALVES) * 64 + key_part / HALVES * 16 + (key_token >> 3) * 4 + (key_token & 3)) * 4 * KW;
   const int v_to = v_m / (16 / G) * V_STRIDE + (v_blk * 16 + G * (v_m % (16 / G))) * 16 + v_sub * 4;
@@ -1296,9 +1315,12 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
     for (int c = 0; c < 4; ++c)            // two keys of 8 bytes: a word of four pieces
       *reinterpret_cast<uint32_t*>(st.v + v_to + 16 * c) = __builtin_amdgcn_perm(wv[2 + c / 2], wv[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
     if (wave == 0) {
-      put_scales<D>(sb, there, st);
+      const BadValues<D> bad = put_scales<D>(sb, there, st);
       const unsigned mask = (unsigned)__ballot(there);
-      if (lane == 0) s_there[buf] = mask;
+      if (lane == 0) {
+        s_note[buf].there = mask; s_note[buf].bad.any = bad.any;
+        if (bad.any) s_note[buf].bad = bad;
+      }
     }
   };
 
@@ -1357,12 +1379,13 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
 #pragma unroll
         for (int j = 0; j < KW; ++j) k[c][half * KW + j] = w[j];
       }
-    const unsigned here = s_there[buf];
+    const unsigned here = s_note[buf].there, any_bad = __builtin_amdgcn_readfirstlane(s_note[buf].bad.any);
     float s[NT][8];
     step_scores<D, NT>(k, [&](int nt, int w) { return __builtin_bit_cast(h8, s_q[(wave * (D / 32) + w) * 64 + lane]); }, qs, st, s);
     uint32_t pw[NT][G + 1][4];
     step_weights<D, NT, NT>(s, here, k0, limit, mul, st, m, o, ob, pw);
     step_values<D, NT, NT>(pw, st, ones, o, ob);
+    if (any_bad) mark_bad<D, NT, NT>(s_note[buf].bad, k0, limit, ob);
     turn(i);
   }
   for (; i < steps; ++i, k0 += AT_STEP) turn(i);

@@ -30,7 +30,7 @@ SPLIT = [(64, "f16", 4, 2, 32, [3000, 200], [1, 1]), (128, "bf16", 6, 2, 16, [29
 
 
 @pytest.mark.parametrize("dim, dtype, heads, kv, page, lens, rows", SPLIT)
-@pytest.mark.parametrize("what", ["query", "keys"])
+@pytest.mark.parametrize("what", ["query", "keys", "values"])
 def test_what_is_not_finite_shows_however_the_axis_is_cut(dim, dtype, heads, kv, page, lens, rows, what):
     rng = np.random.default_rng(40)
     pool, parts, table, n_pages = filled(rng, lens, page, kv, dim)
