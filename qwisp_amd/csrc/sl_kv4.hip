@@ -716,10 +716,61 @@ struct BadValues {
   unsigned any = 0;
   uint32_t keys[D / 64];                      // by group, where there are any
 };
+// Weights meet the values as fp16 operands, p s and p, which have 11 bits from 2^-14 to 2^16 and lose them below.  So both are taken in units:
+// p is formed 2^6 times too large (a row's output is a quotient, from which that falls out), and the value scales of a group are taken times a power of
+// two that brings the largest near 2^6.  It only falls while a wave goes along its keys, and its sums with it; below 1 it
+// stands where scales beyond 128 (values beyond some 1000) are met, and only then can a scale 2^21 below the largest lose bits.
+// p keeps its 11 bits down to 2^-20 and p s down to 2^-25 of the largest s; they are there down to 2^-31 and 2^-36.  One key 13 above 4095
+// others, values of 0.02: rows in bf16 are off by 1.6e-3 of their size, which is that type's own rounding (without units 6e-3 with
+// 64 dims, 2.3e-2 in tiles of 64 rows); values of 1e-5: 1.5e-3 (4.7e-2).  Some ten instructions a step: 32 lanes of 256 dims 1.4 us of 38, a prompt 5 of 140.
+constexpr float P_UNIT_LOG2 = 6.0f;
+constexpr uint32_t UNIT_TOP = 0x58005800u;          // 128 as halves: p reaches 2^8.875, p s then 2^15.875
+template <int D>
+struct ValueUnit {
+  uint32_t f[(D / 64 + 1) / 2];                // by group, as halves; the same in all lanes
+  SL_DEV bool operator!=(const ValueUnit& o) const {
+    bool other = false;
+#pragma unroll
+    for (int w = 0; w < (D / 64 + 1) / 2; ++w) other = other || f[w] != o.f[w];
+    return other;
+  }
+  SL_DEV int log2_of(int g) const { return (int)((f[g / 2] >> (16 * (g & 1) + 10)) & 31u) - 15; }
+};
+template <int D>
+SL_DEV ValueUnit<D> first_unit() {
+  ValueUnit<D> u;
+#pragma unroll
+  for (int w = 0; w < (D / 64 + 1) / 2; ++w) u.f[w] = 0x78007800u;            // 2^15
+  return u;
+}
+SL_DEV float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+SL_DEV uint32_t max_halves(uint32_t a, uint32_t b) {                           // of two pairs of 16-bit numbers
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+// The unit for value scales (lanes 32..63, two groups a word) of which one is too large for the present one.
+template <int D>
+SL_DEV void lower_unit(const uint32_t (&sc)[(D / 64 + 1) / 2], ValueUnit<D>& unit) {
+#pragma unroll
+  for (int w = 0; w < (D / 64 + 1) / 2; ++w) {
+    uint32_t x = sc[w] & 0x7fff7fffu;
+    x = max_halves(x, dpp_u<DPP_XOR1>(x)); x = max_halves(x, dpp_u<DPP_XOR2>(x));
+    x = max_halves(x, dpp_u<DPP_HALF_MIRROR>(x)); x = max_halves(x, dpp_u<DPP_MIRROR>(x));
+    x = max_halves((uint32_t)__builtin_amdgcn_readlane((int)x, 32), (uint32_t)__builtin_amdgcn_readlane((int)x, 48));
+    uint32_t f = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int top = (int)((x >> (16 * u)) & 0x7fffu), old = (int)((unit.f[w] >> (16 * u)) & 0xffffu);
+      const int e = top >= 0x400 ? (top >> 10) - 15 : 31 - __builtin_clz(top | 1) - 24;          // 2^e <= the largest < 2^(e+1)
+      f |= (uint32_t)min(old, top ? (min(15, 5 - e) + 15) << 10 : old) << (16 * u);
+    }
+    unit.f[w] = __builtin_amdgcn_readfirstlane(f);
+  }
+}
 // Scales and biases (lanes 0..31: key `lane`, lanes 32..63: value of key lane - 32) into LDS; a key that is not there gets
 // zeros.  Value lanes turn b into b + 8 s; a group in which that is not finite gets zeros and is named in what comes back.
 template <int D>
-SL_DEV BadValues<D> put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& st) {
+SL_DEV BadValues<D> put_scales(const uint32_t (&sb)[D / 64], bool there, const StepLds& st, ValueUnit<D>& unit) {
   constexpr int G = D / 64, W = (G + 1) / 2;
   const int lane = threadIdx.x & 63;
   uint32_t sc[W], bi[W];
@@ -748,6 +799,17 @@ SL_DEV BadValues<D> put_scales(const uint32_t (&sb)[D / 64], bool there, const S
       if (bad) { bi[g / 2] &= ~half; sc[g / 2] &= ~half; }
     }
   }
+  auto in_unit = [&](int w) { return __builtin_bit_cast(uint32_t, as_h2(sc[w]) * as_h2(unit.f[w])); };
+  uint32_t over = 0, x[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) { x[w] = in_unit(w); over |= (x[w] & 0x7fff7fffu) + (0x7fff7fffu - UNIT_TOP); }
+  if (__any((over & 0x80008000u) != 0 && lane >= 32)) {
+    lower_unit<D>(sc, unit);
+#pragma unroll
+    for (int w = 0; w < W; ++w) x[w] = in_unit(w);
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w) sc[w] = lane < 32 ? sc[w] : x[w];
   if constexpr (G == 4) {
     *reinterpret_cast<uint2*>(st.ks + lane * G) = make_uint2(sc[0], sc[1]);
     if (lane < 32) *reinterpret_cast<uint2*>(st.kb + lane * G) = make_uint2(bi[0], bi[1]);
@@ -833,8 +895,7 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
 #pragma unroll
     for (int t = 1; t < 8; ++t) top = fmaxf(top, s[nt][t]);
     top = rows4_max(top);
-    // The reference moves only where a row's maximum has grown past it by a factor of 2^2.875 = 7.3: until then p lies above 1, and
-    // p s stays within fp16 (|s| < 8734.1, for no value lies beyond 65504).
+    // The reference moves only where a row's maximum has grown past it by a factor of 2^2.875 = 7.3: until then p lies above 1.
     if (__any((top - m[nt]) * mul[nt] > 2.875f)) {
       const float next = fmaxf(m[nt], top), back = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m[nt] - next) * mul[nt]);
       ob[nt] = ob[nt] * back;
@@ -844,7 +905,7 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
         for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
       m[nt] = next;
     }
-    const float from = m[nt] == -__builtin_inff() ? 0.0f : -m[nt] * mul[nt];
+    const float from = m[nt] == -__builtin_inff() ? 0.0f : fmaf(-m[nt], mul[nt], P_UNIT_LOG2);
     float p[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(fmaf(s[nt][t], mul[nt], from));
@@ -854,6 +915,21 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
     for (int g = 0; g < G; ++g)
 #pragma unroll
       for (int t = 0; t < 4; ++t) pw[nt][g][t] = pair_of(fmaf(p[2 * t], nth_half(vs, 2 * t * G + g), 0.0f), fmaf(p[2 * t + 1], nth_half(vs, (2 * t + 1) * G + g), 0.0f));   // (fma: takes the half as it is)
+  }
+}
+// The sums of (p s) c and of p s brought to another unit.
+template <int D, int NT>
+SL_DEV void change_unit(const ValueUnit<D>& was, const ValueUnit<D>& unit, f4 (&o)[NT][D / 64][4], f4 (&ob)[NT]) {
+  const int kg = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int g = 0; g < D / 64; ++g) {
+    const float by = pow2(unit.log2_of(g) - was.log2_of(g));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      ob[nt][g] = kg == 2 ? ob[nt][g] * by : ob[nt][g];                // (lanes of the third 16 hold rows 8..11 of ob)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * by;
+    }
   }
 }
 // Rows that see a key whose values in a group are not finite: their sum over b + 8 s of that group becomes NaN, and all its dims with it.
@@ -1001,18 +1077,22 @@ SL_DEV void finish_row(const sl_kv4_attn_args& a, int t, int head, int d, float4
 }
 // A wave's sums of one row tile to LDS [16 rows][D + 4], times f: lane (n16, kg) holds dims 64 g + 16 kg + 4 r + i of row n16.
 template <int D>
-SL_DEV void put_sums(const f4 (&o)[D / 64][4], const f4& ob, float f, float* to) {
+SL_DEV void put_sums(const f4 (&o)[D / 64][4], const f4& ob, const ValueUnit<D>& unit, float f, float* to) {
   const int lane = threadIdx.x & 63, n16 = lane & 15, kg = lane >> 4;
-  float bias[D / 64];
+  float bias[D / 64], even[D / 64], odd[D / 64];
 #pragma unroll
-  for (int g = 0; g < D / 64; ++g) bias[g] = fmaf(-8.0f, __shfl(ob[g], n16 + 32), __shfl(ob[g], n16));
+  for (int g = 0; g < D / 64; ++g) {
+    const float back = pow2(-unit.log2_of(g));
+    even[g] = 16777216.0f * back; odd[g] = 1048576.0f * back;
+    bias[g] = fmaf(-8.0f * back, __shfl(ob[g], n16 + 32), __shfl(ob[g], n16));
+  }
 #pragma unroll
   for (int g = 0; g < D / 64; ++g)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       float4 y;
-      y.x = fmaf(o[g][0][r], 16777216.0f, bias[g]) * f; y.y = fmaf(o[g][1][r], 1048576.0f, bias[g]) * f;
-      y.z = fmaf(o[g][2][r], 16777216.0f, bias[g]) * f; y.w = fmaf(o[g][3][r], 1048576.0f, bias[g]) * f;
+      y.x = fmaf(o[g][0][r], even[g], bias[g]) * f; y.y = fmaf(o[g][1][r], odd[g], bias[g]) * f;
+      y.z = fmaf(o[g][2][r], even[g], bias[g]) * f; y.w = fmaf(o[g][3][r], odd[g], bias[g]) * f;
       *reinterpret_cast<float4*>(to + n16 * (D + 4) + 64 * g + 16 * kg + 4 * r) = y;
     }
 }
@@ -1142,6 +1222,8 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
         for (int i = 0; i < 4; ++i) o[nt][g][i] = f4{0, 0, 0, 0};
     }
 
+    ValueUnit<D> unit = first_unit<D>();
+
     // ---- keys: a step of 32 for the first LIVE row tiles ----
     auto keys_loop = [&](auto live_tiles) {
       constexpr int LIVE = decltype(live_tiles)::value;
@@ -1149,7 +1231,9 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
         const bool more = k0 + AT_UNIT < key1;
         const unsigned there = (unsigned)__ballot(cur.there);
         wave_lds_order();
-        const BadValues<D> bad = put_scales<D>(cur.sb, cur.there, st);
+        const ValueUnit<D> was = unit;
+        const BadValues<D> bad = put_scales<D>(cur.sb, cur.there, st, unit);
+        if (unit != was) change_unit<D, NT>(was, unit, o, ob);
         // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
 #pragma unroll
         for (int c = 0; c < G; ++c) {
@@ -1196,7 +1280,7 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
 #pragma unroll
       for (int w = 0; w < AT_WAVES; ++w) top = fmaxf(top, s_m[w * 16 * NT + nt * 16 + n16]);
       const float f = m[nt] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[nt] - top);
-      put_sums<D>(o[nt], ob[nt], f, s_o + wave * 16 * (D + 4));
+      put_sums<D>(o[nt], ob[nt], unit, f, s_o + wave * 16 * (D + 4));
       lds_barrier();
       // a thread per four dims of a row
       for (int i = tid; i < 16 * (D / 4); i += 256) {
@@ -1302,8 +1386,9 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
     }
   };
   auto step_lds = [&](int buf) { return lds + buf * L::STEP; };
-  struct Note { unsigned there; BadValues<D> bad; };
-  Note* s_note = reinterpret_cast<Note*>(s_m);                         // by buffer: the keys that are there; free until the end
+  struct Note { unsigned there; ValueUnit<D> unit; BadValues<D> bad; };
+  Note* s_note = reinterpret_cast<Note*>(s_m);                         // by buffer: the keys that are there, the values' unit; free until the end
+  ValueUnit<D> unit_put = first_unit<D>(), unit = unit_put;            // of the first wave's last step in LDS, of this wave's sums
   // keys: [operand][half of the row's quarter][quarter][row of the operand]; values: pieces of 4 dims, two keys a word
   const int k_to = ((((key_token >> 2) & 1) * HALVES + key_part % HALVES) * 64 + key_part / HALVES * 16 + (key_token >> 3) * 4 + (key_token & 3)) * 4 * KW;
   const int v_to = v_m / (16 / G) * V_STRIDE + (v_blk * 16 + G * (v_m % (16 / G))) * 16 + v_sub * 4;
@@ -1315,10 +1400,10 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
     for (int c = 0; c < 4; ++c)            // two keys of 8 bytes: a word of four pieces
       *reinterpret_cast<uint32_t*>(st.v + v_to + 16 * c) = __builtin_amdgcn_perm(wv[2 + c / 2], wv[c / 2], c & 1 ? 0x07060302u : 0x05040100u);
     if (wave == 0) {
-      const BadValues<D> bad = put_scales<D>(sb, there, st);
+      const BadValues<D> bad = put_scales<D>(sb, there, st, unit_put);
       const unsigned mask = (unsigned)__ballot(there);
       if (lane == 0) {
-        s_note[buf].there = mask; s_note[buf].bad.any = bad.any;
+        s_note[buf].there = mask; s_note[buf].unit = unit_put; s_note[buf].bad.any = bad.any;
         if (bad.any) s_note[buf].bad = bad;
       }
     }
@@ -1380,6 +1465,10 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
         for (int j = 0; j < KW; ++j) k[c][half * KW + j] = w[j];
       }
     const unsigned here = s_note[buf].there, any_bad = __builtin_amdgcn_readfirstlane(s_note[buf].bad.any);
+    ValueUnit<D> now = s_note[buf].unit;
+#pragma unroll
+    for (uint32_t& f : now.f) f = __builtin_amdgcn_readfirstlane(f);
+    if (now != unit) { change_unit<D, NT>(unit, now, o, ob); unit = now; }
     float s[NT][8];
     step_scores<D, NT>(k, [&](int nt, int w) { return __builtin_bit_cast(h8, s_q[(wave * (D / 32) + w) * 64 + lane]); }, qs, st, s);
     uint32_t pw[NT][G + 1][4];
@@ -1395,7 +1484,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
   const float total = sum_of<D>(ob[0]);
   if (kg == 0) { s_m[wave * 16 + n16] = m[0]; s_l[wave * 16 + n16] = total; }
   float* s_o = reinterpret_cast<float*>(lds);
-  put_sums<D>(o[0], ob[0], 1.0f, s_o + wave * 16 * (D + 4));
+  put_sums<D>(o[0], ob[0], unit, 1.0f, s_o + wave * 16 * (D + 4));
   lds_barrier();
   for (int i = tid; i < 64 * (D / 4); i += 256) {
     const int in = i / (D / 4), d = 4 * (i % (D / 4));

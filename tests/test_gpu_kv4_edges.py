@@ -1,5 +1,5 @@
-"""The 4-bit cache's attention where numbers are not finite: against the plain 64-bit form, with tolerances that follow the values'
-own size."""
+"""The 4-bit cache's attention where numbers are not finite, very small or very unlike: against the plain 64-bit form,
+with tolerances that follow the values' own size."""
 import numpy as np
 import pytest
 
@@ -100,3 +100,80 @@ def compare(have, want, var, size, fp32=2.0 ** -15, least=2.0 ** -25):
     assert rms(err) <= 2 * np.sqrt(var.mean()) + fp32 * rms(size) + least, (rms(err), np.sqrt(var.mean()), rms(size))
     worst = err / (7 * np.sqrt(var) + 4 * fp32 * size + 2 * least)
     assert worst.max() <= 1, worst.max()
+
+
+# (dim, dtype, heads, kv, page, lengths, rows)
+SHAPES = [(64, "bf16", 4, 4, 32, [4096, 333], [1, 1]), (128, "f16", 8, 2, 16, [3000, 4100], [2, 3]), (256, "f16", 4, 1, 64, [5000], [1]),
+          (64, "f16", 2, 2, 64, [4000], [40]), (128, "bf16", 2, 1, 32, [3500], [24]), (256, "f16", 4, 1, 64, [2048], [20])]
+
+
+def case(shape, seed, values, sink=0.0, mean=1.0):
+    """Keys of size one; values of the given size around a mean per dim; with a sink the first key lies along all queries
+    and stands `sink` above the others, its own value near zero."""
+    dim, dtype, heads, kv, page, lens, rows = shape
+    rng = np.random.default_rng(seed)
+    count = [-(-n // page) for n in lens]
+    order = rng.permutation(sum(count) + 2).astype(np.int32)
+    table = np.full((len(lens), max(count)), -1, np.int32)
+    n_rows = len(order) * page
+    u = rng.normal(size=dim)
+    u /= np.linalg.norm(u)
+    k = rng.normal(size=(n_rows, kv, dim))
+    v = values * (mean * rng.normal(size=(1, kv, dim)) + 0.5 * rng.normal(size=(n_rows, kv, dim)))
+    q = rng.normal(size=(sum(rows), heads, dim))
+    if sink:
+        k -= (k @ u)[..., None] * u
+        q = 0.3 * (q - (q @ u)[..., None] * u) + 8 * u
+    at = 0
+    for r, c in enumerate(count):
+        table[r, :c] = order[at:at + c]
+        at += c
+        if sink:
+            first = table[r, 0] * page
+            k[first] = u * (sink / 8 * dim ** 0.5)
+            v[first] = 0.001 * v[first]
+    parts = dict(k=ref.quantise(k), v=ref.quantise(v))
+    pool = kv4().Pool(gpu(ref.pack(parts["k"], parts["v"], page, kv, dim)), page, kv, dim)
+    return pool, gpu(q, DTYPES[dtype]), parts, table, offsets(rows)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("values", [1.0, 1e-2, 1e-4, 1e-5])
+@pytest.mark.parametrize("mean", [0.0, 1.0])
+def test_values_of_any_size_keep_their_digits(shape, values, mean):
+    dim, dtype, heads, kv, page, lens, rows = shape
+    pool, q, parts, table, start = case(shape, 41, values, mean=mean)
+    q = q.to(torch.bfloat16)                                 # (outputs of any size keep their digits)
+    have = f64(call(pool, q, table, start, lens))
+    compare(have, *expected(f64(q), parts, table, start, lens, page, dim ** -0.5, HALF_STEP["bf16"]), least=0.0)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("values, sink", [(0.1, 10.0), (0.02, 13.0), (1.0, 16.0), (1e-3, 13.0)])
+def test_one_key_far_above_the_rest(shape, values, sink):
+    dim, dtype, heads, kv, page, lens, rows = shape
+    pool, q, parts, table, start = case(shape, 42, values, sink)
+    have = f64(call(pool, q, table, start, lens))
+    compare(have, *expected(f64(q), parts, table, start, lens, page, dim ** -0.5, HALF_STEP[dtype]))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_values_that_grow_along_the_axis(shape):
+    """Values of sizes from e^-7 to e^7 within a sequence, the largest in its middle, and weights that fall as the values grow,
+    so that all of them count: the unit of the weighted scales changes on the way."""
+    dim, dtype, heads, kv, page, lens, rows = shape
+    pool, q, parts, table, start = case(shape, 43, 1.0)
+    rng = np.random.default_rng(44)
+    u = rng.normal(size=dim)
+    u /= np.linalg.norm(u)
+    for r, n in enumerate(lens):
+        at = table[r, np.arange(n) // page] * page + np.arange(n) % page
+        size = 7.0 * np.sin(np.linspace(-np.pi / 2, 3 * np.pi / 2, n))[:, None, None]
+        k = 0.3 * rng.normal(size=(n, kv, dim)) - size * u * (dim ** 0.5 / 8)
+        for name, x in (("k", k), ("v", rng.normal(size=(n, kv, dim)) * np.exp(size))):
+            for key, y in ref.quantise(x).items():
+                parts[name][key][at] = y
+    pool = kv4().Pool(gpu(ref.pack(parts["k"], parts["v"], page, kv, dim)), page, kv, dim)
+    q = gpu(0.3 * rng.normal(size=tuple(q.shape)) + 8 * u, torch.bfloat16)
+    have = f64(call(pool, q, table, start, lens))
+    compare(have, *expected(f64(q), parts, table, start, lens, page, dim ** -0.5, HALF_STEP["bf16"]), least=0.0)
