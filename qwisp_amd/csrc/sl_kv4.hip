@@ -905,7 +905,15 @@ SL_DEV void step_weights(float (&s)[LIVE][8], unsigned there, int k0, const int 
         for (int i = 0; i < 4; ++i) o[nt][g][i] = o[nt][g][i] * back;
       m[nt] = next;
     }
-    const float from = m[nt] == -__builtin_inff() ? 0.0f : fmaf(-m[nt], mul[nt], P_UNIT_LOG2);
+    float from = m[nt] == -__builtin_inff() ? 0.0f : fmaf(-m[nt], mul[nt], P_UNIT_LOG2);
+    // The fused difference is off by the rounding of m * mul: 2^-12 here at most.  Beyond that the scores are subtracted first, which is
+    // exact where it counts, next to the reference.
+    if (__any(fabsf(from) > 4096.0f)) {
+      const float ref = m[nt] == -__builtin_inff() ? 0.0f : m[nt];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) s[nt][t] = s[nt][t] - ref;
+      from = P_UNIT_LOG2;
+    }
     float p[8];
 #pragma unroll
     for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(fmaf(s[nt][t], mul[nt], from));
@@ -1024,7 +1032,7 @@ SL_DEV void put_query(const uint2 (&raw)[D / 64], int in, bool valid, int limit,
   }
   top = fmaxf(top, dpp_f<DPP_XOR1>(top)); top = fmaxf(top, dpp_f<DPP_XOR2>(top));
   top = fmaxf(top, dpp_f<DPP_HALF_MIRROR>(top)); top = fmaxf(top, dpp_f<DPP_MIRROR>(top));
-  const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 100);
+  const int e = min(max((int)((__float_as_uint(top) >> 23) & 255u) - 127, -100), 127);
   const float f = __uint_as_float((uint32_t)(127 + 10 - e) << 23) * (scale < 0.0f ? -1.0f : 1.0f);
   float sum = 0.0f;
 #pragma unroll
@@ -1040,8 +1048,8 @@ SL_DEV void put_query(const uint2 (&raw)[D / 64], int in, bool valid, int limit,
     }
   }
   if (l16 == 0) {
-    // (a factor of zero would leave hidden keys without their minus infinity)
-    q.mul[in] = fmaxf(fabsf(scale) * 1.44269504088896f * (16777216.0f * __uint_as_float((uint32_t)(127 - 10 + e) << 23)), 1e-30f);
+    // (a factor of zero would leave hidden keys without their minus infinity, one of infinity the largest score without its zero)
+    q.mul[in] = fminf(fmaxf(fabsf(scale) * (1.44269504088896f * 16777216.0f) * pow2(e - 10), 1e-30f), 3e38f);
     q.limit[in] = limit;
   }
   // operand word w of quarter kg in group g: dims 64 g + 16 kg + 8 w + (0 4 | 1 5 | 2 6 | 3 7), the odd ones / 16

@@ -1,4 +1,4 @@
-"""The 4-bit cache's attention where numbers are not finite, very small or very unlike: against the plain 64-bit form,
+"""The 4-bit cache's attention where numbers are not finite, very small, very large or very unlike: against the plain 64-bit form,
 with tolerances that follow the values' own size."""
 import numpy as np
 import pytest
@@ -177,3 +177,38 @@ def test_values_that_grow_along_the_axis(shape):
     q = gpu(0.3 * rng.normal(size=tuple(q.shape)) + 8 * u, torch.bfloat16)
     have = f64(call(pool, q, table, start, lens))
     compare(have, *expected(f64(q), parts, table, start, lens, page, dim ** -0.5, HALF_STEP["bf16"]), least=0.0)
+
+
+# ---- very large scores ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim, heads, kv, page, lens, rows", [(128, 4, 2, 32, [500, 33], [1, 2]), (64, 3, 3, 16, [400], [33]), (256, 4, 1, 64, [300], [20]), (256, 8, 2, 64, [3000], [1])])
+@pytest.mark.parametrize("dtype, size", [("f16", 2.0 ** 15), ("bf16", 2.0 ** 20), ("bf16", 2.0 ** 60), ("bf16", 2.0 ** 105)])
+def test_scores_beyond_what_fp32_tells_apart_choose_the_largest(dim, heads, kv, page, lens, rows, dtype, size):
+    """Scores of 1e7 and more: one key has all the weight.  Rows whose two largest scores lie within fp32's error of them are left out."""
+    rng = np.random.default_rng(45)
+    pool, parts, table, _ = filled(rng, lens, page, kv, dim)
+    k = ref.quantise(rng.normal(size=parts["k"]["codes"].shape) * 3000)
+    bad = np.isnan(parts["k"]["scale"])
+    for key in k:
+        parts["k"][key] = np.where(bad if key != "codes" else False, parts["k"][key], k[key])
+    pool = kv4().Pool(gpu(ref.pack(parts["k"], parts["v"], page, kv, dim)), page, kv, dim)
+    start = offsets(rows)
+    q = gpu(rng.normal(size=(int(start[-1]), heads, dim)).clip(-1.9, 1.9) * size, DTYPES[dtype])
+    have, qq = f64(call(pool, q, table, start, lens)), f64(q)
+    kk, vv = ref.values(parts["k"]), ref.values(parts["v"])
+    used = 0
+    for r, n in enumerate(lens):
+        j = np.arange(n)
+        at = table[r, j // page] * page + j % page
+        for i in range(rows[r]):
+            m = n - rows[r] + i + 1
+            for h in range(heads):
+                g = h // (heads // kv)
+                terms = kk[at[:m], g] * qq[start[r] + i, h]
+                s = terms.sum(-1)
+                two = np.sort(s)[-2:]
+                if two[1] - two[0] <= 2.0 ** -24 * (dim + 8) * 4 * np.abs(terms).sum(-1).max():
+                    continue
+                used += 1
+                want, e = vv[at[s.argmax()], g], 2 * H * (np.abs(vv[at[s.argmax()], g]) + 8 * np.abs(np.repeat(parts["v"]["scale"][at[s.argmax()], g], 64)))
+                assert (np.abs(have[start[r] + i, h] - want) <= e + HALF_STEP[dtype] * np.abs(want) + 2.0 ** -25).all()
+    assert used > 0
