@@ -338,6 +338,7 @@ typedef struct sl_sched sl_sched;
  * error.  The caller serialises submit and round. */
 int sl_sched_create(const sl_batch_slots* slots, int token_budget, sl_token_fn on_token, sl_finish_fn on_finish,
                     void* user, sl_sched** out);
+/* Releases the slots of requests that have not ended, so that another scheduler can be made on the same table. */
 void sl_sched_destroy(sl_sched* s);
 int sl_sched_submit(sl_sched* s, const int32_t* prompt, int n_prompt, int max_tokens, const int32_t* stop, int n_stop);
 int sl_sched_round(sl_sched* s);

@@ -147,7 +147,13 @@ int sl_sched_create(const sl_batch_slots* slots, int token_budget, sl_token_fn o
   *out = s;
   return SL_OK;
 }
-void sl_sched_destroy(sl_sched* s) { delete s; }
+void sl_sched_destroy(sl_sched* s) {
+  if (!s) return;
+  for (int b : s->pending) s->slots.release(s->slots.ctx, b);          // the slots of what has not ended are free again
+  for (int b = 0; b < s->slots.slot_count; ++b)
+    if (s->active[b].job >= 0) s->slots.release(s->slots.ctx, b);
+  delete s;
+}
 
 int sl_sched_submit(sl_sched* s, const int32_t* prompt, int n_prompt, int max_tokens, const int32_t* stop, int n_stop) {
   if (!s || !prompt || n_prompt < 1 || n_stop < 0 || (n_stop > 0 && !stop)) return SL_ERR_ARG;
