@@ -186,10 +186,27 @@ struct sl_lane_slots {
   std::vector<int32_t> toks, outs;
   int chunk = 1, max_seq = 0;
   long kv_budget_tokens = 0;
-  // lanes with 4-bit caches share pages (page_size > 0): requests let in wait for the pages of their whole length
+  // lanes with 4-bit caches share pages (page_size > 0): a request begins once there are pages for its whole length, and until then waits
+  // in its slot, in front of those that come later
   int32_t page_size = 0, n_pages = 0;
-  long promised = 0;                // pages of requests let in that have not begun
+  struct Waiting { int slot; long pages; };
+  std::vector<Waiting> waiting;     // in the order in which they came
   long pages(long tokens) const { return (tokens + page_size - 1) / page_size; }
+  // Pages that are spoken for: by requests that have begun, by those that wait in front of `slot` (-1: by all that wait), and by others.
+  long spoken(int slot) const {
+    long n = others();
+    for (size_t i = 0; i < reserved.size(); ++i)
+      if ((int)i != slot) n += pages(reserved[i]);
+    for (const Waiting& w : waiting) {
+      if (w.slot == slot) break;
+      n += w.pages;
+    }
+    return n;
+  }
+  void no_longer_waits(int slot) {
+    for (size_t i = 0; i < waiting.size(); ++i)
+      if (waiting[i].slot == slot) { waiting.erase(waiting.begin() + (long)i); return; }
+  }
   long others() const {             // pages of sequences that are not slots
     long held = n_pages - sl_kv4_free_pages(lanes[0], nullptr, nullptr);
     for (sl_engine* e : lanes) held -= pages(sl_position(e));
@@ -207,8 +224,15 @@ int lane_admit_step(void* ctx, const int32_t* prompt, int n_prompt, int slot, in
   if (seq_budget > L->max_seq || n_prompt + 1 > L->max_seq) return -1;      // would overflow the lane's KV arena
   sl_engine* e = L->lanes[slot];
   if (L->pos[slot] == 0 && L->page_size && seq_budget > 0) {
-    L->promised -= L->promised < L->pages(seq_budget) ? L->promised : L->pages(seq_budget);
-    if (L->pages(seq_budget) > L->n_pages) return -1;                       // more than all pages
+    const long need = L->pages(seq_budget);
+    const long spoken = L->spoken(slot);
+    if (need > L->n_pages) return -1;                                       // more than all pages
+    if (spoken + need > L->n_pages) {
+      for (const auto& w : L->waiting) if (w.slot == slot) return 1;
+      L->waiting.push_back({slot, need});
+      return 1;
+    }
+    L->no_longer_waits(slot);
   }
   if (L->pos[slot] == 0) {
     if (sl_reset(e) != SL_OK) return -1;
@@ -243,20 +267,18 @@ void lane_release(void* ctx, int slot) {
   sl_lane_slots* L = (sl_lane_slots*)ctx;
   if (slot < 0 || slot >= (int)L->lanes.size()) return;
   L->pos[slot] = 0; L->reserved[slot] = 0;
+  L->no_longer_waits(slot);
   if (L->page_size) (void)sl_reset(L->lanes[slot]);        // its pages go to the others now, not when the slot is used again
 }
 int lane_can_admit(void* ctx, int prompt_len, int seq_budget) {
   sl_lane_slots* L = (sl_lane_slots*)ctx;
+  (void)prompt_len;
   long held = 0;
   for (int r : L->reserved) held += r;
   if (held + seq_budget > L->kv_budget_tokens) return 0;
-  // (what no pages could ever hold is let in, for admit_step to refuse; a request of no tokens never comes there)
-  if (!L->page_size || seq_budget > L->max_seq || L->pages(seq_budget) > L->n_pages || seq_budget <= prompt_len + 1) return 1;
-  long used = L->promised + L->others();
-  for (int r : L->reserved) used += L->pages(r);
-  if (used + L->pages(seq_budget) > L->n_pages) return 0;
-  L->promised += L->pages(seq_budget);
-  return 1;
+  // (what no pages could ever hold is let in, for admit_step to refuse)
+  if (!L->page_size || seq_budget > L->max_seq || L->pages(seq_budget) > L->n_pages) return 1;
+  return L->spoken(-1) + L->pages(seq_budget) <= L->n_pages ? 1 : 0;
 }
 
 }  // namespace
