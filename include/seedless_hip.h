@@ -348,9 +348,10 @@ int sl_sched_round(sl_sched* s);
  * (<= 0: n_slots * max_seq_len).  Fills `table` for sl_sched_create; destroy after the scheduler, before `base`.
  * On a base with 4-bit caches (sl_set_kv4) a request's pages go back when it ends, and one begins only once the pages hold what
  * all that have begun may grow to: can_admit says so (and changes nothing), and admit_step of a request for which they do not yet returns 1
- * with nothing consumed; later requests do not begin in front of it.  A request that needs more pages than there are ends like one whose
- * prompt fails.  Without a budget (kv_budget_tokens <= 0) the pages have to hold every slot at max_seq_len, else SL_ERR_TOO_LARGE.
- * (A scheduler without a token budget names no length: there a request that finds no pages ends, as any whose prompt fails.) */
+ * with nothing consumed; later requests do not begin in front of it.  A request ends like one whose prompt fails if it needs more
+ * pages than there are, or than sequences beside the slots (the base's own, other lanes) leave while no slot is in use.  Without
+ * a budget (kv_budget_tokens <= 0) the pages have to hold every slot at max_seq_len, else SL_ERR_TOO_LARGE.  (A scheduler without a
+ * token budget names no length: there a request that finds no pages ends, as any whose prompt fails.) */
 typedef struct sl_lane_slots sl_lane_slots;
 int sl_lane_slots_create(const sl_engine* base, int n_slots, int chunk_rows, int max_seq_len, long kv_budget_tokens,
                          sl_lane_slots** out, sl_batch_slots* table);

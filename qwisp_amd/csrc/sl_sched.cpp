@@ -193,15 +193,16 @@ struct sl_lane_slots {
   std::vector<Waiting> waiting;     // in the order in which they came
   long pages(long tokens) const { return (tokens + page_size - 1) / page_size; }
   // Pages that are spoken for: by requests that have begun, by those that wait in front of `slot` (-1: by all that wait), and by others.
-  long spoken(int slot) const {
-    long n = others();
+  struct Spoken { long pages; bool own; };
+  Spoken spoken(int slot) const {
+    Spoken s{others(), false};
     for (size_t i = 0; i < reserved.size(); ++i)
-      if ((int)i != slot) n += pages(reserved[i]);
+      if (reserved[i] && (int)i != slot) { s.pages += pages(reserved[i]); s.own = true; }
     for (const Waiting& w : waiting) {
       if (w.slot == slot) break;
-      n += w.pages;
+      s.pages += w.pages; s.own = true;
     }
-    return n;
+    return s;
   }
   void no_longer_waits(int slot) {
     for (size_t i = 0; i < waiting.size(); ++i)
@@ -225,9 +226,12 @@ int lane_admit_step(void* ctx, const int32_t* prompt, int n_prompt, int slot, in
   sl_engine* e = L->lanes[slot];
   if (L->pos[slot] == 0 && L->page_size && seq_budget > 0) {
     const long need = L->pages(seq_budget);
-    const long spoken = L->spoken(slot);
-    if (need > L->n_pages) return -1;                                       // more than all pages
-    if (spoken + need > L->n_pages) {
+    const auto spoken = L->spoken(slot);
+    if (need > L->n_pages || (spoken.pages + need > L->n_pages && !spoken.own)) {      // more than all pages, or than sequences beside the slots leave:
+      L->no_longer_waits(slot);                                                       // nothing that ends here would let it begin
+      return -1;
+    }
+    if (spoken.pages + need > L->n_pages) {
       for (const auto& w : L->waiting) if (w.slot == slot) return 1;
       L->waiting.push_back({slot, need});
       return 1;
@@ -278,7 +282,8 @@ int lane_can_admit(void* ctx, int prompt_len, int seq_budget) {
   if (held + seq_budget > L->kv_budget_tokens) return 0;
   // (what no pages could ever hold is let in, for admit_step to refuse)
   if (!L->page_size || seq_budget > L->max_seq || L->pages(seq_budget) > L->n_pages) return 1;
-  return L->spoken(-1) + L->pages(seq_budget) <= L->n_pages ? 1 : 0;
+  const auto spoken = L->spoken(-1);
+  return spoken.pages + L->pages(seq_budget) <= L->n_pages || !spoken.own ? 1 : 0;
 }
 
 }  // namespace

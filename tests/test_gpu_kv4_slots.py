@@ -67,6 +67,24 @@ def test_slots_of_a_scheduler_that_is_destroyed_serve_the_next(hybrid_model, kv4
     base.close()
 
 
+def test_a_request_that_others_pages_keep_out_for_good_ends(hybrid_model):  # noqa: F811
+    """The base's own sequence holds three of eight pages: a request for seven of them would wait for ever."""
+    from qwisp_amd.engine import LaneScheduler
+    cfg, dev = hybrid_model
+    base = make(cfg, dev, page_size=16, n_pages=8, max_m=8, max_seq_len=128)
+    for i in range(5):
+        assert base.step_argmax([i] * 8) is not None
+    sched = LaneScheduler(base, slots=2, chunk_rows=8, max_seq_len=128, token_budget=16, kv_budget_tokens=256)
+    jobs = jobs_of([(20, 10), (60, 50), (30, 40)], 52)
+    for p, n in jobs:
+        sched.submit(p, n)
+    want = alone(cfg, dev, jobs)
+    assert sched.run(max_rounds=400) == [want[0], [], want[2]]
+    assert base.kv4_free_pages() == 5
+    sched.close()
+    base.close()
+
+
 def test_large_requests_are_not_overtaken_for_ever(hybrid_model):  # noqa: F811
     """One request that needs all pages among many small ones: it begins before the small ones behind it."""
     from qwisp_amd import abi
