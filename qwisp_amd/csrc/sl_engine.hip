@@ -520,15 +520,16 @@ void launch_gdn_mixer(sl_engine* e, LayerDev& L, int li, int M, const HiddenArgs
 void kv4_failed(sl_engine* e, const char* what, int status) {
   if (e->fault.empty()) e->fault = std::string(what) + " failed with status " + std::to_string(status);
 }
-// Pages and row offsets of a call: lens.nw[i] rows come to sequence i (rows in the sequences' order), on e's stream.
-void kv4_begin(sl_engine* e, const Kv4Lens& lens) {
+// Pages and row offsets of a call: lens.nw[i] rows come to sequence i (rows in the sequences' order), on e's stream.  look: the slots
+// of rows that are there already; who holds which page stays as it is.
+void kv4_begin(sl_engine* e, const Kv4Lens& lens, bool look = false) {
   Kv4Store& k = *e->kv4;
   k.rows = k.most_rows = k.most_keys = 0;
   for (int i = 0; i < KV4_SEQS; ++i) {
     k.rows += lens.nw[i];
     k.most_rows = std::max(k.most_rows, lens.nw[i]);
     if (lens.nw[i]) k.most_keys = std::max(k.most_keys, lens.ctx[i] + lens.nw[i]);
-    if (k.seq[i]) k.seq[i]->kv4_rows = lens.ctx[i] + lens.nw[i];
+    if (k.seq[i] && !look) k.seq[i]->kv4_rows = lens.ctx[i] + lens.nw[i];
   }
   hipLaunchKernelGGL(k_kv4_lens, dim3(1), dim3(KV4_SEQS), 0, e->stream, lens, k.ctx, k.nw);
   const int a = k.now, b = 1 - a;
@@ -536,7 +537,7 @@ void kv4_begin(sl_engine* e, const Kv4Lens& lens) {
                            k.table[b], k.held[b], k.free_list[b], k.free_count[b], k.q_start, k.kv_len, k.slot, k.pos, k.unserved};
   const int r = sl_kv4_plan(&p, e->stream);
   if (r) { kv4_failed(e, "sl_kv4_plan", r); return; }
-  k.now = b;
+  if (!look) k.now = b;
 }
 void kv4_begin(sl_engine* e, int M) {
   Kv4Lens lens = kv4_lens(*e->kv4);
@@ -1702,12 +1703,12 @@ int sl_persist_restore(sl_engine* e, const void* src, size_t len) {
 }
 
 namespace {
-// Slots of rows 0 .. n - 1 of this sequence (and pages for them), as if they came now.
-int kv4_whole(sl_engine* e, int n) {
+// Slots of rows 0 .. n - 1 of this sequence: where they are (look), or as if they came now, with pages for them.
+int kv4_whole(sl_engine* e, int n, bool look) {
   Kv4Lens lens = kv4_lens(*e->kv4);
   lens.ctx[e->kv4_seq] = 0; lens.nw[e->kv4_seq] = n;
-  if (!kv4_fits(*e->kv4, lens)) return SL_ERR_TOO_LARGE;
-  kv4_begin(e, lens);
+  if (!look && !kv4_fits(*e->kv4, lens)) return SL_ERR_TOO_LARGE;
+  kv4_begin(e, lens, look);
   return e->fault.empty() ? SL_OK : SL_ERR_DEVICE;
 }
 // Device memory for the span of a call.
@@ -1721,7 +1722,7 @@ int kv4_read_rows(sl_engine* e, const LayerDev& L, uint16_t* k, uint16_t* v) {
   const size_t row = (size_t)SL_ATT_KV * SL_ATT_D * 2, head = SL_ATT_D * 2;
   Temp t;                                               // (before the plan: no work stays behind a call that fails)
   SL_TRY(e, hipMalloc(&t.p, 2 * n * row));
-  int r = kv4_whole(e, n); if (r) return r;
+  int r = kv4_whole(e, n, true); if (r) return r;
   uint8_t* dev[2] = {(uint8_t*)t.p, (uint8_t*)t.p + n * row};
   const sl_kv4_pool pool = kv4_pool(*e->kv4, L);
   r = sl_kv4_read(&pool, e->kv4->slot, n, SL_F16, dev[0], dev[1], e->stream);
@@ -1738,7 +1739,7 @@ int kv4_load_rows(sl_engine* e, const LayerDev& L, const uint16_t* k, const uint
   const size_t bytes = (size_t)SL_ATT_KV * n * SL_ATT_D * 2;
   Temp t;
   if (n > 0) SL_TRY(e, hipMalloc(&t.p, 2 * bytes));
-  int r = kv4_whole(e, n); if (r) return r;
+  int r = kv4_whole(e, n, false); if (r) return r;
   if (n == 0) return SL_OK;
   uint16_t* dev[2] = {(uint16_t*)t.p, (uint16_t*)((uint8_t*)t.p + bytes)};
   SL_TRY(e, hipMemcpyAsync(dev[0], k, bytes, hipMemcpyHostToDevice, e->stream));

@@ -104,3 +104,22 @@ def test_large_requests_are_not_overtaken_for_ever(hybrid_model):  # noqa: F811
     assert ended.index(2) == 2
     sched.close()
     base.close()
+
+
+def test_reading_a_cache_changes_nothing(hybrid_model):  # noqa: F811
+    """A rewound sequence still has the rows behind the rewind, and reading what is in front of it leaves them there."""
+    cfg, dev = hybrid_model
+    e = make(cfg, dev, page_size=16, max_m=8, max_seq_len=96)
+    for i in range(5):
+        assert e.step_argmax([i] * 8) is not None
+    early = e.full_snapshot()
+    for i in range(3):
+        assert e.step_argmax([9 + i] * 8) is not None
+    late, free = e.full_snapshot(), e.kv4_free_pages()
+    want = int(e.step_argmax([7])[0])
+    assert e.full_restore(late) and e.full_restore(early) and e.position == 40
+    k, v = e.read_layer_cache(3)
+    assert k.shape[1] == 40 and np.isfinite(k).all()
+    assert e.full_restore(late) and e.position == 64 and e.kv4_free_pages() == free
+    assert int(e.step_argmax([7])[0]) == want
+    e.close()
