@@ -130,8 +130,9 @@ struct Kv4Store {
   int32_t *ctx = nullptr, *nw = nullptr, *q_start = nullptr, *kv_len = nullptr, *slot = nullptr, *pos = nullptr, *unserved = nullptr;
   int now = 0;
   int rows = 0, most_rows = 0, most_keys = 0;      // of the call at work
-  void* workspace = nullptr;
+  void* workspace = nullptr;                       // for any call of the engine and its lanes, so that no call allocates; cache rows on their way, too
   int64_t workspace_bytes = 0;
+  ~Kv4Store() { if (workspace) (void)hipFree(workspace); }
 };
 
 struct sl_engine {
@@ -544,26 +545,48 @@ void kv4_begin(sl_engine* e, int M) {
   lens.nw[e->kv4_seq] = M;
   kv4_begin(e, lens);
 }
-sl_kv4_pool kv4_pool(const Kv4Store& k, const LayerDev& L) { return sl_kv4_pool{L.kv4, k.n_pages, k.page_size, SL_ATT_KV, SL_ATT_D}; }
+sl_kv4_pool kv4_pool(const Kv4Store& k, void* pages) { return sl_kv4_pool{pages, k.n_pages, k.page_size, SL_ATT_KV, SL_ATT_D}; }
+sl_kv4_attn_args kv4_attn_args(const Kv4Store& k, int rows, int most_rows, int most_keys) {
+  sl_kv4_attn_args t{};
+  t.n_req = KV4_SEQS; t.n_tokens = rows; t.n_heads = SL_ATT_HEADS; t.dtype = SL_F16; t.table_width = k.width; t.max_rows = most_rows; t.max_keys = most_keys;
+  t.scale = 0.0625f;
+  return t;
+}
+// Room for every call of up to max_m rows: a sequence's rows, or single rows of several.  (What a call takes grows with the longest length, but
+// for the step at twice its rows, above which they count as rows behind a long context.)
+int kv4_reserve(Kv4Store& k, int max_m) {
+  const sl_kv4_pool pool = kv4_pool(k, nullptr);
+  int64_t most = (int64_t)2 * 1024 * SL_ATT_KV * SL_ATT_D * 2;
+  for (int m = 1; m <= max_m; ++m)
+    for (const int rows : {m, 1})
+      for (const int keys : {(int)std::min<int64_t>(2ll * rows, k.max_seq), k.max_seq}) {
+        if (rows == 1 && m > KV4_SEQS) continue;
+        const sl_kv4_attn_args t = kv4_attn_args(k, m, rows, keys);
+        const int64_t need = sl_kv4_attention_workspace(&pool, &t);
+        if (need == 0) return SL_ERR_TOO_LARGE;
+        most = std::max(most, need);
+      }
+  if (most <= k.workspace_bytes) return SL_OK;
+  void* p = nullptr;
+  if (hipMalloc(&p, (size_t)most) != hipSuccess) { (void)hipGetLastError(); return SL_ERR_TOO_LARGE; }
+  if (k.workspace) (void)hipFree(k.workspace);          // (no call is at work, and hipFree waits for what still runs)
+  k.workspace = p; k.workspace_bytes = most;
+  return SL_OK;
+}
 // Attention of one layer over the 4-bit caches: projection rows in e->proj, gated output rows to e->ycore.
 void launch_attn_kv4(sl_engine* e, const LayerDev& L, int M) {
   if (!e->fault.empty()) return;
   Kv4Store& k = *e->kv4;
-  const sl_kv4_pool pool = kv4_pool(k, L);
+  const sl_kv4_pool pool = kv4_pool(k, L.kv4);
   const uint16_t *q = e->proj, *kk = e->proj + 8192, *vv = kk + SL_ATT_KV * SL_ATT_D;
   const sl_kv4_append_args a{M, SL_ATT_HEADS, SL_ROPE_DIM, e->max_seq, SL_F16, 0, EPS, q, kk, vv, L.q_norm, L.k_norm, e->rope_cos, e->rope_sin, k.slot, k.pos, e->qrot,
                              PROJ_STRIDE, 2 * SL_ATT_D, PROJ_STRIDE, SL_ATT_D, PROJ_STRIDE, SL_ATT_D, SL_ATT_HEADS * SL_ATT_D, SL_ATT_D};
   int r = sl_kv4_append(&pool, &a, e->stream);
   if (r) { kv4_failed(e, "sl_kv4_append", r); return; }
-  sl_kv4_attn_args t{KV4_SEQS, M, SL_ATT_HEADS, SL_F16, k.width, k.most_rows, k.most_keys, 0.0625f, e->qrot, e->proj + SL_ATT_D, e->ycore,
-                     SL_ATT_HEADS * SL_ATT_D, SL_ATT_D, PROJ_STRIDE, 2 * SL_ATT_D, SL_ATT_HEADS * SL_ATT_D, SL_ATT_D, k.table[k.now], k.q_start, k.kv_len, nullptr, 0};
-  const int64_t need = sl_kv4_attention_workspace(&pool, &t);
-  if (need > k.workspace_bytes) {              // grows with the rows of a call; calls are serialised, hipFree waits for what still runs
-    if (k.workspace) (void)hipFree(k.workspace);
-    k.workspace = nullptr; k.workspace_bytes = 0;
-    if (!ok(e, hipMalloc(&k.workspace, (size_t)need), "hipMalloc")) return;
-    k.workspace_bytes = need;
-  }
+  sl_kv4_attn_args t = kv4_attn_args(k, M, k.most_rows, k.most_keys);
+  t.q = e->qrot; t.gate = e->proj + SL_ATT_D; t.out = e->ycore;
+  t.q_token = t.out_token = SL_ATT_HEADS * SL_ATT_D; t.q_head = t.out_head = SL_ATT_D; t.gate_token = PROJ_STRIDE; t.gate_head = 2 * SL_ATT_D;
+  t.table = k.table[k.now]; t.q_start = k.q_start; t.kv_len = k.kv_len;
   t.workspace = k.workspace; t.workspace_bytes = k.workspace_bytes;
   r = sl_kv4_attention(&pool, &t, e->stream);
   if (r) kv4_failed(e, "sl_kv4_attention", r);
@@ -1024,6 +1047,7 @@ int sl_lane_create(const sl_engine* base, int max_m, int max_seq_len, sl_engine*
     if (max_seq_len > kv4->max_seq || max_m > kv4->max_rows) return SL_ERR_ARG;
     for (int i = 0; i < KV4_SEQS && seq < 0; ++i) if (!kv4->seq[i]) seq = i;
     if (seq < 0) return SL_ERR_TOO_LARGE;
+    const int r = kv4_reserve(*kv4, max_m); if (r) return r;
   }
   sl_engine* e = new sl_engine();
   *out = e;
@@ -1256,10 +1280,7 @@ void sl_destroy(sl_engine* e) {
   sl_engine* root = e->base_of;
   if (e->stream) (void)hipStreamSynchronize(e->stream);
   if (e->kv4) e->kv4->seq[e->kv4_seq] = nullptr;      // (its pages go back with the next plan)
-  if (e->kv4 && !root) {
-    if (e->kv4->workspace) (void)hipFree(e->kv4->workspace);
-    delete e->kv4;
-  }
+  if (!root) delete e->kv4;
   for (void* p : e->allocs) (void)hipFree(p);
   if (e->pinned) (void)hipHostFree(e->pinned);
   for (hipEvent_t ev : e->head_ev) (void)hipEventDestroy(ev);
@@ -1711,45 +1732,45 @@ int kv4_whole(sl_engine* e, int n, bool look) {
   kv4_begin(e, lens, look);
   return e->fault.empty() ? SL_OK : SL_ERR_DEVICE;
 }
-// Device memory for the span of a call.
-struct Temp {
-  void* p = nullptr;
-  ~Temp() { if (p) (void)hipFree(p); }
-};
+int kv4_rows_at_once(const Kv4Store& k) { return (int)std::min<int64_t>(k.workspace_bytes / (2 * SL_ATT_KV * SL_ATT_D * 2), 1 << 16); }
 int kv4_read_rows(sl_engine* e, const LayerDev& L, uint16_t* k, uint16_t* v) {
-  const int n = e->pos;
+  const int n = e->pos, most = kv4_rows_at_once(*e->kv4);
   if (n == 0 || (!k && !v)) return SL_OK;
   const size_t row = (size_t)SL_ATT_KV * SL_ATT_D * 2, head = SL_ATT_D * 2;
-  Temp t;                                               // (before the plan: no work stays behind a call that fails)
-  SL_TRY(e, hipMalloc(&t.p, 2 * n * row));
   int r = kv4_whole(e, n, true); if (r) return r;
-  uint8_t* dev[2] = {(uint8_t*)t.p, (uint8_t*)t.p + n * row};
-  const sl_kv4_pool pool = kv4_pool(*e->kv4, L);
-  r = sl_kv4_read(&pool, e->kv4->slot, n, SL_F16, dev[0], dev[1], e->stream);
-  if (r) { kv4_failed(e, "sl_kv4_read", r); return SL_ERR_DEVICE; }
+  uint8_t* dev[2] = {(uint8_t*)e->kv4->workspace, (uint8_t*)e->kv4->workspace + most * row};
+  const sl_kv4_pool pool = kv4_pool(*e->kv4, L.kv4);
   uint16_t* host[2] = {k, v};
-  for (int i = 0; i < 2; ++i)
-    for (int h = 0; h < SL_ATT_KV && host[i]; ++h)
-      SL_TRY(e, hipMemcpy2DAsync(host[i] + (size_t)h * n * SL_ATT_D, head, dev[i] + h * head, row, head, n, hipMemcpyDeviceToHost, e->stream));
+  for (int at = 0; at < n; at += most) {
+    const int some = std::min(most, n - at);
+    r = sl_kv4_read(&pool, e->kv4->slot + at, some, SL_F16, dev[0], dev[1], e->stream);
+    if (r) { kv4_failed(e, "sl_kv4_read", r); return SL_ERR_DEVICE; }
+    for (int i = 0; i < 2; ++i)
+      for (int h = 0; h < SL_ATT_KV && host[i]; ++h)
+        SL_TRY(e, hipMemcpy2DAsync(host[i] + ((size_t)h * n + at) * SL_ATT_D, head, dev[i] + h * head, row, head, some, hipMemcpyDeviceToHost, e->stream));
+  }
   SL_TRY(e, hipStreamSynchronize(e->stream));
   return SL_OK;
 }
 int kv4_load_rows(sl_engine* e, const LayerDev& L, const uint16_t* k, const uint16_t* v, int n) {
   if (n > 0 && (!k || !v)) return SL_ERR_ARG;           // (both are quantised together)
-  const size_t bytes = (size_t)SL_ATT_KV * n * SL_ATT_D * 2;
-  Temp t;
-  if (n > 0) SL_TRY(e, hipMalloc(&t.p, 2 * bytes));
   int r = kv4_whole(e, n, false); if (r) return r;
-  if (n == 0) return SL_OK;
-  uint16_t* dev[2] = {(uint16_t*)t.p, (uint16_t*)((uint8_t*)t.p + bytes)};
-  SL_TRY(e, hipMemcpyAsync(dev[0], k, bytes, hipMemcpyHostToDevice, e->stream));
-  SL_TRY(e, hipMemcpyAsync(dev[1], v, bytes, hipMemcpyHostToDevice, e->stream));
-  const sl_kv4_pool pool = kv4_pool(*e->kv4, L);
+  const int most = kv4_rows_at_once(*e->kv4);
+  const size_t head = (size_t)most * SL_ATT_D;
+  uint16_t* dev[2] = {(uint16_t*)e->kv4->workspace, (uint16_t*)e->kv4->workspace + SL_ATT_KV * head};
+  const uint16_t* host[2] = {k, v};
+  const sl_kv4_pool pool = kv4_pool(*e->kv4, L.kv4);
   sl_kv4_append_args a{};
-  a.n_tokens = n; a.dtype = SL_F16; a.k = dev[0]; a.v = dev[1]; a.slot = e->kv4->slot;
-  a.k_token = a.v_token = SL_ATT_D; a.k_head = a.v_head = (int64_t)n * SL_ATT_D;
-  r = sl_kv4_append(&pool, &a, e->stream);
-  if (r) { kv4_failed(e, "sl_kv4_append", r); return SL_ERR_DEVICE; }
+  a.dtype = SL_F16; a.k = dev[0]; a.v = dev[1];
+  a.k_token = a.v_token = SL_ATT_D; a.k_head = a.v_head = (int64_t)head;
+  for (int at = 0; at < n; at += most) {
+    a.n_tokens = std::min(most, n - at); a.slot = e->kv4->slot + at;
+    for (int i = 0; i < 2; ++i)
+      for (int h = 0; h < SL_ATT_KV; ++h)
+        SL_TRY(e, hipMemcpyAsync(dev[i] + h * head, host[i] + ((size_t)h * n + at) * SL_ATT_D, (size_t)a.n_tokens * SL_ATT_D * 2, hipMemcpyHostToDevice, e->stream));
+    r = sl_kv4_append(&pool, &a, e->stream);
+    if (r) { kv4_failed(e, "sl_kv4_append", r); return SL_ERR_DEVICE; }
+  }
   SL_TRY(e, hipStreamSynchronize(e->stream));
   return SL_OK;
 }
@@ -1786,7 +1807,7 @@ int sl_set_kv4(sl_engine* e, int page_size, int n_pages) {
   std::vector<void*> pages(e->n_layers, nullptr);
   for (int i = 0; i < e->n_layers && got; ++i)
     if (!e->layers[i].is_linear) got = (pages[i] = get((size_t)n_pages * page_bytes)) != nullptr;
-  if (!got) {
+  if (!got || kv4_reserve(*k, e->max_m) != SL_OK) {
     for (void* p : mem) (void)hipFree(p);
     return SL_ERR_TOO_LARGE;
   }

@@ -123,3 +123,49 @@ def test_reading_a_cache_changes_nothing(hybrid_model):  # noqa: F811
     assert e.full_restore(late) and e.position == 64 and e.kv4_free_pages() == free
     assert int(e.step_argmax([7])[0]) == want
     e.close()
+
+
+@pytest.mark.parametrize("hybrid", [False, True])
+def test_steps_and_cache_calls_take_no_memory(hybrid_model, hybrid):  # noqa: F811
+    """All that they need is there once the engine and its lanes are: a device that fills up later ends no step.  (The first of two
+    engines goes the same way before, so that what the runtime takes for a kernel's first launch has been taken.)"""
+    from . import kv4_ref as ref
+    cfg, dev = hybrid_model
+    for first in (True, False):
+        e = make(cfg, dev, page_size=64, n_pages=80, max_m=64, max_seq_len=2048)
+        e.set_hybrid(hybrid)
+        lanes = [e.new_lane(max_m=512 if i == 0 else 16, max_seq_len=2048) for i in range(3)]
+        lanes[0].set_hybrid(hybrid)
+        rng = np.random.default_rng(54)
+        torch.cuda.synchronize()
+        free = torch.cuda.mem_get_info()[0]
+        kept = [(e, rng.normal(size=(2, 700, 256)).astype(np.float16)), (lanes[1], rng.normal(size=(2, 1025, 256)).astype(np.float16))]
+        for x, rows in kept:
+            assert x.load_layer_cache(3, rows, rows[:, ::-1])
+        assert e.step_argmax([1] * 64) is not None and e.chained_step_argmax(3, 4) is not None and e.step_argmax([2] * 7) is not None
+        for n in (512, 1, 300, 5):
+            assert lanes[0].forward_tokens([4] * n, on_device=True)
+        assert e.lane_step_argmax(lanes[::-1], [1, 2, 3]) is not None
+        for x, rows in kept:
+            k, v = x.read_layer_cache(3)
+            n = rows.shape[1]
+            for got, y in ((k, rows), (v, rows[:, ::-1])):
+                assert np.array_equal(got[:, :n], ref.values(ref.quantise(y.astype(np.float64))).astype(np.float32).astype(np.float16))
+        torch.cuda.synchronize()
+        assert first or torch.cuda.mem_get_info()[0] == free
+        for x in lanes:
+            x.close()
+        e.close()
+
+
+def test_long_caches_are_loaded_and_read_in_pieces(hybrid_model):  # noqa: F811
+    """More rows than are on their way at once (a few thousand on an engine of single rows)."""
+    from . import kv4_ref as ref
+    cfg, dev = hybrid_model
+    e = make(cfg, dev, page_size=128, max_m=1, max_seq_len=20000)
+    rng = np.random.default_rng(55)
+    k, v = (rng.normal(size=(2, 19999, 256)).astype(np.float16) for _ in range(2))
+    assert e.load_layer_cache(3, k, v) and e.position == 19999
+    for got, x in zip(e.read_layer_cache(3), (k, v)):
+        assert np.array_equal(got, ref.values(ref.quantise(x.astype(np.float64))).astype(np.float32).astype(np.float16))
+    e.close()
