@@ -392,7 +392,9 @@ int sl_set_hybrid(sl_engine* e, int enable);
  * engine are freed.  To be called once, on a new engine (not a lane) before its first token and its first lane; at most 63 lanes, with
  * max_seq_len and max_m up to the engine's max_seq_len (or its max_m, if that is larger).
  * A call for which the pages do not suffice returns SL_ERR_TOO_LARGE and changes nothing; pages return when a sequence
- * is rolled back, reset or destroyed, with the next step of any of them.  Steps and the calls that read or load a cache take no device
+ * is rolled back, reset or destroyed, with the next step of any of them.  sl_greedy_generate and sl_spec_generate ask for the pages
+ * of their whole run first (the drafts and chains of the latter need a few more rows for a while, as they need them of max_seq_len:
+ * where those do not suffice it ends after a part of its run).  Steps and the calls that read or load a cache take no device
  * memory: this call and sl_lane_create make room for all rows of a call (for up to 512 rows 85 MB, 2048 245, 8192 350, 32768 1100).
  * Steps then run kernel by kernel (sl_set_persistent has no effect), with the operators below in the attention layers
  * and the same arithmetic everywhere else.  Results are no longer bit-identical to the oracle; they are deterministic, and a

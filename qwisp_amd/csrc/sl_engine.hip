@@ -2001,6 +2001,7 @@ int sl_greedy_generate(sl_engine* e, const int32_t* prompt, int n_prompt, int n_
   if (!prompt || n_prompt < 1 || n_new < 0 || (n_new > 0 && !out) || !e->has_head) return SL_ERR_ARG;
   if (chain_k < 1) chain_k = 1;
   if (chain_k > MAX_CHAIN) chain_k = MAX_CHAIN;
+  if (n_prompt > INT32_MAX - n_new || !kv4_room(e, n_prompt + std::max(n_new - 1, 0))) return SL_ERR_TOO_LARGE;
   int done = 0, last_m = 0;
   while (done < n_prompt) {                    // the rows of a chunk stay on the device: only the last row of the last chunk is used
     last_m = n_prompt - done < e->max_m ? n_prompt - done : e->max_m;

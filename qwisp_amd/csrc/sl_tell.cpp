@@ -258,6 +258,12 @@ extern "C" int sl_spec_generate(sl_engine* e, const int32_t* prompt, int n_promp
   if (!e) return SL_ERR_ARG;
   const int max_rows = sl_max_rows(e);
   if (max_rows < 1) return SL_ERR_ARG;
+  int32_t page = 0;
+  const int left = sl_kv4_free_pages(e, &page, nullptr);
+  if (left >= 0 && n_prompt > 0 && n_new >= 0) {           // 4-bit caches: pages for all tokens of the run, before its first step
+    const long pos = sl_position(e), end = pos + n_prompt + (n_new > 0 ? n_new - 1 : 0);
+    if ((end + page - 1) / page - (pos + page - 1) / page > left) return SL_ERR_TOO_LARGE;
+  }
   EngineCtx x{e, {}, 1};
   sl_spec_backend b;
   b.ctx = &x; b.max_rows = max_rows;

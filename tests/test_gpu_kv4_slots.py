@@ -169,3 +169,13 @@ def test_long_caches_are_loaded_and_read_in_pieces(hybrid_model):  # noqa: F811
     for got, x in zip(e.read_layer_cache(3), (k, v)):
         assert np.array_equal(got, ref.values(ref.quantise(x.astype(np.float64))).astype(np.float32).astype(np.float16))
     e.close()
+
+
+def test_a_run_that_does_not_fit_changes_nothing(hybrid_model):  # noqa: F811
+    cfg, dev = hybrid_model
+    e = make(cfg, dev, page_size=16, n_pages=4, max_m=8, max_seq_len=128)
+    assert e.greedy_generate([5] * 60, 6) is None and e.gpu_fault is None
+    assert e.position == 0 and e.kv4_free_pages() == 4
+    assert e.spec_generate([5] * 60, 6) is None and e.position == 0 and e.kv4_free_pages() == 4
+    assert e.greedy_generate([5] * 60, 5) is not None and e.position == 64
+    e.close()
