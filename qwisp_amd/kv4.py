@@ -8,7 +8,8 @@ what each computes, refuses and leaves alone.
 
 torch only owns the memory.  Calls enqueue on torch's current stream of the tensors' device and return without waiting;
 they can be captured into a graph.  A call that the library refuses raises SeedlessError, a tensor of the wrong kind
-ValueError; nothing is copied or converted on the way.
+ValueError; nothing is copied or converted on the way.  The operators have no gradients: a tensor that asks for one is refused
+outside torch.no_grad().
 """
 import ctypes as C
 from typing import NamedTuple
@@ -71,7 +72,13 @@ def _flat(t, shape, dtype, device, what):
         raise ValueError(f"{what}: a tensor is wanted")
     if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: {dtype} {list(shape)} side by side on {device} is wanted, got {t.dtype} {list(t.shape)} on {t.device}")
+    _no_grad(t, what)
     return t.data_ptr()
+
+
+def _no_grad(t, what):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, and the operators on the 4-bit cache have none: detach it, or call under torch.no_grad()")
 
 
 def _rows(t, shape, dtype, device, what):
@@ -82,6 +89,7 @@ def _rows(t, shape, dtype, device, what):
     if t.dtype is not dtype or t.shape != shape or t.device != device or dim != 1:
         raise ValueError(f"{what}: {dtype} {list(shape)} with dims side by side on {device} is wanted, got {t.dtype} {list(t.shape)} "
                          f"with strides {t.stride()} on {t.device}")
+    _no_grad(t, what)
     return t.data_ptr(), token if shape[0] > 1 else 0, head if shape[1] > 1 else 0
 
 

@@ -212,3 +212,30 @@ def test_scores_beyond_what_fp32_tells_apart_choose_the_largest(dim, heads, kv, 
                 want, e = vv[at[s.argmax()], g], 2 * H * (np.abs(vv[at[s.argmax()], g]) + 8 * np.abs(np.repeat(parts["v"]["scale"][at[s.argmax()], g], 64)))
                 assert (np.abs(have[start[r] + i, h] - want) <= e + HALF_STEP[dtype] * np.abs(want) + 2.0 ** -25).all()
     assert used > 0
+
+
+# ---- arguments --------------------------------------------------------------------------------------------------------------
+def small_calls():
+    """Calls that work, by keyword."""
+    m = kv4()
+    pool = m.new_pool(2, 16, 1, 64)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    half = dict(dtype=torch.float16, device="cuda")
+    q, one, two = torch.zeros(2, 1, 64, **half), torch.zeros(1, **i32), torch.arange(2, **i32)
+    cos, sin = m.rope_tables(4, 16)
+    plan = dict(ctx_len=one, new_len=one + 2, table=torch.full((1, 2), -1, **i32), held=one.clone(), free=two, free_count=one + 2, page_size=16, max_tokens=2)
+    append = dict(pool=pool, q=q, k=q + 1, v=q + 2, slot=two, pos=two, cos=cos, sin=sin, q_weight=torch.ones(64, **half), k_weight=torch.ones(64, **half))
+    attention = dict(pool=pool, q=q, table=torch.zeros(1, 1, **i32), q_start=one.new_tensor([0, 2]), kv_len=one + 2, max_rows=2, max_keys=2, gate=q + 1)
+    return m, dict(plan=plan, append=append, attention=attention, read=dict(pool=pool, slots=two))
+
+
+@pytest.mark.parametrize("name, arg", [("append", x) for x in ("q", "k", "v", "cos", "sin", "q_weight", "k_weight")] + [("attention", "q"), ("attention", "gate")])
+def test_tensors_that_ask_for_gradients_are_refused(name, arg):
+    m, calls = small_calls()
+    args = calls[name]
+    want = getattr(m, name)(**args)
+    args = {**args, arg: args[arg].clone().requires_grad_()}
+    with pytest.raises(ValueError, match=arg):
+        getattr(m, name)(**args)
+    with torch.no_grad():
+        assert torch.equal(getattr(m, name)(**args), want)
