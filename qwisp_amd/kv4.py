@@ -76,6 +76,12 @@ def _flat(t, shape, dtype, device, what):
     return t.data_ptr()
 
 
+def _tensors(**named):
+    for what, t in named.items():
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: a tensor is wanted")
+
+
 def _no_grad(t, what):
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires a gradient, and the operators on the 4-bit cache have none: detach it, or call under torch.no_grad()")
@@ -95,6 +101,7 @@ def _rows(t, shape, dtype, device, what):
 
 def _pool(pool):
     p, page_size, n_kv, head_dim = pool
+    _tensors(pages=p)
     n = page_bytes(page_size, n_kv, head_dim)
     if p.dtype is not torch.uint8 or not p.is_cuda or p.dim() != 2 or p.shape[1] != n or not p.is_contiguous():
         raise ValueError(f"pages: uint8 [n_pages, {n}] side by side on a GPU is wanted, got {p.dtype} {list(p.shape)} on {p.device}")
@@ -124,6 +131,7 @@ def _call(name, device, *args):
 def plan(ctx_len, new_len, table, held, free, free_count, page_size, max_tokens, out=None):
     """sl_kv4_plan: page tables, slots and row offsets of one step from the requests' lengths (int32 tensors).  `out`: a
     Plan whose tensors are written, none of which may be an input; without it they come as parts of one new tensor."""
+    _tensors(ctx_len=ctx_len, table=table, free=free)
     dev, i32 = ctx_len.device, torch.int32
     if not ctx_len.is_cuda or ctx_len.dim() != 1 or table.dim() != 2 or free.dim() != 1 or max_tokens < 0:
         raise ValueError("lengths [n_req], table [n_req, width] and free [n_free] on a GPU are wanted")
@@ -150,6 +158,7 @@ def append(pool, q, k, v, slot, pos, cos, sin, q_weight, k_weight, eps=1e-6, out
     """sl_kv4_append: queries normed and rotated are returned, keys normed and rotated and values go into the pool.  q None:
     keys and values only; cos and sin None: no rotation; a weight None: no norm."""
     p, dev = _pool(pool), pool.pages.device
+    _tensors(k=k)
     if k.dtype not in _DTYPES or k.dim() != 3:
         raise ValueError(f"keys [tokens, heads, dims] in float16 or bfloat16 are wanted, got {k.dtype} {list(k.shape)}")
     dt, n, dim = k.dtype, k.shape[0], pool.head_dim
@@ -158,6 +167,7 @@ def append(pool, q, k, v, slot, pos, cos, sin, q_weight, k_weight, eps=1e-6, out
     heads = max_pos = rot = 0
     cos_at = sin_at = pos_at = qw_at = kw_at = None
     if q is not None:
+        _tensors(q=q)
         heads = q.shape[1] if q.dim() == 3 else 0
         shape = (n, heads, dim)
         if out is None:
@@ -167,7 +177,7 @@ def append(pool, q, k, v, slot, pos, cos, sin, q_weight, k_weight, eps=1e-6, out
             qw_at = _flat(q_weight, (dim,), dt, dev, "q_weight")
     if k_weight is not None:
         kw_at = _flat(k_weight, (dim,), dt, dev, "k_weight")
-    if (cos is None) != (sin is None) or (cos is not None and cos.dim() != 2):
+    if (cos is None) != (sin is None) or (cos is not None and not (isinstance(cos, torch.Tensor) and cos.dim() == 2)):
         raise ValueError("cos and sin [positions, rotated dims / 2] are wanted, or neither")
     if cos is not None:
         max_pos, rot = cos.shape[0], 2 * cos.shape[1]
@@ -191,6 +201,7 @@ def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, g
     attention_workspace() bytes) is taken from torch if it is not given.  Rows that no request has are not written: in
     a new `out` they hold whatever the memory held."""
     p, dev = _pool(pool), pool.pages.device
+    _tensors(q=q, table=table)
     if q.dtype not in _DTYPES or q.dim() != 3 or table.dim() != 2:
         raise ValueError(f"queries [tokens, heads, dims] in float16 or bfloat16 and a table [n_req, width] are wanted, got {q.dtype} {list(q.shape)}, {list(table.shape)}")
     n, heads, n_req, dim = q.shape[0], q.shape[1], table.shape[0], pool.head_dim
@@ -209,7 +220,7 @@ def attention(pool, q, table, q_start, kv_len, max_rows, max_keys, scale=None, g
     if need > 0:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        elif workspace.dtype is not torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+        elif not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
             raise ValueError("workspace: uint8 side by side on the pool's device is wanted")
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
     _call("sl_kv4_attention", dev, p, a)
@@ -225,6 +236,7 @@ def attention_workspace(pool, n_tokens, n_heads, n_req, table_width, max_rows, m
 def read(pool, slots, dtype=torch.float32):
     """sl_kv4_read: keys and values [n, n_kv, head_dim] (float32 or float16) of the given slots."""
     p, dev = _pool(pool), pool.pages.device
+    _tensors(slots=slots)
     if slots.dim() != 1 or dtype not in (torch.float32, torch.float16):
         raise ValueError("slots [n] and float32 or float16 values are wanted")
     n = slots.shape[0]

@@ -239,3 +239,20 @@ def test_tensors_that_ask_for_gradients_are_refused(name, arg):
         getattr(m, name)(**args)
     with torch.no_grad():
         assert torch.equal(getattr(m, name)(**args), want)
+
+
+def test_what_is_no_tensor_is_refused():
+    m, calls = small_calls()
+    for name, args in calls.items():
+        for arg, t in args.items():
+            if not isinstance(t, torch.Tensor):
+                continue
+            for bad in (None, [1, 2]):
+                if bad is None and (name, arg) in (("append", "q"), ("append", "q_weight"), ("append", "k_weight"), ("attention", "gate")):
+                    continue                                 # (may be left out)
+                with pytest.raises(ValueError, match=arg):
+                    getattr(m, name)(**{**args, arg: bad})
+    with pytest.raises(ValueError, match="pages"):
+        m.read(m.Pool(None, 16, 1, 64), calls["read"]["slots"])
+    with pytest.raises(ValueError, match="workspace"):
+        m.attention(**{**calls["attention"], "workspace": [1]})
