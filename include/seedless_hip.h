@@ -525,7 +525,7 @@ int sl_kv4_append(const sl_kv4_pool* pool, const sl_kv4_append_args* a, void* st
  * Rows q_start[r] .. q_start[r+1] - 1 are request r's last tokens: row i of n sees keys 0 .. kv_len[r] - n + i.  A row
  * that sees no key is zeros; rows behind q_start[n_req], and rows of a request from max_rows on, are left as they
  * were.  Keys whose page id lies outside the pool are not there (as if masked); what masked places hold never matters.
- * Scores, softmax statistics and sums are fp32, the result is rounded once.  max_rows: the most rows of one request;
+ * scale is finite.  Scores, softmax statistics and sums are fp32, the result is rounded once.  max_rows: the most rows of one request;
  * max_keys: about how many keys the longest request has, by which long axes are split (any value >= 1 gives right
  * results).  The same inputs give the same bits; how long axes are cut depends on all lengths of the call, so a request's
  * last bits may differ between batches. */

@@ -150,3 +150,8 @@ def test_sizes_beyond_a_launch_are_refused():
     assert dll.sl_kv4_attention(pool(), attn(n_tokens=1 << 24, max_rows=1 << 24), None) == abi.SL_ERR_TOO_LARGE
     assert dll.sl_kv4_attention(pool(n_kv=2), attn(n_tokens=1 << 22, max_rows=1 << 22, n_heads=16, n_req=4096), None) == abi.SL_ERR_TOO_LARGE
     assert dll.sl_kv4_attention(pool(), attn(n_req=4097), None) == abi.SL_ERR_TOO_LARGE
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_attention_refuses_a_scale_that_is_not_finite(scale):
+    assert lib.get().dll.sl_kv4_attention(pool(), attn(scale=scale), None) == abi.SL_ERR_ARG
