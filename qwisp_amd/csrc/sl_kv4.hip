@@ -1242,7 +1242,7 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
         wave_lds_order();
         const ValueUnit<D> was = unit;
         const BadValues<D> bad = put_scales<D>(cur.sb, cur.there, st, unit);
-        if (unit != was) change_unit<D, NT>(was, unit, o, ob);
+        if (unit != was && k0 != key0 + wave * AT_STEP) change_unit<D, NT>(was, unit, o, ob);      // (no sums yet in the first step)
         // values: the piece of 4 dims that belongs to lane m' of group g, 8 keys together
 #pragma unroll
         for (int c = 0; c < G; ++c) {
@@ -1477,7 +1477,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attn_tile(Pool pool, sl_kv4_attn
     ValueUnit<D> now = s_note[buf].unit;
 #pragma unroll
     for (uint32_t& f : now.f) f = __builtin_amdgcn_readfirstlane(f);
-    if (now != unit) { change_unit<D, NT>(unit, now, o, ob); unit = now; }
+    if (now != unit) { if (i > 0) change_unit<D, NT>(unit, now, o, ob); unit = now; }              // (no sums yet in the first step)
     float s[NT][8];
     step_scores<D, NT>(k, [&](int nt, int w) { return __builtin_bit_cast(h8, s_q[(wave * (D / 32) + w) * 64 + lane]); }, qs, st, s);
     uint32_t pw[NT][G + 1][4];
