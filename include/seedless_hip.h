@@ -350,8 +350,9 @@ int sl_sched_round(sl_sched* s);
  * all that have begun may grow to: can_admit says so (and changes nothing), and admit_step of a request for which they do not yet returns 1
  * with nothing consumed; later requests do not begin in front of it.  A request ends like one whose prompt fails if it needs more
  * pages than there are, or than sequences beside the slots (the base's own, other lanes) leave while no slot is in use.  Without
- * a budget (kv_budget_tokens <= 0) the pages have to hold every slot at max_seq_len, else SL_ERR_TOO_LARGE.  (A scheduler without a
- * token budget names no length: there a request that finds no pages ends, as any whose prompt fails.) */
+ * a budget (kv_budget_tokens <= 0) the pages have to hold every slot at max_seq_len, else SL_ERR_TOO_LARGE.  (Sequences beside the
+ * slots that grow meanwhile take pages without asking: a prompt that finds none ends, a decode step returns SL_ERR_TOO_LARGE and can be tried again.
+ * A scheduler without a token budget names no length: there a request that finds no pages ends, as any whose prompt fails.) */
 typedef struct sl_lane_slots sl_lane_slots;
 int sl_lane_slots_create(const sl_engine* base, int n_slots, int chunk_rows, int max_seq_len, long kv_budget_tokens,
                          sl_lane_slots** out, sl_batch_slots* table);
@@ -525,7 +526,10 @@ int sl_kv4_append(const sl_kv4_pool* pool, const sl_kv4_append_args* a, void* st
  * Rows q_start[r] .. q_start[r+1] - 1 are request r's last tokens: row i of n sees keys 0 .. kv_len[r] - n + i.  A row
  * that sees no key is zeros; rows behind q_start[n_req], and rows of a request from max_rows on, are left as they
  * were.  Keys whose page id lies outside the pool are not there (as if masked); what masked places hold never matters.
- * scale is finite.  Scores, softmax statistics and sums are fp32, the result is rounded once.  max_rows: the most rows of one request;
+ * scale is finite.  A value group that is not finite makes its own dims of the rows that see it NaN, a key or query that is not finite whole rows.
+ * Scores, maxima and sums are fp32.  Weights meet the values as fp16 operands (p s, p and b + 8 s, by half a step of 2^-11 each) in units that keep those
+ * 11 bits for weights down to 2^-20 of a row's largest, whatever the values' size; the softmax's sum is that of the rounded weights; the result is rounded
+ * once.  max_rows: the most rows of one request;
  * max_keys: about how many keys the longest request has, by which long axes are split (any value >= 1 gives right
  * results).  The same inputs give the same bits; how long axes are cut depends on all lengths of the call, so a request's
  * last bits may differ between batches. */

@@ -491,11 +491,12 @@ __global__ __launch_bounds__(256) void k_kv4_read(Pool pool, const int32_t* slot
 // 16 * NT query rows (row = token * group + head within the group):
 //   S[key, row] = sum over groups of 64 dims of  s_g * (sum q c) + b_g * (sum q)      c = code
 //   O[dim, row] += sum over keys of  (p s_g) * (c - 8)  +  p * (b_g + 8 s_g)
-// Codes become fp16 operands without rounding: for the keys a masked nibble IS the fp16 number c * 2^-24 (or c * 2^-20 four
-// bits up, which the query's operand makes good), for the values c - 8 is formed through 1024 + c.  So the scales meet
-// fp32 scores, and the weights p s_g are the only operands that are rounded (11 bits); centred codes keep
-// that rounding at the size of a value's own spread.  Queries become fp16 after a power of two per row that puts the largest
-// near 2^10: exact for both element types but for dims 2^-20 below the row's largest.
+// Codes become fp16 operands without rounding: a masked nibble IS the fp16 number c * 2^-24 (or c * 2^-20 four bits up; the
+// query's operand makes that good for the keys, the last step for the values).  So the scales meet fp32 scores.  Rounded to fp16 on the
+// way, by half a step of 2^-11 each, are the operands p s_g, p and b_g + 8 s_g of the second line, and the softmax's sum is that of
+// the rounded p, so that weights stay in proportion; the first meets c - 8 (the sums take the 8 off), which keeps its rounding at the size of a
+// value's own spread.  Everything else, scores, maxima and sums, is fp32.  Queries become fp16 after a power of two per row that
+// puts the largest near 2^10: exact for both element types but for dims 2^-20 below the row's largest.
 // Layouts: S comes out with a lane holding 8 consecutive keys of one row, which is how the second product wants p, because
 // row m of the two key operands is key 8 (m / 4) + m % 4 (+ 4).  Values are stored as a lane loads them (8 keys x D/16
 // dims) and change lanes through LDS on their way, so that the 16 rows of an operand lie in one group and share p s_g.
@@ -719,11 +720,12 @@ struct BadValues {
 };
 // Weights meet the values as fp16 operands, p s and p, which have 11 bits from 2^-14 to 2^16 and lose them below.  So both are taken in units:
 // p is formed 2^6 times too large (a row's output is a quotient, from which that falls out), and the value scales of a group are taken times a power of
-// two that brings the largest near 2^6.  It only falls while a wave goes along its keys, and its sums with it; below 1 it
+// two, 2^15 at most, that brings the largest near 2^6.  It only falls while a wave goes along its keys, and its sums with it; below 1 it
 // stands where scales beyond 128 (values beyond some 1000) are met, and only then can a scale 2^21 below the largest lose bits.
 // p keeps its 11 bits down to 2^-20 and p s down to 2^-25 of the largest s; they are there down to 2^-31 and 2^-36.  One key 13 above 4095
 // others, values of 0.02: rows in bf16 are off by 1.6e-3 of their size, which is that type's own rounding (without units 6e-3 with
-// 64 dims, 2.3e-2 in tiles of 64 rows); values of 1e-5: 1.5e-3 (4.7e-2).  Some ten instructions a step: 32 lanes of 256 dims 1.4 us of 38, a prompt 5 of 140.
+// 64 dims, 2.3e-2 in tiles of 64 rows); values of 1e-5: 1.5e-3 (4.7e-2).  Some ten instructions a step and the first step's maximum: with
+// what else keeps numbers that are not finite and large scores right, one token at 4K 0.6 us of 18, 32 lanes of 256 dims 1.2 of 43, a prompt 3.5 of 143.
 constexpr float P_UNIT_LOG2 = 6.0f;
 constexpr uint32_t UNIT_TOP = 0x58005800u;          // 128 as halves: p reaches 2^8.875, p s then 2^15.875
 template <int D>
@@ -1116,10 +1118,10 @@ SL_DEV void put_row(const sl_kv4_attn_args& a, const AttnCut& cut, long slot, in
   }
 }
 
-// Up to 16 (NT = 1) or 32 rows a workgroup.  What bounds it: one token at 4K 9.5 us, start and end (lengths, table, page, queries, the
-// join in LDS) with one round of keys between; 32 lanes at 1K-16K 33 us, the same 9 us and 107 MB at 4.5 TB/s; six requests
-// of 3-5 rows at 20-32K, 128 dims, 49 us, 187 MB, vector instructions in 67 % of the slots; 2333 rows behind 4-16K, 64 dims,
-// 189 us, 92 % of the slots (unpacking 1/2, softmax and weights 1/2; the matrix cores are busy 21 %).
+// Up to 16 (NT = 1) or 32 rows a workgroup.  What bounds it: one token at 4K 10.9 us, start and end (lengths, table, page, queries, the
+// join in LDS) with one round of keys between; 32 lanes at 1K-16K 34 us, the same 10 us and 107 MB at 4.5 TB/s; six requests
+// of 3-5 rows at 20-32K, 128 dims, 51 us, 187 MB, vector instructions in 68 % of the slots; 2333 rows behind 4-16K, 64 dims,
+// 185 us, 90 % of the slots (unpacking 1/2, softmax and weights 1/2; the matrix cores are busy 22 %).
 // Workgroups on a compute unit: by the registers, of which the running sums alone take NT * D / 4.
 constexpr int attn_places(int dim, int nt) { return dim == 64 ? (nt == 1 ? 4 : 3) : (dim == 128 && nt == 1 ? 3 : 2); }
 template <int D, bool BF, int NT>
@@ -1317,8 +1319,8 @@ __global__ __launch_bounds__(256, attn_places(D, NT)) void k_kv4_attn(Pool pool,
 // waves a SIMD).  The waves lay a step's bytes out in LDS together, a step ahead of its use, so the registers hold no bytes but
 // those on their way.  (With fewer dims a wave has room for 32 rows, and waves that unpack their own keys are faster than
 // ones that meet at a barrier every step: 64 rows of 128 dims against 32K keys 121 us, with this kernel's scheme 190.)
-// A prompt of 2048 rows and 16 heads 141 us, 245 TFLOP/s: 512 workgroups, two to a unit, and the last row tile's 64 steps of 2.2 us
-// are its length; 512 rows behind 8K 176 us, 400 TFLOP/s.
+// A prompt of 2048 rows and 16 heads 144 us, 239 TFLOP/s: 512 workgroups, two to a unit, and the last row tile's 64 steps of 2.2 us
+// are its length; 512 rows behind 8K 180 us, 395 TFLOP/s.
 template <int D>
 struct TileLds {
   static constexpr int KEYS = 16 * D;                                  // key words in the order of the lanes
