@@ -351,8 +351,8 @@ int sl_sched_round(sl_sched* s);
  * with nothing consumed; later requests do not begin in front of it.  A request ends like one whose prompt fails if it needs more
  * pages than there are, or than sequences beside the slots (the base's own, other lanes) leave while no slot is in use.  Without
  * a budget (kv_budget_tokens <= 0) the pages have to hold every slot at max_seq_len, else SL_ERR_TOO_LARGE.  (Sequences beside the
- * slots that grow meanwhile take pages without asking: a prompt that finds none ends, a decode step returns SL_ERR_TOO_LARGE and can be tried again.
- * A scheduler without a token budget names no length: there a request that finds no pages ends, as any whose prompt fails.) */
+ * slots that grow meanwhile take pages without asking, and a scheduler without a token budget names no lengths: a prompt that then finds
+ * no pages ends, and a decode step returns SL_ERR_TOO_LARGE until some come free.) */
 typedef struct sl_lane_slots sl_lane_slots;
 int sl_lane_slots_create(const sl_engine* base, int n_slots, int chunk_rows, int max_seq_len, long kv_budget_tokens,
                          sl_lane_slots** out, sl_batch_slots* table);

@@ -1754,7 +1754,7 @@ int sl_kv4_attention(const sl_kv4_pool* p, const sl_kv4_attn_args* a, void* stre
   Pool pool;
   int r = pool_of(p, pool); if (r) return r;
   if (!a || a->n_req < 0 || a->n_tokens < 0 || a->table_width < 0 || (a->dtype != SL_F16 && a->dtype != SL_BF16)) return SL_ERR_ARG;
-  if (a->n_heads < 1 || a->n_heads % p->n_kv || a->max_rows < 0 || a->max_keys < 1 || !(std::fabs(a->scale) <= 3.4028234e38f)) return SL_ERR_ARG;
+  if (a->n_heads < 1 || a->n_heads % p->n_kv || a->max_rows < 0 || a->max_keys < 1 || !std::isfinite(a->scale)) return SL_ERR_ARG;
   if (a->n_req == 0 || a->n_tokens == 0 || a->max_rows == 0) return SL_OK;
   if (!a->q || !a->out || !a->q_start || !a->kv_len || (!a->table && a->table_width > 0)) return SL_ERR_ARG;
   const void* sixteen[] = {a->q, a->gate, a->out};
