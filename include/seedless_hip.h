@@ -504,7 +504,7 @@ typedef struct {
 } sl_kv4_plan_args;
 int sl_kv4_plan(const sl_kv4_plan_args* a, void* stream);
 
-/* Norm of queries and keys per head (x / sqrt(mean(x^2) + eps) * weight; a NULL weight leaves that norm out), rotation of
+/* Norm of queries and keys per head (x * rsqrt(mean(x^2) + eps) * weight; a NULL weight leaves that norm out), rotation of
  * the pairs (i, i + rot_dim/2) of the first rot_dim dims by the angle tables' row of the token's position, queries to
  * q_out, keys and the values as they are into the cache at `slot`.  Queries are computed in fp32 and rounded once, keys
  * in double precision up to their codes.  A token whose slot is outside the pool stores nothing (its query row is

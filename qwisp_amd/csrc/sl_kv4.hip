@@ -258,11 +258,9 @@ SL_DEV double sum_lanes(double v) {
 template <int LANES>
 SL_DEV float sum_lanes(float v) { return tree_sum<LANES>(v); }
 SL_DEV float inv_sqrt(float x) { return __builtin_amdgcn_rsqf(x); }
-SL_DEV double inv_sqrt(double x) {                    // the instruction's estimate and two Newton steps: within 2^-51
-  double y = __builtin_amdgcn_rsq(x);
-  y = y * fma(-0.5 * x * y, y, 1.5);
-  return y * fma(-0.5 * x * y, y, 1.5);
-}
+// (Not a shorter form: where a group's largest is the opposite of its smallest, the last bit decides between 7 and 8 steps.  An estimate with two
+// Newton steps, within 2^-51, gave 1-2 % of such rows another scale than x * rsqrt(mean + eps) * weight in doubles has, at the same speed.)
+SL_DEV double inv_sqrt(double x) { return rsqrt(x); }
 
 // What a lane needs of a token beside its row: four weights, four cosines and sines, and from which lane the other half comes.
 struct Turn {

@@ -214,6 +214,31 @@ def test_scores_beyond_what_fp32_tells_apart_choose_the_largest(dim, heads, kv, 
     assert used > 0
 
 
+# ---- keys whose group lies on the border of two scales ----------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_normed_keys_between_two_counts_of_steps(dim, dtype):
+    """A group whose largest is the opposite of its smallest lies 7.5 steps from its edge, and the last bit of the norm's factor decides
+    between 7 and 8: it has to be that of x * rsqrt(mean + eps) * weight in double precision, as torch has it.  The squares and
+    their sum are exact here."""
+    m, rng = kv4(), np.random.default_rng(46)
+    n, page = 4096, 64
+    x = rng.integers(-40, 41, (n, 1, dim)) / 16.0
+    edge = rng.integers(41, 64, (n, 1, dim // 64)) / 16.0
+    w = 1 + 0.1 * rng.normal(size=dim)
+    for g in range(dim // 64):
+        x[:, :, 64 * g + 7], x[:, :, 64 * g + 50] = edge[:, :, g], -edge[:, :, g]
+        w[64 * g + 7] = w[64 * g + 50] = 1.5
+    k, w = gpu(x, DTYPES[dtype]), gpu(np.clip(w, 0.5, 1.5), DTYPES[dtype])
+    pool = m.new_pool(n // page, page, 1, dim)
+    m.append(pool, None, k, k, gpu(np.arange(n, dtype=np.int32)), None, None, None, None, w)
+    y = k.double() * torch.rsqrt((k.double() * k.double()).mean(-1, keepdim=True) + 1e-6) * w.double()
+    have, want = ref.unpack(pool.pages.cpu().numpy(), page, 1, dim)["k"], ref.quantise(y.cpu().numpy())
+    other = (have["scale"] != want["scale"]).any(-1).sum()
+    assert other == 0, f"{other} of {n} rows have another scale"
+    assert np.array_equal(have["bias"], want["bias"]) and np.array_equal(have["codes"], want["codes"])
+
+
 # ---- arguments --------------------------------------------------------------------------------------------------------------
 def small_calls():
     """Calls that work, by keyword."""
